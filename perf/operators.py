@@ -263,11 +263,22 @@ def backend():
     return BACKEND[0]
 
 
+class Memory:
+    """A buffer of the handle, and what torch reads it through: it lives as long as a tensor over it does."""
+
+    def __init__(self, size):
+        self.buffer = backend().create(size)
+        self.__cuda_array_interface__ = {"shape": (size,), "typestr": "|u1", "data": (self.buffer.device_ptr, False), "version": 2}
+
+    def __del__(self):
+        backend().release(self.buffer)
+
+
 class Plan:
     """A state's buffers on the handle and its recorded operators; torch sees the buffers without a copy."""
 
     def __init__(self, state):
-        self.held = []
+        self.memory = {}  # of each buffer
         self.graph = None
         b = backend()
         case = state["case"]
@@ -311,15 +322,15 @@ class Plan:
             self.record(lambda: b.kv_read(cache, shape, spans, s, t, keys, h * w, values, h * w, out_dtype=case["dtype"]))
 
     def buffer(self, size):
-        self.held.append(backend().create(size))
-        return self.held[-1]
+        memory = Memory(size)
+        self.memory[memory.buffer.id] = memory
+        return memory.buffer
 
     def new(self, shape):
         return self.buffer(4 * math.prod(shape))
 
     def view(self, buffer, shape, dtype=torch.float32):
-        raw = type("Raw", (), {"__cuda_array_interface__": {"shape": (buffer.len,), "typestr": "|u1", "data": (buffer.device_ptr, False), "version": 2}})()
-        return torch.as_tensor(raw, device=DEVICE).view(dtype).view(shape)
+        return torch.as_tensor(self.memory[buffer.id], device=DEVICE).view(dtype).view(shape)
 
     def given(self, state, name):
         """The input's values in a buffer of the handle; the state keeps the tensor that shows them."""
@@ -342,9 +353,7 @@ class Plan:
         b.begin()
         b.kv_write(cache, shape, spans, s, n, rows.slice(0, half), h * w, rows.slice(half, half), h * w)
         b.commit()
-        for used in (rows, spans):
-            self.held.remove(used)
-            b.release(used)
+        del self.memory[rows.id], self.memory[spans.id]
 
     def record(self, operators):
         torch.cuda.synchronize()
@@ -359,8 +368,6 @@ class Plan:
     def __del__(self):
         if self.graph is not None:
             backend().graph_release(self.graph)
-        for buffer in self.held:
-            backend().release(buffer)
 
 
 # ---- the work and the exact results ---------------------------------------------------------------------------------------------
