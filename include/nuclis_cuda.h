@@ -315,6 +315,69 @@ int nu_cuda_add(nu_cuda *h, const nu_buffer *x, const nu_buffer *y, size_t count
  * logit is NaN or infinite. The scratch of the reference's two passes belongs to the handle here. */
 int nu_cuda_argmax(nu_cuda *h, const nu_buffer *logits, size_t count, const nu_buffer *result);
 
+/* Log probabilities of given tokens, next to `argmax`: what an answer's logprobs, a scored prompt or a perplexity need
+ * of the head's logits, in one pass over them. Row r is the `count` F32 values at logits + r * in_stride; with
+ * p = softmax(row), every value as the definition gives it in F32 accuracy:
+ *   logprobs[r]      ln p of `tokens`[r] (one uint32 a row). A token of `count` or more gives NaN.
+ *   entropies[r]     -sum p ln p, in nats
+ *   top[r][0..k)     the k most likely tokens, the lowest index first among equals; top_logprobs[r][0..k) their ln p.
+ * k is 0 (then `top` and `top_logprobs` may be NULL) to 32, and at most `count`. Logits of minus infinity are masked
+ * tokens: probability 0, log probability minus infinity. A row that a mask leaves empty has log probabilities of minus
+ * infinity, entropy 0, and its first k indexes as alternatives. A row with a NaN or plus infinity has NaN everywhere and
+ * 0xffffffff for its alternatives. The result is the same from run to run. */
+int nu_cuda_token_logprobs(nu_cuda *h, const nu_buffer *logits, size_t rows, size_t count, size_t in_stride, const nu_buffer *tokens,
+                           const nu_buffer *logprobs, const nu_buffer *entropies, size_t k, const nu_buffer *top, const nu_buffer *top_logprobs);
+
+/* ---- key/value cache and attention: what a layer does between its QKV and its O projection --------
+ *
+ * A cache keeps the keys and values of `slots` sequences of up to `capacity` positions, quantized to GGUF blocks of 32
+ * (NU_Q8_0 or NU_Q4_0, keys and values each their own), for `heads` key/value heads of `width` values. The bytes are in
+ * the order that attention reads them in, which is this library's own: they are written by kv_write and read by kv_read
+ * and attention alone. A buffer of zeros is a cache of zeros. `width` is a multiple of 32, at most 512; `capacity` a
+ * multiple of 16. */
+typedef struct nu_kv_cache {
+    uint32_t key_encoding, value_encoding;
+    uint64_t slots, capacity, heads, width;
+} nu_kv_cache;
+/* Bytes of the buffer that holds the cache; 0 if the shape is not one of the above. */
+size_t nu_cuda_kv_bytes(const nu_kv_cache *cache);
+
+/* The rows of a call belong to `sequences` sequences of `tokens` rows each: row s * tokens + i is row i of sequence s. The
+ * `spans` buffer holds one of these per sequence, 16-byte aligned ON THE DEVICE, so that a retained graph serves every
+ * later step: write the new positions into the buffer and launch it again. Rows 0 .. count-1 stand at positions first ..
+ * first+count-1 of slot `slot`; the rows behind them are padding, neither read nor written. A span with a slot or a
+ * position outside the cache, or a count above `tokens`, is treated as empty, and the commit or graph launch that met it
+ * returns NU_ERR_EXECUTION; the other sequences are served. */
+typedef struct nu_kv_span {
+    uint32_t slot, first, count, reserved;
+} nu_kv_span;
+
+/* Quantizes rows of keys and values (F32, [heads][width] contiguous within a row, strides in floats) into the cache. The
+ * rule is GGUF's, in F32: Q8_0 d = amax / 127, code = round(x * (1 / d)); Q4_0 d = m / -8 with m the first value of the largest
+ * magnitude, code = min(15, trunc(x * (1 / d) + 8.5)); d is stored as f16. A scale beyond f16 saturates, a block with a NaN or
+ * an infinity reads back as NaN. Where two spans of one call cover the same position, the later span's row is kept. */
+int nu_cuda_kv_write(nu_cuda *h, const nu_buffer *buffer, const nu_kv_cache *cache, const nu_buffer *spans, size_t sequences, size_t tokens,
+                     const nu_buffer *keys, size_t key_stride, const nu_buffer *values, size_t value_stride);
+/* The reverse: rows of the cache decoded to `out_dtype` NU_F32 (the exact d * code) or NU_BF16 (rounded to nearest even);
+ * strides in elements. The two outputs may interleave in one buffer at one stride, but not overlap. */
+int nu_cuda_kv_read(nu_cuda *h, const nu_buffer *buffer, const nu_kv_cache *cache, const nu_buffer *spans, size_t sequences, size_t tokens,
+                    const nu_buffer *keys, size_t key_stride, const nu_buffer *values, size_t value_stride, uint32_t out_dtype);
+
+/* Causal attention over the cache: the row at position p of a slot sees the positions max(0, p - window + 1) .. p of it
+ * (window 0: all from 0), which must have been written. `heads` query heads, a multiple of the cache's: query head h
+ * reads key/value head h / (heads / cache heads).
+ *   output[row][h] = sum_j softmax_j(scale * query[row][h] . key_j) value_j
+ * Queries are F32, [heads][width] contiguous within a row, strides in elements; scale 0 stands for 1 / sqrt(width).
+ * `out_dtype` NU_F32 gives the result in F32 accuracy for any number of rows; NU_BF16 rounds it to BF16 (what `matmul` takes as
+ * its input), and may use 16-bit operands in the products where a call has many rows. */
+typedef struct nu_attention {
+    uint64_t heads, q_stride, out_stride;
+    uint32_t out_dtype, window;
+    float scale;
+} nu_attention;
+int nu_cuda_attention(nu_cuda *h, const nu_buffer *buffer, const nu_kv_cache *cache, const nu_buffer *spans, size_t sequences, size_t tokens,
+                      const nu_buffer *queries, const nu_buffer *output, const nu_attention *spec);
+
 /* `Backend.combineExperts` (ops/experts.zig:79-92); `scales` may be NULL. */
 int nu_cuda_combine_experts(nu_cuda *h, const nu_buffer *values, const nu_buffer *weights, const nu_buffer *indices,
                             const nu_buffer *scales, const nu_buffer *output, const nu_combine_shape *shape);

@@ -11,5 +11,5 @@ There is no CPU fallback: importing works anywhere, but creating a
 ``Backend`` without the built library or without a B200 raises.
 """
 from .errors import NuclisError  # noqa: F401
-from .backend import Backend, Buffer, Matrix, ExpertMatrix, Segment, SegmentMode, CombineShape  # noqa: F401
+from .backend import Backend, Buffer, Matrix, ExpertMatrix, KvCache, Segment, SegmentMode, CombineShape, kv_spans  # noqa: F401
 from . import encoding  # noqa: F401

@@ -40,6 +40,15 @@ class CNorm(ctypes.Structure):
     _fields_ = [("rows", sz), ("width", sz), ("in_stride", sz), ("out_stride", sz), ("eps", ctypes.c_float)]
 
 
+class CKvCache(ctypes.Structure):
+    _fields_ = [("key_encoding", u32), ("value_encoding", u32), ("slots", u64), ("capacity", u64), ("heads", u64), ("width", u64)]
+
+
+class CAttention(ctypes.Structure):
+    _fields_ = [("heads", u64), ("q_stride", u64), ("out_stride", u64), ("out_dtype", u32), ("window", u32), ("scale", ctypes.c_float)]
+
+
+KP = ctypes.POINTER(CKvCache)
 BP, MP, EP, SP = ctypes.POINTER(CBuffer), ctypes.POINTER(CMatrix), ctypes.POINTER(CExpertMatrix), ctypes.POINTER(CSegment)
 
 # name -> (restype, argtypes); every function declared in include/nuclis_cuda.h
@@ -84,6 +93,11 @@ SIGNATURES = {
     "nu_cuda_add_rms_norm": (cint, [vp, BP, BP, BP, BP, ctypes.POINTER(CNorm)]),
     "nu_cuda_add": (cint, [vp, BP, BP, sz]),
     "nu_cuda_argmax": (cint, [vp, BP, sz, BP]),
+    "nu_cuda_token_logprobs": (cint, [vp, BP, sz, sz, sz, BP, BP, BP, sz, BP, BP]),
+    "nu_cuda_kv_bytes": (sz, [KP]),
+    "nu_cuda_kv_write": (cint, [vp, BP, KP, BP, sz, sz, BP, sz, BP, sz]),
+    "nu_cuda_kv_read": (cint, [vp, BP, KP, BP, sz, sz, BP, sz, BP, sz, u32]),
+    "nu_cuda_attention": (cint, [vp, BP, KP, BP, sz, sz, BP, BP, ctypes.POINTER(CAttention)]),
     "nu_cuda_route": (cint, [vp, BP, sz, sz, sz, sz, BP, BP]),
     "nu_cuda_expert_lists_words": (sz, [sz, sz]),
     "nu_cuda_expert_lists": (cint, [vp, BP, sz, sz, sz, BP]),

@@ -74,6 +74,37 @@ class CombineShape:
     rows: int = 1
 
 
+@dataclass(frozen=True)
+class KvCache:
+    """Shape of a quantized key/value cache (``nu_kv_cache``): ``slots`` sequences of up to ``capacity`` positions (a multiple of
+    16), ``heads`` key/value heads of ``width`` values (a multiple of 32, at most 512), Q8_0 or Q4_0 blocks. No counterpart in
+    the reference's backend, whose caches are a session's business."""
+    slots: int
+    capacity: int
+    heads: int
+    width: int
+    key_encoding: int = 8
+    value_encoding: int = 8
+
+    def _c(self) -> _lib.CKvCache:
+        return _lib.CKvCache(self.key_encoding, self.value_encoding, self.slots, self.capacity, self.heads, self.width)
+
+    @property
+    def bytes(self) -> int:
+        """Length of the buffer that holds the cache; raises InvalidShape for a shape that is not served."""
+        n = _lib.load().nu_cuda_kv_bytes(ctypes.byref(self._c()))
+        if not n:
+            raise NuclisError(4, "kv cache: shape or encoding")
+        return n
+
+
+def kv_spans(spans) -> np.ndarray:
+    """The contents of a spans buffer: ``(slot, first, count)`` of each sequence of a call (``nu_kv_span``)."""
+    out = np.zeros((len(spans), 4), dtype=np.uint32)
+    out[:, :3] = np.asarray(spans, dtype=np.uint32).reshape(len(spans), 3)
+    return out
+
+
 class Buffer:
     """``Buffer`` (root.zig:62-86): a byte range of a device buffer; ``slice`` derives sub-ranges."""
 
@@ -326,6 +357,32 @@ class Backend:
     def argmax(self, logits: Buffer, count: int, result: Buffer) -> None:
         """Index of the largest logit into `result` (one uint32; 0xffffffff if a logit is not finite)."""
         self._check(self._lib.nu_cuda_argmax(self._h, logits._c(), count, result._c()))
+
+    def token_logprobs(self, logits: Buffer, rows: int, count: int, in_stride: int, tokens: Buffer, logprobs: Buffer, entropies: Buffer, k: int = 0,
+                       top: Buffer | None = None, top_logprobs: Buffer | None = None) -> None:
+        """Of each of ``rows`` rows of ``count`` logits: ln p of its token in ``tokens`` (uint32), the entropy in nats, and the ``k`` most
+        likely tokens with their ln p (see nu_cuda_token_logprobs)."""
+        self._check(self._lib.nu_cuda_token_logprobs(self._h, logits._c(), rows, count, in_stride, tokens._c(), logprobs._c(), entropies._c(), k,
+                                                     top._c() if top is not None else None, top_logprobs._c() if top_logprobs is not None else None))
+
+    def kv_write(self, cache: Buffer, shape: KvCache, spans: Buffer, sequences: int, tokens: int, keys: Buffer, key_stride: int, values: Buffer,
+                 value_stride: int) -> None:
+        """Quantizes rows of keys and values into the cache: row s * tokens + i goes to position first + i of the slot that
+        span s names, for i < count (``kv_spans``; the spans are read on the device, so a retained graph follows them)."""
+        self._check(self._lib.nu_cuda_kv_write(self._h, cache._c(), shape._c(), spans._c(), sequences, tokens, keys._c(), key_stride, values._c(), value_stride))
+
+    def kv_read(self, cache: Buffer, shape: KvCache, spans: Buffer, sequences: int, tokens: int, keys: Buffer, key_stride: int, values: Buffer,
+                value_stride: int, out_dtype: int = 0) -> None:
+        """Decodes rows of the cache to F32 or BF16, the reverse of ``kv_write``."""
+        self._check(self._lib.nu_cuda_kv_read(self._h, cache._c(), shape._c(), spans._c(), sequences, tokens, keys._c(), key_stride, values._c(), value_stride,
+                                              out_dtype))
+
+    def attention(self, cache: Buffer, shape: KvCache, spans: Buffer, sequences: int, tokens: int, queries: Buffer, q_stride: int, heads: int, output: Buffer,
+                  out_stride: int, scale: float | None = None, window: int = 0, out_dtype: int = 0) -> None:
+        """Causal grouped-query attention of ``heads`` query heads over the cache: the row at position p sees the last ``window``
+        positions up to p (0: all). ``scale`` defaults to 1 / sqrt(width); ``out_dtype`` F32 or BF16 (see nu_cuda_attention)."""
+        spec = _lib.CAttention(heads, q_stride, out_stride, out_dtype, window, 0.0 if scale is None else scale)
+        self._check(self._lib.nu_cuda_attention(self._h, cache._c(), shape._c(), spans._c(), sequences, tokens, queries._c(), output._c(), ctypes.byref(spec)))
 
     def route(self, logits: Buffer, experts: int, k: int, rows: int, in_stride: int, indices: Buffer, weights: Buffer) -> None:
         self._check(self._lib.nu_cuda_route(self._h, logits._c(), experts, k, rows, in_stride, indices._c(), weights._c()))

@@ -6,10 +6,12 @@
 
 #include <dlfcn.h>
 
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 
 #include "kernels.hpp"
+#include "kv_layout.cuh"
 #include "nu_device.cuh"
 
 namespace nu {
@@ -327,6 +329,7 @@ int Backend::checkKernelStatus() {
     if (status != 0) {
         cudaMemsetAsync(counters_, 0, (counters_len_ + 3) * sizeof(uint32_t), stream_);  // counters, status word, the chain kernel's two arrival counts
         cudaStreamSynchronize(stream_);
+        if (status == 3) return fail(NU_ERR_EXECUTION, "a span of rows lies outside the key/value cache: its sequence was left out");
         return fail(NU_ERR_EXECUTION, status == 2 ? "allreduce over peer memory: a rank never arrived (bounded wait ran out); the path stays closed" : "a kernel gave up a bounded wait (copy never completed)");
     }
     return NU_OK;
@@ -782,6 +785,154 @@ int Backend::argmax(const Buffer &logits, size_t count, const Buffer &result) {
     wrote(result);
     opBoundary();
     return cuda(cudaGetLastError(), "argmax: launch");
+}
+
+// No reference analogue: see nu_cuda_token_logprobs in the header and logprobs.cu.
+int Backend::tokenLogprobs(const Buffer &logits, size_t rows, size_t count, size_t in_stride, const Buffer &tokens, const Buffer &logprobs, const Buffer &entropies, size_t k,
+                           const Buffer *top, const Buffer *top_logprobs) {
+    if (rows == 0 || count == 0 || count > 0x7fffffffull || rows > (1u << 22) || in_stride < count || in_stride > (1ull << 40) || k > LOGPROB_ALTERNATIVES || k > count)
+        return fail(NU_ERR_INVALID_SHAPE, "token_logprobs: shape");
+    if (k && (!top || !top_logprobs)) return fail(NU_ERR_INVALID_SHAPE, "token_logprobs: alternatives without a buffer for them");
+    LogprobJob j{};
+    j.logits = (const float *)resolve(logits, ((rows - 1) * in_stride + count) * 4);
+    j.tokens = (const uint32_t *)resolve(tokens, rows * 4);
+    j.logprobs = (float *)resolve(logprobs, rows * 4);
+    j.entropies = (float *)resolve(entropies, rows * 4);
+    if (!j.logits || !j.tokens || !j.logprobs || !j.entropies || logits.offset % 4 || tokens.offset % 4 || logprobs.offset % 4 || entropies.offset % 4)
+        return fail(NU_ERR_INVALID_SHAPE, "token_logprobs: buffer too short");
+    if (k) {
+        j.top = (uint32_t *)resolve(*top, rows * k * 4);
+        j.top_logprobs = (float *)resolve(*top_logprobs, rows * k * 4);
+        if (!j.top || !j.top_logprobs || top->offset % 4 || top_logprobs->offset % 4) return fail(NU_ERR_INVALID_SHAPE, "token_logprobs: buffer too short");
+    }
+    // outputs apart from the inputs and from one another
+    const struct { const Buffer *b; size_t len; } part[] = {{&logprobs, rows * 4}, {&entropies, rows * 4}, {k ? top : nullptr, rows * k * 4}, {k ? top_logprobs : nullptr, rows * k * 4},
+                                                            {&logits, ((rows - 1) * in_stride + count) * 4}, {&tokens, rows * 4}};
+    for (int a = 0; a < 4; ++a)
+        for (int b = a + 1; b < 6; ++b)
+            if (part[a].b && part[b].b && overlaps(*part[a].b, part[a].len, *part[b].b, part[b].len)) return fail(NU_ERR_INVALID_SHAPE, "token_logprobs: an output overlaps another buffer");
+    if (int rc = needRecording()) return rc;
+    j.rows = (uint32_t)rows; j.count = (uint32_t)count; j.stride = in_stride; j.k = (uint32_t)k;
+    j.partials = partials_; j.partials_floats = partials_floats_; j.counters = counters_; j.counters_len = counters_len_; j.sm_count = sm_count_;
+    launches_ += launch_token_logprobs(stream_, j);
+    wrote(logprobs); wrote(entropies);
+    if (k) { wrote(*top); wrote(*top_logprobs); }
+    opBoundary();
+    return cuda(cudaGetLastError(), "token_logprobs: launch");
+}
+
+// ---- key/value cache and attention (kv_layout.cuh) ----
+
+size_t Backend::kvBytes(const nu_kv_cache &c) {
+    const bool k8 = c.key_encoding == NU_Q8_0, v8 = c.value_encoding == NU_Q8_0;
+    if ((!k8 && c.key_encoding != NU_Q4_0) || (!v8 && c.value_encoding != NU_Q4_0)) return 0;
+    if (c.width == 0 || c.width % 32 || c.width > 512 || c.capacity == 0 || c.capacity % KV_GRANULE || c.capacity > (1ull << 31)) return 0;
+    if (c.heads == 0 || c.heads > 1024 || c.slots == 0 || c.slots > (1u << 16)) return 0;
+    const uint64_t bytes = c.slots * c.heads * (c.capacity / KV_GRANULE);  // at most 2^53
+    const uint64_t granule = kv_layout((uint32_t)c.width, k8, v8).bytes;
+    return bytes > (1ull << 62) / granule ? 0 : (size_t)(bytes * granule);
+}
+
+// The checks that the three operators share; `who` starts the messages.
+int Backend::kvJob(const char *who, const Buffer &buffer, const nu_kv_cache &c, const Buffer &spans, size_t sequences, size_t tokens, KvCacheJob *job, const void **span_ptr) {
+    const std::string name(who);
+    for (const uint32_t e : {c.key_encoding, c.value_encoding})
+        if (e != NU_Q8_0 && e != NU_Q4_0) return fail(NU_ERR_UNSUPPORTED_ENCODING, (name + ": a cache is Q8_0 or Q4_0").c_str());
+    const size_t bytes = kvBytes(c);
+    if (!bytes) return fail(NU_ERR_INVALID_SHAPE, (name + ": cache shape").c_str());
+    if (sequences == 0 || sequences > 4096 || tokens == 0 || tokens > (1u << 20)) return fail(NU_ERR_INVALID_SHAPE, (name + ": sequences or tokens").c_str());
+    uint8_t *base = resolve(buffer, bytes);
+    *span_ptr = resolve(spans, sequences * sizeof(nu_kv_span));
+    if (!base || !*span_ptr) return fail(NU_ERR_INVALID_SHAPE, (name + ": cache or spans buffer too short").c_str());
+    if (buffer.offset % 16 || spans.offset % 16) return fail(NU_ERR_INVALID_SHAPE, (name + ": cache and spans lie on 16-byte boundaries").c_str());
+    *job = {base, c.key_encoding == NU_Q8_0, c.value_encoding == NU_Q8_0, (uint32_t)c.slots, (uint32_t)c.capacity, (uint32_t)c.heads, (uint32_t)c.width, counters_ + counters_len_};
+    return NU_OK;
+}
+
+namespace {
+// Bytes from the first to the last of `rows` rows; 0 when the stride is too small or beyond all bounds.
+size_t rowsBytes(size_t rows, size_t width, size_t stride, size_t element) {
+    if (stride < width || stride > (1ull << 40)) return 0;
+    return ((rows - 1) * stride + width) * element;
+}
+}  // namespace
+
+int Backend::kvWrite(const Buffer &buffer, const nu_kv_cache &c, const Buffer &spans, size_t sequences, size_t tokens, const Buffer &keys, size_t key_stride,
+                     const Buffer &values, size_t value_stride) {
+    KvCacheJob job;
+    const void *span = nullptr;
+    if (int rc = kvJob("kv_write", buffer, c, spans, sequences, tokens, &job, &span)) return rc;
+    const size_t width = c.heads * c.width, rows = sequences * tokens;
+    const size_t klen = rowsBytes(rows, width, key_stride, 4), vlen = rowsBytes(rows, width, value_stride, 4);
+    if (!klen || !vlen) return fail(NU_ERR_INVALID_SHAPE, "kv_write: stride");
+    if (rows * ((width + 127) / 128) > (1ull << 31)) return fail(NU_ERR_TOO_LARGE, "kv_write: too many rows in one call");
+    const float *k = (const float *)resolve(keys, klen), *v = (const float *)resolve(values, vlen);
+    if (!k || !v || keys.offset % 4 || values.offset % 4) return fail(NU_ERR_INVALID_SHAPE, "kv_write: buffer too short");
+    const size_t bytes = kvBytes(c);
+    if (overlaps(buffer, bytes, keys, klen) || overlaps(buffer, bytes, values, vlen) || overlaps(buffer, bytes, spans, sequences * sizeof(nu_kv_span)))
+        return fail(NU_ERR_INVALID_SHAPE, "kv_write: the cache overlaps an input");
+    if (int rc = needRecording()) return rc;
+    launches_ += launch_kv_write(stream_, job, span, (uint32_t)sequences, (uint32_t)tokens, k, key_stride, v, value_stride);
+    wrote(buffer);
+    opBoundary();
+    return cuda(cudaGetLastError(), "kv_write: launch");
+}
+
+int Backend::kvRead(const Buffer &buffer, const nu_kv_cache &c, const Buffer &spans, size_t sequences, size_t tokens, const Buffer &keys, size_t key_stride,
+                    const Buffer &values, size_t value_stride, uint32_t out_dtype) {
+    KvCacheJob job;
+    const void *span = nullptr;
+    if (int rc = kvJob("kv_read", buffer, c, spans, sequences, tokens, &job, &span)) return rc;
+    if (out_dtype != NU_F32 && out_dtype != NU_BF16) return fail(NU_ERR_INVALID_SHAPE, "kv_read: output type");
+    const size_t element = out_dtype == NU_F32 ? 4 : 2, width = c.heads * c.width, rows = sequences * tokens;
+    const size_t klen = rowsBytes(rows, width, key_stride, element), vlen = rowsBytes(rows, width, value_stride, element);
+    if (!klen || !vlen) return fail(NU_ERR_INVALID_SHAPE, "kv_read: stride");
+    if (rows * ((width + 127) / 128) > (1ull << 31)) return fail(NU_ERR_TOO_LARGE, "kv_read: too many rows in one call");
+    void *k = resolve(keys, klen), *v = resolve(values, vlen);
+    if (!k || !v || keys.offset % element || values.offset % element) return fail(NU_ERR_INVALID_SHAPE, "kv_read: buffer too short");
+    const size_t bytes = kvBytes(c), spans_len = sequences * sizeof(nu_kv_span);
+    if (overlaps(buffer, bytes, keys, klen) || overlaps(buffer, bytes, values, vlen) || overlaps(spans, spans_len, keys, klen) || overlaps(spans, spans_len, values, vlen))
+        return fail(NU_ERR_INVALID_SHAPE, "kv_read: an output overlaps the cache or the spans");
+    if (overlaps(keys, klen, values, vlen)) {  // fused rows: one stride, each row's keys clear of the values on either side
+        const size_t apart = (keys.offset < values.offset ? values.offset - keys.offset : keys.offset - values.offset) / element % key_stride;
+        if (key_stride != value_stride || apart < width || apart + width > key_stride) return fail(NU_ERR_INVALID_SHAPE, "kv_read: the outputs overlap");
+    }
+    if (int rc = needRecording()) return rc;
+    launches_ += launch_kv_read(stream_, job, span, (uint32_t)sequences, (uint32_t)tokens, k, key_stride, v, value_stride, out_dtype == NU_BF16);
+    wrote(keys); wrote(values);
+    opBoundary();
+    return cuda(cudaGetLastError(), "kv_read: launch");
+}
+
+int Backend::attention(const Buffer &buffer, const nu_kv_cache &c, const Buffer &spans, size_t sequences, size_t tokens, const Buffer &queries, const Buffer &output,
+                       const nu_attention &a) {
+    KvCacheJob job;
+    const void *span = nullptr;
+    if (int rc = kvJob("attention", buffer, c, spans, sequences, tokens, &job, &span)) return rc;
+    if (a.heads == 0 || a.heads % c.heads || a.heads > 16384) return fail(NU_ERR_INVALID_SHAPE, "attention: query heads are a multiple of the cache's");
+    if (a.out_dtype != NU_F32 && a.out_dtype != NU_BF16) return fail(NU_ERR_INVALID_SHAPE, "attention: output type");
+    if (!(a.scale >= 0.0f) || a.scale > 3.0e38f || a.window > (1u << 31)) return fail(NU_ERR_INVALID_SHAPE, "attention: scale or window");
+    const size_t element = a.out_dtype == NU_F32 ? 4 : 2, width = a.heads * c.width, rows = sequences * tokens;
+    const size_t qlen = rowsBytes(rows, width, a.q_stride, 4), olen = rowsBytes(rows, width, a.out_stride, element);
+    if (!qlen || !olen) return fail(NU_ERR_INVALID_SHAPE, "attention: stride");
+    if (rows * a.heads > (1ull << 31)) return fail(NU_ERR_TOO_LARGE, "attention: too many rows in one call");
+    AttentionJob j{};
+    j.queries = (const float *)resolve(queries, qlen);
+    j.out = resolve(output, olen);
+    if (!j.queries || !j.out || queries.offset % 4 || output.offset % element) return fail(NU_ERR_INVALID_SHAPE, "attention: buffer too short");
+    if (overlaps(output, olen, queries, qlen) || overlaps(output, olen, buffer, kvBytes(c)) || overlaps(output, olen, spans, sequences * sizeof(nu_kv_span)))
+        return fail(NU_ERR_INVALID_SHAPE, "attention: the output overlaps an input");
+    if (int rc = needRecording()) return rc;
+    j.cache = job; j.spans = span;
+    j.sequences = (uint32_t)sequences; j.tokens = (uint32_t)tokens;
+    j.q_stride = a.q_stride; j.out_stride = a.out_stride; j.heads = (uint32_t)a.heads;
+    j.bf16 = a.out_dtype == NU_BF16; j.window = a.window; j.generic = generic_only;
+    j.scale = a.scale > 0.0f ? a.scale : 1.0f / sqrtf((float)c.width);
+    j.partials = partials_; j.counters = counters_; j.sm_count = sm_count_;
+    launches_ += launch_attention(stream_, j);
+    wrote(output);
+    opBoundary();
+    return cuda(cudaGetLastError(), "attention: launch");
 }
 
 // ops/experts.zig:29-34.
@@ -1325,6 +1476,27 @@ int nu_cuda_add(nu_cuda *h, const nu_buffer *x, const nu_buffer *y, size_t count
 int nu_cuda_argmax(nu_cuda *h, const nu_buffer *logits, size_t count, const nu_buffer *result) {
     NU_H(h); NU_P(logits && result);
     return h->b->argmax(*logits, count, *result);
+}
+int nu_cuda_token_logprobs(nu_cuda *h, const nu_buffer *logits, size_t rows, size_t count, size_t in_stride, const nu_buffer *tokens, const nu_buffer *logprobs,
+                           const nu_buffer *entropies, size_t k, const nu_buffer *top, const nu_buffer *top_logprobs) {
+    NU_H(h); NU_P(logits && tokens && logprobs && entropies);
+    return h->b->tokenLogprobs(*logits, rows, count, in_stride, *tokens, *logprobs, *entropies, k, top, top_logprobs);
+}
+size_t nu_cuda_kv_bytes(const nu_kv_cache *cache) { return cache ? nu::Backend::kvBytes(*cache) : 0; }
+int nu_cuda_kv_write(nu_cuda *h, const nu_buffer *buffer, const nu_kv_cache *cache, const nu_buffer *spans, size_t sequences, size_t tokens, const nu_buffer *keys,
+                     size_t key_stride, const nu_buffer *values, size_t value_stride) {
+    NU_H(h); NU_P(buffer && cache && spans && keys && values);
+    return h->b->kvWrite(*buffer, *cache, *spans, sequences, tokens, *keys, key_stride, *values, value_stride);
+}
+int nu_cuda_kv_read(nu_cuda *h, const nu_buffer *buffer, const nu_kv_cache *cache, const nu_buffer *spans, size_t sequences, size_t tokens, const nu_buffer *keys,
+                    size_t key_stride, const nu_buffer *values, size_t value_stride, uint32_t out_dtype) {
+    NU_H(h); NU_P(buffer && cache && spans && keys && values);
+    return h->b->kvRead(*buffer, *cache, *spans, sequences, tokens, *keys, key_stride, *values, value_stride, out_dtype);
+}
+int nu_cuda_attention(nu_cuda *h, const nu_buffer *buffer, const nu_kv_cache *cache, const nu_buffer *spans, size_t sequences, size_t tokens, const nu_buffer *queries,
+                      const nu_buffer *output, const nu_attention *spec) {
+    NU_H(h); NU_P(buffer && cache && spans && queries && output && spec);
+    return h->b->attention(*buffer, *cache, *spans, sequences, tokens, *queries, *output, *spec);
 }
 int nu_cuda_route_local(nu_cuda *h, const nu_buffer *indices, const nu_buffer *weights, size_t count, size_t first_expert, size_t local_experts,
                         const nu_buffer *local_indices, const nu_buffer *local_weights) {

@@ -24,6 +24,7 @@ struct FastJob;
 struct FastJobBox;
 struct FastChain;
 struct FastJob;
+struct KvCacheJob;
 
 using Buffer = nu_buffer;
 using Matrix = nu_matrix;
@@ -80,6 +81,15 @@ public:
     int addRmsNorm(const Buffer &residual, const Buffer &input, const Buffer &weight, const Buffer &output, const nu_norm &spec);
     int add(const Buffer &x, const Buffer &y, size_t count);
     int argmax(const Buffer &logits, size_t count, const Buffer &result);
+    int tokenLogprobs(const Buffer &logits, size_t rows, size_t count, size_t in_stride, const Buffer &tokens, const Buffer &logprobs, const Buffer &entropies, size_t k,
+                      const Buffer *top, const Buffer *top_logprobs);
+    static size_t kvBytes(const nu_kv_cache &cache);
+    int kvWrite(const Buffer &buffer, const nu_kv_cache &cache, const Buffer &spans, size_t sequences, size_t tokens, const Buffer &keys, size_t key_stride,
+                const Buffer &values, size_t value_stride);
+    int kvRead(const Buffer &buffer, const nu_kv_cache &cache, const Buffer &spans, size_t sequences, size_t tokens, const Buffer &keys, size_t key_stride,
+               const Buffer &values, size_t value_stride, uint32_t out_dtype);
+    int attention(const Buffer &buffer, const nu_kv_cache &cache, const Buffer &spans, size_t sequences, size_t tokens, const Buffer &queries, const Buffer &output,
+                  const nu_attention &spec);
     int route(const Buffer &logits, size_t experts, size_t k, size_t rows, size_t in_stride, const Buffer &indices, const Buffer &weights);
     int routeLocal(const Buffer &indices, const Buffer &weights, size_t count, size_t first, size_t local, const Buffer &local_indices, const Buffer &local_weights);
     int matvecExpertsGrouped(const Buffer &weights, const ExpertMatrix &tensor, const Buffer &indices, size_t slots,
@@ -118,6 +128,7 @@ private:
     // Device address of a view after checking that `need` bytes fit in it and in its buffer.
     uint8_t *resolve(const Buffer &b, size_t need);
     static bool overlaps(const Buffer &a, size_t a_len, const Buffer &b, size_t b_len);
+    int kvJob(const char *who, const Buffer &buffer, const nu_kv_cache &cache, const Buffer &spans, size_t sequences, size_t tokens, KvCacheJob *job, const void **span_ptr);
     int needRecording(bool keep_chain = false);
     void opBoundary();
     void wrote(const Buffer &b);

@@ -61,7 +61,7 @@ bool fast_supported(const FastJob &job) {
 }
 
 bool fast_configure() {
-    return q4k_i8_configure() && q6k_i8_configure() && q8_0_i8_configure() && block32_i8_configure() && q5k_i8_configure() && q23k_i8_configure() && prefill_configure() && expert_gemv_configure() && chain_configure();
+    return q4k_i8_configure() && q6k_i8_configure() && q8_0_i8_configure() && block32_i8_configure() && q5k_i8_configure() && q23k_i8_configure() && prefill_configure() && expert_gemv_configure() && chain_configure() && attention_configure();
 }
 
 int launch_fast(cudaStream_t s, const FastJob &job) {

@@ -192,4 +192,55 @@ int launch_gather_sum(cudaStream_t s, const PushParams &p);
 uint32_t prepared_layout(uint32_t enc, uint32_t rows, uint32_t columns);
 int launch_prepare(cudaStream_t s, uint32_t enc, const uint8_t *src, uint8_t *dst, uint32_t rows, uint32_t columns);
 
+// ---- the quantized key/value cache and the attention that reads it (kv_layout.cuh) ---------
+struct KvCacheJob {
+    uint8_t *base;
+    bool k8, v8;  // Q8_0 instead of Q4_0
+    uint32_t slots, capacity, heads, width;
+    uint32_t *status;  // raised when a span lies outside the cache
+};
+// keys and values: [sequences * tokens] rows at their strides (in elements); spans: one nu_kv_span a sequence, on the device.
+int launch_kv_write(cudaStream_t s, const KvCacheJob &cache, const void *spans, uint32_t sequences, uint32_t tokens, const float *keys, size_t key_stride,
+                    const float *values, size_t value_stride);
+int launch_kv_read(cudaStream_t s, const KvCacheJob &cache, const void *spans, uint32_t sequences, uint32_t tokens, void *keys, size_t key_stride, void *values,
+                   size_t value_stride, bool bf16);
+struct AttentionJob {
+    KvCacheJob cache;
+    const void *spans;
+    uint32_t sequences, tokens;
+    const float *queries;
+    size_t q_stride;
+    uint32_t heads;  // query heads, a multiple of the cache's
+    void *out;
+    size_t out_stride;
+    bool bf16;
+    float scale;
+    uint32_t window;  // 0: none
+    bool generic;
+    float *partials;     // of the handle
+    uint32_t *counters;  // of the handle, zero between launches
+    int sm_count;
+};
+bool attention_configure();
+int launch_attention(cudaStream_t s, const AttentionJob &job);
+
+// ---- log probabilities of given tokens (logprobs.cu) --------------------------------------
+constexpr uint32_t LOGPROB_ALTERNATIVES = 32;
+struct LogprobJob {
+    const float *logits;
+    uint32_t rows, count;
+    size_t stride;
+    const uint32_t *tokens;
+    float *logprobs, *entropies;
+    uint32_t k;
+    uint32_t *top;
+    float *top_logprobs;
+    float *partials;     // of the handle
+    size_t partials_floats;
+    uint32_t *counters;  // of the handle, zero between launches
+    size_t counters_len;
+    int sm_count;
+};
+int launch_token_logprobs(cudaStream_t s, const LogprobJob &job);
+
 }  // namespace nu

@@ -1,0 +1,620 @@
+// Causal grouped-query attention over the quantized cache, in F32 accuracy.
+//
+//     out = sum_j softmax_j(scale q . k_j) v_j,   j in [max(0, p - window + 1), p]   for the row at position p
+//
+// split_kernel (widths 64, 128, 256) reads every cache byte of a head once for up to eight query rows and runs both products
+// on mma.sync.m16n8k16 without losing F32 accuracy:
+//
+//   * Codes are whole numbers of at most eight bits, so they are exact in f16; a block's scale is applied to the product, not
+//     to the codes. What is not exact in f16, the query and the probabilities, is split: x = hi + lo / 2048 with hi and lo in
+//     f16 (22 bits). The 16 rows of the A operand are the hi parts of eight query rows and their lo parts, so the split
+//     costs no second instruction, and the two sums of a row come out in the same thread.
+//   * q . k = sum_b d_b (q_b . c_b): one accumulator pair of instructions per block of 32, then one F32 FMA with d_b.
+//   * p v = sum_j (p_j d_jb) c_j: the scale goes into the probability, once per block, before it is split. The products
+//     p d are kept near one by a power of two per warp (`bias`), raised when a larger scale comes by: f16's range is no limit, and what
+//     is lost of a position is below 2^-36 of the largest value seen.
+//   * The running maximum of a row is only raised when a score passes it by 8 (in log2): the accumulators are rarely rescaled.
+//
+// Work split: the granules of all (sequence, row tile, head) units are laid end to end and every block takes the same
+// number of them, whatever the lengths are; they are counted on the device from the spans, so a recorded launch fits every
+// later length. A unit that spans blocks is joined by the block that arrives last, in block order: nothing depends on timing.
+// Within a block the warps take turns at stages of one or two granules, each through its own ring of bulk copies.
+//
+// generic_kernel: one warp per query row and head, any width up to 512; also what generic_only selects.
+#include <cuda_bf16.h>
+
+#include "kernels.hpp"
+#include "kv_layout.cuh"
+#include "launch.cuh"
+
+namespace nu {
+
+namespace {
+
+constexpr uint32_t SPIN_LIMIT = 1u << 22;
+
+struct AttentionParams {
+    KvView c;
+    const KvSpan *spans;
+    uint32_t sequences, tokens;
+    const float *q;
+    size_t q_stride;
+    uint32_t group;  // query heads of a key/value head
+    uint32_t tiles;  // row tiles of a (sequence, head): ceil(tokens * group / 8)
+    void *out;
+    size_t out_stride;
+    bool bf16;
+    float scale;     // times log2(e)
+    uint32_t window; // 0: none
+    float *partials;      // [block][2][rows * (width + 2)]
+    uint32_t *counters;   // one a block, zero between launches
+};
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void store_out(const AttentionParams &p, size_t index, float v) {
+    if (p.bf16) ((__nv_bfloat16 *)p.out)[index] = __float2bfloat16_rn(v);
+    else ((float *)p.out)[index] = v;
+}
+
+// ---- any width ---------------------------------------------------------------------------------------------------------
+
+constexpr int GENERIC_WARPS = 4;
+constexpr uint32_t GENERIC_WIDTH = 512;
+
+__device__ __forceinline__ float key_value(const KvLayout &l, const uint8_t *g, uint32_t at, uint32_t dim) {
+    const float d = __half2float(*(const __half *)(g + l.k_scales + (at * l.blocks + dim / 32) * 2));
+    const uint32_t i = dim % 8, t = dim % 32 / 8;
+    if (l.k8) {
+        const uint32_t w = *(const uint32_t *)(g + kv_key_word(l, at, dim / 32, t, i % 4 / 2));
+        return d * (float)((int)(w >> (8 * (i % 2 * 2 + i / 4)) & 255u) - 128);
+    }
+    return d * (float)((int)(*(const uint32_t *)(g + kv_key_word(l, at, dim / 32, t, 0)) >> (4 * i) & 15u) - 8);
+}
+__device__ __forceinline__ float value_value(const KvLayout &l, const uint8_t *g, uint32_t at, uint32_t dim) {
+    const float d = __half2float(*(const __half *)(g + l.v_scales + (at * l.blocks + dim / 32) * 2));
+    const uint32_t byte = g[kv_value_byte(l, at, dim)];
+    return d * (float)(l.v8 ? (int)byte - 128 : (int)(byte >> (dim & 8 ? 4 : 0) & 15u) - 8);
+}
+
+__global__ void __launch_bounds__(GENERIC_WARPS * 32) generic_kernel(const AttentionParams p) {
+    __shared__ float queries[GENERIC_WARPS][GENERIC_WIDTH];
+    wait_for_previous_operator();
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32, width = p.c.l.width, heads = p.c.heads * p.group;
+    const size_t item = (size_t)blockIdx.x * GENERIC_WARPS + warp, r = item / heads;
+    const uint32_t head = (uint32_t)(item % heads);
+    if (r >= (size_t)p.sequences * p.tokens) return;
+    const KvSpan span = kv_span(p.c, p.spans, (uint32_t)(r / p.tokens), p.tokens);
+    const uint32_t i = (uint32_t)(r % p.tokens);
+    if (i >= span.count) return;
+    const uint32_t pos = span.first + i, low = p.window && pos >= p.window ? pos - p.window + 1 : 0;
+    const float *q = p.q + r * p.q_stride + (size_t)head * width;
+    for (uint32_t d = lane; d < width; d += 32) queries[warp][d] = q[d] * p.scale;
+    __syncwarp();
+    const uint8_t *base = kv_head(p.c, span.slot, head / p.group);
+    float m = -INFINITY, sum = 0.0f, acc[GENERIC_WIDTH / 32];
+#pragma unroll
+    for (int k = 0; k < (int)GENERIC_WIDTH / 32; ++k) acc[k] = 0.0f;
+    for (uint64_t j0 = low; j0 <= pos; j0 += 32) {
+        const uint64_t j = j0 + lane;
+        float s = -INFINITY;
+        if (j <= pos) {
+            const uint8_t *g = base + (size_t)(j / KV_GRANULE) * p.c.l.bytes;
+            s = 0.0f;
+            for (uint32_t d = 0; d < width; ++d) s = fmaf(queries[warp][d], key_value(p.c.l, g, (uint32_t)(j % KV_GRANULE), d), s);
+        }
+        float top = s;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float next = fmaxf(m, top), f = next == -INFINITY ? 1.0f : exp2f(m - next);
+        const float w = j <= pos ? exp2f(s - (next == -INFINITY ? 0.0f : next)) : 0.0f;
+        sum = sum * f + w;
+        m = next;
+#pragma unroll
+        for (int k = 0; k < (int)GENERIC_WIDTH / 32; ++k) acc[k] *= f;
+        const uint32_t n = (uint32_t)min((uint64_t)32, pos - j0 + 1);
+        for (uint32_t l = 0; l < n; ++l) {
+            const float wl = __shfl_sync(0xffffffffu, w, l);
+            const uint8_t *g = base + (size_t)((j0 + l) / KV_GRANULE) * p.c.l.bytes;
+#pragma unroll
+            for (int k = 0; k < (int)GENERIC_WIDTH / 32; ++k)
+                if (k * 32 < (int)width) acc[k] = fmaf(wl, value_value(p.c.l, g, (uint32_t)((j0 + l) % KV_GRANULE), k * 32 + lane), acc[k]);
+        }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+#pragma unroll
+    for (int k = 0; k < (int)GENERIC_WIDTH / 32; ++k)
+        if (k * 32 < (int)width) store_out(p, r * p.out_stride + (size_t)head * width + k * 32 + lane, acc[k] / sum);
+}
+
+// ---- widths 64, 128, 256 -------------------------------------------------------------------------------------------------
+
+constexpr int ROWS = 8;  // query rows of a unit
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
+    for (uint32_t i = 0; i < SPIN_LIMIT; ++i) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (done) return true;
+    }
+    return false;
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void mma(float c[4], const uint4 a, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t h2(__half2 x) { return *(const uint32_t *)&x; }
+__device__ __forceinline__ __half2 as_h2(uint32_t x) { return *(const __half2 *)&x; }
+// Four-bit codes in bits 0..3 / 4..7 of the bytes 0 and 2 of w, as whole numbers code - 8 in f16: the code is placed in the
+// low bits of 1024 (or, shifted by four, of 1024 = 64 * 16), which one exact operation takes off again.
+__device__ __forceinline__ uint32_t low_codes(uint32_t w) { return h2(__hsub2(as_h2((w & 0x000f000fu) | 0x64006400u), as_h2(0x64086408u))); }
+__device__ __forceinline__ uint32_t high_codes(uint32_t w) { return h2(__hfma2(as_h2((w & 0x00f000f0u) | 0x64006400u), as_h2(0x2c002c00u), as_h2(0xd480d480u))); }
+// Eight-bit codes in bytes 0, 1 (or 2, 3) of w, as code - 128.
+__device__ __forceinline__ uint32_t byte_codes(uint32_t w, uint32_t selector) { return h2(__hsub2(as_h2(__byte_perm(w, 0x64646464u, selector)), as_h2(0x64806480u))); }
+
+__device__ __forceinline__ uint32_t pack_hi_lo(float x, float y, uint32_t &lo) {
+    const __half2 hi = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(hi);
+    lo = h2(__floats2half2_rn((x - f.x) * 2048.0f, (y - f.y) * 2048.0f));
+    return h2(hi);
+}
+constexpr float LO = 1.0f / 2048.0f;
+
+// N words of a lane's codes in a tile, kept in vectors.
+template <int N, int VEC>
+__device__ __forceinline__ void load_words(const uint8_t *tile, uint32_t lane, uint32_t (&w)[N]) {
+#pragma unroll
+    for (int v = 0; v < N * 4 / VEC; ++v) {
+        const uint8_t *src = tile + v * 32 * VEC + lane * VEC;
+        if (VEC == 16) {
+            const uint4 x = *(const uint4 *)src;
+            w[v * 4] = x.x; w[v * 4 + 1] = x.y; w[v * 4 + 2] = x.z; w[v * 4 + 3] = x.w;
+        } else {
+            const uint2 x = *(const uint2 *)src;
+            w[v * 2] = x.x; w[v * 2 + 1] = x.y;
+        }
+    }
+}
+// The scales of positions at, at + 1 (NB each): N = NB words.
+template <int NB>
+__device__ __forceinline__ void load_scales(const uint8_t *scales, uint32_t at, uint32_t (&w)[NB]) {
+    const uint8_t *src = scales + at * NB * 2;
+#pragma unroll
+    for (int i = 0; i < NB; i += 4) {
+        if (NB == 2) {
+            const uint2 x = *(const uint2 *)src;
+            w[0] = x.x; w[1] = x.y;
+        } else {
+            const uint4 x = *(const uint4 *)(src + i * 4);
+            w[i] = x.x; w[i + 1] = x.y; w[i + 2] = x.z; w[i + 3] = x.w;
+        }
+    }
+}
+template <int NB>
+__device__ __forceinline__ float scale_of(const uint32_t (&w)[NB], int e, int b) {
+    const int i = e * NB + b;
+    return __half2float(__ushort_as_half((unsigned short)(i % 2 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu)));
+}
+
+template <int W, bool K8, bool V8>
+struct Split {
+    static constexpr int WARPS = 8, THREADS = WARPS * 32;
+    static constexpr int NB = W / 32, KT = W / 16, NT = W / 8;
+    static constexpr KvLayout L = kv_layout(W, K8, V8);
+    static constexpr int SG = L.bytes <= 2560 ? 2 : 1;  // granules of a stage
+    static constexpr int STAGE = SG * (int)L.bytes;
+    static constexpr int RING = 196 * 1024 / WARPS;
+    static constexpr int STAGES = RING / STAGE < 8 ? RING / STAGE : 8;
+    static constexpr int JOIN = WARPS * ROWS * W * 4;  // the warps' accumulators; takes the ring's place
+    static constexpr int BUFFER = WARPS * STAGES * STAGE > JOIN ? WARPS * STAGES * STAGE : JOIN;
+    static constexpr int FRAGMENTS = KT * 512;
+    static constexpr int SMEM = BUFFER + FRAGMENTS + WARPS * STAGES * 8 + (WARPS * 2 + 1) * ROWS * 4 + 64;
+    static constexpr int PARTIAL = ROWS * (W + 2);
+    static_assert(STAGES >= 2, "a ring needs two stages");
+};
+
+// The granules that the rows of tile `tile` of a sequence see: [first, first + count).
+__device__ __forceinline__ void unit_range(const AttentionParams &p, const KvSpan &s, uint32_t tile, uint32_t &first, uint32_t &count) {
+    const uint64_t rows = (uint64_t)s.count * p.group, r0 = (uint64_t)tile * ROWS;
+    first = count = 0;
+    if (r0 >= rows) return;
+    const uint64_t r1 = min(rows, r0 + ROWS) - 1;
+    const uint32_t low = s.first + (uint32_t)(r0 / p.group), high = s.first + (uint32_t)(r1 / p.group);
+    first = (p.window && low >= p.window ? low - p.window + 1 : 0) / KV_GRANULE;
+    count = high / KV_GRANULE + 1 - first;
+}
+
+template <int W, bool K8, bool V8>
+__global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 1) split_kernel(const __grid_constant__ AttentionParams p) {
+    using S = Split<W, K8, V8>;
+    constexpr int NB = S::NB, NT = S::NT, WARPS = S::WARPS, STAGES = S::STAGES, SG = S::SG;
+    constexpr KvLayout L = S::L;
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint8_t *ring = smem;
+    float *join = (float *)smem;
+    uint4 *fragments = (uint4 *)(smem + S::BUFFER);                     // [KT][32]
+    uint64_t *bars = (uint64_t *)(smem + S::BUFFER + S::FRAGMENTS);     // [WARPS][STAGES]
+    float *join_m = (float *)(bars + WARPS * STAGES);                   // [WARPS][ROWS]
+    float *join_l = join_m + WARPS * ROWS;                              // [WARPS][ROWS]
+    float *row_scale = join_l + WARPS * ROWS;                           // [ROWS]
+    uint32_t *word = (uint32_t *)(row_scale + ROWS);                    // broadcast words
+    __shared__ unsigned long long sums[WARPS], start[2];
+
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid / 32, g = lane / 4, t = lane % 4;
+    if (lane == 0)
+        for (int i = 0; i < STAGES; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bars + warp * STAGES + i)), "r"(1));
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncwarp();
+    wait_for_previous_operator();
+
+    // ---- this block's share: granules [begin, end) of all units' laid end to end, unit = (sequence, tile, head) ----
+    const size_t entries = (size_t)p.sequences * p.tiles, per = (entries + S::THREADS - 1) / S::THREADS;
+    const size_t e0 = min(entries, tid * per), e1 = min(entries, e0 + per);
+    unsigned long long mine = 0;
+    for (size_t e = e0; e < e1; ++e) {
+        uint32_t first, count;
+        unit_range(p, kv_span(p.c, p.spans, (uint32_t)(e / p.tiles), p.tokens), (uint32_t)(e % p.tiles), first, count);
+        mine += (unsigned long long)count * p.c.heads;
+    }
+    unsigned long long before = mine;  // inclusive sum over the warp's lanes
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long x = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= (uint32_t)o) before += x;
+    }
+    if (lane == 31) sums[warp] = before;
+    __syncthreads();
+    unsigned long long total = 0;
+    for (int w = 0; w < WARPS; ++w) {
+        if (w == (int)warp) before += total;
+        total += sums[w];
+    }
+    before -= mine;
+    const unsigned long long sh = (total + gridDim.x - 1) / gridDim.x;
+    unsigned long long at = blockIdx.x * sh;
+    const unsigned long long end = min(total, at + sh);
+    if (at >= end) return;  // the whole block
+    if (at >= before && at < before + mine) {  // one thread
+        for (size_t e = e0; e < e1; ++e) {
+            uint32_t first, count;
+            unit_range(p, kv_span(p.c, p.spans, (uint32_t)(e / p.tiles), p.tokens), (uint32_t)(e % p.tiles), first, count);
+            const unsigned long long n = (unsigned long long)count * p.c.heads;
+            if (at < before + n) { start[0] = e; start[1] = before; break; }
+            before += n;
+        }
+    }
+    __syncthreads();
+    unsigned long long entry = start[0], entry_begin = start[1];  // the entry that `at` lies in, and where its granules begin
+
+    uint32_t turn = 0;  // stages this warp has taken, over all segments: position and phase in the ring
+    bool alive = true;
+    while (at < end) {
+        // ---- the segment: granules [g0, g0 + n) of one unit ----
+        const KvSpan span = kv_span(p.c, p.spans, (uint32_t)(entry / p.tiles), p.tokens);
+        const uint32_t tile = (uint32_t)(entry % p.tiles);
+        uint32_t first, count;
+        unit_range(p, span, tile, first, count);
+        if (at - entry_begin >= (unsigned long long)count * p.c.heads) {  // all its heads are done (or it has no rows)
+            entry_begin += (unsigned long long)count * p.c.heads;
+            ++entry;
+            continue;
+        }
+        const uint32_t head = (uint32_t)((at - entry_begin) / count);
+        const unsigned long long unit_begin = entry_begin + (unsigned long long)head * count;
+        const uint32_t skip = (uint32_t)(at - unit_begin), n = (uint32_t)min((unsigned long long)(count - skip), end - at), g0 = first + skip;
+        const uint8_t *base = kv_head(p.c, span.slot, head) + (size_t)g0 * L.bytes;
+        const uint32_t stages = (n + SG - 1) / SG, mystages = stages > warp ? (stages - warp + WARPS - 1) / WARPS : 0;
+        auto request = [&](uint32_t i) {  // the warp's stage i of this segment
+            const uint32_t st = warp + i * WARPS, pos = (turn + i) % STAGES;
+            const uint32_t bytes = min((uint32_t)SG, n - st * SG) * L.bytes;
+            bulk_load(smem_u32(ring + (warp * STAGES + pos) * S::STAGE), base + (size_t)st * S::STAGE, bytes, smem_u32(bars + warp * STAGES + pos));
+        };
+        if (lane == 0)
+            for (uint32_t i = 0; i < min(mystages, (uint32_t)STAGES); ++i) request(i);
+
+        // ---- the rows, split into f16 halves after a power of two that brings each row's largest value to [1, 2) ----
+        const size_t rows0 = (size_t)(entry / p.tiles) * p.tokens;  // the sequence's first row in the call
+        const uint64_t live_rows = (uint64_t)span.count * p.group;
+        for (uint32_t r = warp; r < ROWS; r += WARPS) {
+            const uint64_t row = (uint64_t)tile * ROWS + r;
+            float x[8] = {};
+            if (row < live_rows && lane < (uint32_t)W / 8) {
+                const float *q = p.q + (rows0 + row / p.group) * p.q_stride + (size_t)(head * p.group + (uint32_t)(row % p.group)) * W + lane * 8;
+                if ((uintptr_t)q % 16 == 0) {
+                    const float4 a = *(const float4 *)q, b = *(const float4 *)(q + 4);
+                    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] = q[i];
+                }
+            }
+            uint32_t top = 0;  // as bits: NaN and infinity come out largest
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+            top = __reduce_max_sync(0xffffffffu, top);
+            // 2^e: from the exponent's bits; rows of zeros and of subnormal values count as 2^-126
+            const int e = (int)max(top >> 23, 1u) - 127;
+            const float down = top >= 0x7f800000u ? NAN : scalbnf(1.0f, -e);
+            if (lane == 0) row_scale[r] = scalbnf(p.scale, e);
+            if (lane < (uint32_t)W / 8) {
+                const uint32_t b = lane / 4, tt = lane % 4;
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) hi[i] = pack_hi_lo(x[i] * down, x[i + 4] * down, lo[i]);
+                // the pair of dimensions i, i + 4 of the eight is the k pair of step i / 2, half i % 2
+                fragments[(2 * b) * 32 + r * 4 + tt] = make_uint4(hi[0], lo[0], hi[1], lo[1]);
+                fragments[(2 * b + 1) * 32 + r * 4 + tt] = make_uint4(hi[2], lo[2], hi[3], lo[3]);
+            }
+        }
+        __syncthreads();
+
+        // positions that this thread's row sees, and those that every row of the tile sees
+        const uint64_t row = (uint64_t)tile * ROWS + g;
+        const uint32_t pos = row < live_rows ? span.first + (uint32_t)(row / p.group) : 0;
+        const uint32_t row_high = pos, row_low = row < live_rows ? (p.window && pos >= p.window ? pos - p.window + 1 : 0) : 1;  // a dead row sees nothing
+        const uint64_t last_row = min(live_rows, (uint64_t)tile * ROWS + ROWS) - 1;
+        const uint32_t tile_high = span.first + (uint32_t)(last_row / p.group), first_pos = span.first + (uint32_t)((uint64_t)tile * ROWS / p.group);
+        const uint32_t tile_low = p.window && first_pos >= p.window ? first_pos - p.window + 1 : 0;   // some row sees [tile_low, tile_high]
+        const uint32_t all_low = p.window && tile_high >= p.window ? tile_high - p.window + 1 : 0;    // every live row sees [all_low, first_pos]
+        const float my_scale = row_scale[g];
+
+        float m = -INFINITY, l = 0.0f, bias = 0x1p40f, o[NT][4];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+
+        for (uint32_t i = 0; i < mystages && alive; ++i) {
+            const uint32_t slot = (turn + i) % STAGES;
+            alive = mbar_wait(smem_u32(bars + warp * STAGES + slot), (turn + i) / STAGES & 1u);
+            if (!__all_sync(0xffffffffu, alive)) {  // a copy never came: report, let the others in flight land, give up the block's results
+                *(volatile uint32_t *)p.c.status = 1u;
+                for (uint32_t k = i + 1; k < min(i + STAGES, mystages); ++k) mbar_wait(smem_u32(bars + warp * STAGES + (turn + k) % STAGES), (turn + k) / STAGES & 1u);
+                alive = false;
+                break;
+            }
+            const uint8_t *stage = ring + (warp * STAGES + slot) * S::STAGE;
+            const uint32_t st = warp + i * WARPS, key0 = (g0 + st * SG) * KV_GRANULE;
+            const uint32_t here = min((uint32_t)SG, n - st * SG) * KV_GRANULE;  // positions that were copied
+            const bool edge = key0 < all_low || key0 + SG * KV_GRANULE - 1 > first_pos || here < SG * KV_GRANULE;
+
+            float s[SG * 2][2];
+#pragma unroll
+            for (int j = 0; j < SG * 2; ++j) {
+                const uint8_t *gran = stage + j / 2 * L.bytes;
+                uint32_t codes[K8 ? 2 * NB : NB], scales[NB];
+                load_words<K8 ? 2 * NB : NB, L.k_vec>(gran + j % 2 * (L.k_scales / 2), lane, codes);
+                load_scales<NB>(gran + L.k_scales, j % 2 * 8 + 2 * t, scales);
+                s[j][0] = s[j][1] = 0.0f;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    if (K8) {
+                        mma(c, fragments[(2 * b) * 32 + lane], byte_codes(codes[2 * b], 0x4140), byte_codes(codes[2 * b], 0x4342));
+                        mma(c, fragments[(2 * b + 1) * 32 + lane], byte_codes(codes[2 * b + 1], 0x4140), byte_codes(codes[2 * b + 1], 0x4342));
+                    } else {
+                        const uint32_t w = codes[b], w8 = w >> 8;
+                        mma(c, fragments[(2 * b) * 32 + lane], low_codes(w), high_codes(w));
+                        mma(c, fragments[(2 * b + 1) * 32 + lane], low_codes(w8), high_codes(w8));
+                    }
+                    s[j][0] = fmaf(scale_of<NB>(scales, 0, b), fmaf(c[2], LO, c[0]), s[j][0]);
+                    s[j][1] = fmaf(scale_of<NB>(scales, 1, b), fmaf(c[3], LO, c[1]), s[j][1]);
+                }
+                s[j][0] *= my_scale;
+                s[j][1] *= my_scale;
+                if (edge) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const uint32_t in = j * 8 + 2 * t + e, key = key0 + in;
+                        if (in >= here || key < row_low || key > row_high) s[j][e] = -INFINITY;
+                    }
+                }
+            }
+
+            // ---- the values' scales, and whether the maximum or the bias has to move ----
+            uint32_t vs[SG * 2][NB];
+            __half2 big = as_h2(0u);
+#pragma unroll
+            for (int j = 0; j < SG * 2; ++j) {
+                load_scales<NB>(stage + j / 2 * L.bytes + L.v_scales, j % 2 * 8 + 2 * t, vs[j]);
+                if (edge) {  // what no row of the tile sees may hold anything
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const uint32_t in = j * 8 + 2 * t + e, key = key0 + in;
+                        if (in >= here || key < tile_low || key > tile_high) {
+#pragma unroll
+                            for (int k = 0; k < NB / 2; ++k) vs[j][e * NB / 2 + k] = 0u;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < NB; ++k) big = __hmax2(big, __habs2(as_h2(vs[j][k])));  // a NaN loses
+            }
+            const float2 big2 = __half22float2(big);
+            const float dmax = fmaxf(big2.x, big2.y);
+            float top = s[0][0];
+#pragma unroll
+            for (int j = 0; j < SG * 2; ++j) top = fmaxf(top, fmaxf(s[j][0], s[j][1]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            if (__any_sync(0xffffffffu, top > m + 8.0f || dmax * bias > 2.0f)) {
+                float d = fmaxf(dmax, __shfl_xor_sync(0xffffffffu, dmax, 1));
+                d = fmaxf(d, __shfl_xor_sync(0xffffffffu, d, 2));
+                const float next = fmaxf(m, top);
+                const float bias_next = d * bias > 2.0f ? scalbnf(1.0f, 127 - (int)(__float_as_uint(fminf(d, 65504.0f)) >> 23)) : bias;
+                const float fl = m == -INFINITY ? 0.0f : exp2_approx(m - next), f = fl * (bias_next / bias);
+                bias = bias_next;
+                m = next;
+                l *= fl;
+#pragma unroll
+                for (int k = 0; k < NT; ++k) { o[k][0] *= f; o[k][1] *= f; o[k][2] *= f; o[k][3] *= f; }
+            }
+            const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int j = 0; j < SG * 2; ++j) {
+                s[j][0] = exp2_approx(s[j][0] - ref);
+                s[j][1] = exp2_approx(s[j][1] - ref);
+                l += s[j][0] + s[j][1];
+            }
+
+            // ---- p v ----
+#pragma unroll
+            for (int k = 0; k < SG; ++k) {
+                uint32_t codes[V8 ? NT : NT / 2];
+                load_words<V8 ? NT : NT / 2, L.v_vec>(stage + k * L.bytes + L.v_codes, lane, codes);
+                const float p0 = s[2 * k][0] * bias, p1 = s[2 * k][1] * bias, p2 = s[2 * k + 1][0] * bias, p3 = s[2 * k + 1][1] * bias;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    float x0 = p0 * scale_of<NB>(vs[2 * k], 0, b), x1 = p1 * scale_of<NB>(vs[2 * k], 1, b);
+                    float x2 = p2 * scale_of<NB>(vs[2 * k + 1], 0, b), x3 = p3 * scale_of<NB>(vs[2 * k + 1], 1, b);
+                    if (edge) {  // a position that this row does not see, another does, and whose scale is a NaN
+                        if (p0 == 0.0f) x0 = 0.0f;
+                        if (p1 == 0.0f) x1 = 0.0f;
+                        if (p2 == 0.0f) x2 = 0.0f;
+                        if (p3 == 0.0f) x3 = 0.0f;
+                    }
+                    uint4 a;
+                    a.x = pack_hi_lo(x0, x1, a.y);
+                    a.z = pack_hi_lo(x2, x3, a.w);
+                    if (V8) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) mma(o[4 * b + q], a, byte_codes(codes[4 * b + q], 0x4140), byte_codes(codes[4 * b + q], 0x4342));
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            const uint32_t w = codes[2 * b + q], w8 = w >> 8;
+                            mma(o[4 * b + 2 * q], a, low_codes(w), low_codes(w8));
+                            mma(o[4 * b + 2 * q + 1], a, high_codes(w), high_codes(w8));
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0 && i + STAGES < mystages) request(i + STAGES);
+        }
+        turn += mystages;
+
+        // ---- join the warps ----
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        if (!__syncthreads_and(alive)) return;  // every warp is done with the ring, which the accumulators now take
+        if (t == 0) { join_m[warp * ROWS + g] = m; join_l[warp * ROWS + g] = l; }
+        const float back = 1.0f / bias;
+#pragma unroll
+        for (int k = 0; k < NT; ++k)
+            *(float2 *)(join + (warp * ROWS + g) * W + k * 8 + 2 * t) = make_float2(fmaf(o[k][2], LO, o[k][0]) * back, fmaf(o[k][3], LO, o[k][1]) * back);
+        __syncthreads();
+        const uint32_t used = min(stages, (uint32_t)WARPS);
+        const bool whole = n == count;
+        const unsigned long long c0 = unit_begin / sh, c1 = (unit_begin + count - 1) / sh;  // the blocks that share the unit
+        float *partial = p.partials + ((size_t)blockIdx.x * 2 + (skip == 0 && !whole)) * S::PARTIAL;  // a unit that starts here goes into the second place
+        for (uint32_t e = tid; e < ROWS * W; e += S::THREADS) {
+            const uint32_t r = e / W;
+            float top = -INFINITY, sum = 0.0f, acc = 0.0f;
+            for (uint32_t w = 0; w < used; ++w) top = fmaxf(top, join_m[w * ROWS + r]);
+            const float ref = top == -INFINITY ? 0.0f : top;
+            for (uint32_t w = 0; w < used; ++w) {
+                const float f = exp2f(join_m[w * ROWS + r] - ref);
+                sum += join_l[w * ROWS + r] * f;
+                acc += join[(w * ROWS + r) * W + e % W] * f;
+            }
+            if (whole) {
+                const uint64_t out_row = (uint64_t)tile * ROWS + r;
+                if (out_row < live_rows)
+                    store_out(p, (rows0 + out_row / p.group) * p.out_stride + (size_t)(head * p.group + (uint32_t)(out_row % p.group)) * W + e % W, acc / sum);
+            } else {
+                partial[e] = acc;
+                if (e % W == 0) { partial[ROWS * W + r] = top; partial[ROWS * W + ROWS + r] = sum; }
+            }
+        }
+        if (!whole) {
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) *word = atomicAdd(p.counters + c0, 1u) == (uint32_t)(c1 - c0);
+            __syncthreads();
+            if (*word) {
+                __threadfence();
+                for (uint32_t e = tid; e < ROWS * W; e += S::THREADS) {
+                    const uint32_t r = e / W;
+                    float top = -INFINITY, sum = 0.0f, acc = 0.0f;
+                    for (unsigned long long c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(p.partials + (c * 2 + (c == c0)) * S::PARTIAL + ROWS * W + r));
+                    const float ref = top == -INFINITY ? 0.0f : top;
+                    for (unsigned long long c = c0; c <= c1; ++c) {
+                        const float *x = p.partials + (c * 2 + (c == c0)) * S::PARTIAL;
+                        const float f = exp2f(__ldcg(x + ROWS * W + r) - ref);
+                        sum += __ldcg(x + ROWS * W + ROWS + r) * f;
+                        acc += __ldcg(x + e) * f;
+                    }
+                    const uint64_t out_row = (uint64_t)tile * ROWS + r;
+                    if (out_row < live_rows)
+                        store_out(p, (rows0 + out_row / p.group) * p.out_stride + (size_t)(head * p.group + (uint32_t)(out_row % p.group)) * W + e % W, acc / sum);
+                }
+                if (tid == 0) p.counters[c0] = 0;
+            }
+        }
+        at += n;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the ring's bytes go back to the copies
+        __syncthreads();
+    }
+}
+
+template <int W, bool K8, bool V8>
+bool configure() {
+    return cudaFuncSetAttribute(split_kernel<W, K8, V8>, cudaFuncAttributeMaxDynamicSharedMemorySize, Split<W, K8, V8>::SMEM) == cudaSuccess;
+}
+template <int W, bool K8, bool V8>
+int launch(cudaStream_t s, const AttentionParams &p, int sm_count) {
+    using S = Split<W, K8, V8>;
+    launch_after_previous_smem(split_kernel<W, K8, V8>, dim3(sm_count), dim3(S::THREADS), S::SMEM, s, p);
+    return 1;
+}
+#define NU_EVERY(F, W, ...) (k8 ? (v8 ? F<W, true, true>(__VA_ARGS__) : F<W, true, false>(__VA_ARGS__)) : (v8 ? F<W, false, true>(__VA_ARGS__) : F<W, false, false>(__VA_ARGS__)))
+
+}  // namespace
+
+bool attention_configure() {
+    bool ok = true;
+    for (int i = 0; i < 4; ++i) {
+        const bool k8 = i & 1, v8 = i & 2;
+        ok = ok && NU_EVERY(configure, 64) && NU_EVERY(configure, 128) && NU_EVERY(configure, 256);
+    }
+    return ok;
+}
+
+int launch_attention(cudaStream_t s, const AttentionJob &j) {
+    const bool k8 = j.cache.k8, v8 = j.cache.v8;
+    const uint32_t width = j.cache.width;
+    AttentionParams p{};
+    p.c = {j.cache.base, kv_layout(width, k8, v8), j.cache.slots, j.cache.heads, j.cache.capacity / KV_GRANULE, j.cache.status};
+    p.spans = (const KvSpan *)j.spans;
+    p.sequences = j.sequences; p.tokens = j.tokens;
+    p.q = j.queries; p.q_stride = j.q_stride;
+    p.group = j.heads / j.cache.heads;
+    p.tiles = (uint32_t)(((uint64_t)j.tokens * p.group + ROWS - 1) / ROWS);
+    p.out = j.out; p.out_stride = j.out_stride; p.bf16 = j.bf16;
+    p.scale = j.scale * 1.4426950408889634f;
+    p.window = j.window;
+    p.partials = j.partials; p.counters = j.counters;
+    if (!j.generic && width == 64) return NU_EVERY(launch, 64, s, p, j.sm_count);
+    if (!j.generic && width == 128) return NU_EVERY(launch, 128, s, p, j.sm_count);
+    if (!j.generic && width == 256) return NU_EVERY(launch, 256, s, p, j.sm_count);
+    const size_t items = (size_t)j.sequences * j.tokens * j.heads;
+    launch_after_previous(generic_kernel, dim3((unsigned)((items + GENERIC_WARPS - 1) / GENERIC_WARPS)), dim3(GENERIC_WARPS * 32), s, p);
+    return 1;
+}
+
+}  // namespace nu
