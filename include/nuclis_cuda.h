@@ -353,7 +353,7 @@ typedef struct nu_kv_span {
 } nu_kv_span;
 
 /* Quantizes rows of keys and values (F32, [heads][width] contiguous within a row, strides in floats) into the cache. The
- * rule is GGUF's, in F32: Q8_0 d = amax / 127, code = round(x * (1 / d)); Q4_0 d = m / -8 with m the first value of the largest
+ * rule is GGUF's, in F32: Q8_0 d = amax * (1 / 127), code = round(x * (1 / d)); Q4_0 d = m / -8 with m the first value of the largest
  * magnitude, code = min(15, trunc(x * (1 / d) + 8.5)); d is stored as f16. A scale beyond f16 saturates, a block with a NaN or
  * an infinity reads back as NaN. Where two spans of one call cover the same position, the later span's row is kept. */
 int nu_cuda_kv_write(nu_cuda *h, const nu_buffer *buffer, const nu_kv_cache *cache, const nu_buffer *spans, size_t sequences, size_t tokens,

@@ -72,6 +72,7 @@ Backend *Backend::create(int device, std::string &error) {
     ok = ok && cudaMalloc(&b->partials_, kPartialsFloats * sizeof(float)) == cudaSuccess;
     ok = ok && cudaMalloc(&b->counters_, (kCounters + 3) * sizeof(uint32_t)) == cudaSuccess;
     ok = ok && cudaMemset(b->counters_, 0, (kCounters + 3) * sizeof(uint32_t)) == cudaSuccess;
+    ok = ok && cudaMallocHost(&b->status_host_, sizeof(uint32_t)) == cudaSuccess;
     ok = ok && cudaMalloc(&b->argmax_records_, (128 * 4 + 4) * sizeof(float)) == cudaSuccess;
     ok = ok && cudaMemset(b->argmax_records_, 0, (128 * 4 + 4) * sizeof(float)) == cudaSuccess;
     if (!ok) {
@@ -104,6 +105,7 @@ Backend::~Backend() {
     if (partials_) cudaFree(partials_);
     if (counters_) cudaFree(counters_);
     if (argmax_records_) cudaFree(argmax_records_);
+    if (status_host_) cudaFreeHost(status_host_);
     if (ev_start_) cudaEventDestroy(ev_start_);
     if (ev_stop_) cudaEventDestroy(ev_stop_);
     if (stream_) cudaStreamDestroy(stream_);
@@ -322,10 +324,12 @@ int Backend::finishCapture(cudaGraphExec_t *exec) {
     return cuda(e, "commit: instantiate");
 }
 
+// Waits for everything enqueued so far and reads the kernels' status word: into pinned memory, so that the copy runs behind the
+// kernels and one wait serves both (a copy to pageable memory after the wait cost a second one, 8 us a replay).
 int Backend::checkKernelStatus() {
-    uint32_t status = 0;
-    if (int rc = cuda(cudaMemcpyAsync(&status, counters_ + counters_len_, sizeof status, cudaMemcpyDeviceToHost, stream_), "status read")) return rc;
-    if (int rc = cuda(cudaStreamSynchronize(stream_), "status sync")) return rc;
+    if (int rc = cuda(cudaMemcpyAsync(status_host_, counters_ + counters_len_, sizeof *status_host_, cudaMemcpyDeviceToHost, stream_), "status read")) return rc;
+    if (int rc = cuda(cudaStreamSynchronize(stream_), "launch: wait")) return rc;
+    const uint32_t status = *status_host_;
     if (status != 0) {
         cudaMemsetAsync(counters_, 0, (counters_len_ + 3) * sizeof(uint32_t), stream_);  // counters, status word, the chain kernel's two arrival counts
         cudaStreamSynchronize(stream_);
@@ -340,12 +344,12 @@ int Backend::runGraph(cudaGraphExec_t exec, uint32_t count, float *elapsed_ms) {
     for (uint32_t i = 0; i < count; ++i)
         if (int rc = cuda(cudaGraphLaunch(exec, stream_), "launch")) return rc;
     if (int rc = cuda(cudaEventRecord(ev_stop_, stream_), "launch: event")) return rc;
-    if (int rc = cuda(cudaStreamSynchronize(stream_), "launch: wait")) return rc;
+    const int rc = checkKernelStatus();
     float ms = 0;
-    cudaEventElapsedTime(&ms, ev_start_, ev_stop_);
+    if (cudaEventElapsedTime(&ms, ev_start_, ev_stop_) != cudaSuccess) return rc ? rc : fail(NU_ERR_EXECUTION, "launch: elapsed time");
     gpu_seconds_ += ms * 1e-3;
     if (elapsed_ms) *elapsed_ms = ms;
-    return checkKernelStatus();
+    return rc;
 }
 
 int Backend::commit() {

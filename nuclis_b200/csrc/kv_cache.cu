@@ -1,7 +1,7 @@
 // Writing rows of keys and values into the quantized cache, and reading them back. Both are one pass over the rows:
 // bound by memory for a prompt, by the launch for a single row.
 //
-// The rule of a block of 32 (GGUF's, in F32 arithmetic): Q8_0 d = amax / 127, code = round(x * (1 / d)) with halves away
+// The rule of a block of 32 (GGUF's, in F32 arithmetic): Q8_0 d = amax * (1 / 127), code = round(x * (1 / d)) with halves away
 // from zero; Q4_0 d = m / -8 with m the first value of the largest magnitude, code = min(15, trunc(x * (1 / d) + 8.5)).
 // The stored scale is d rounded to f16. A block whose scale rounds to zero stores zeros; one whose scale passes the f16
 // range stores the largest scale and saturated codes; one that holds a NaN or an infinity stores a NaN scale, so that it
@@ -35,7 +35,7 @@ __device__ __forceinline__ uint32_t quantize4(const float x[4], float &scale) {
         bad |= __shfl_xor_sync(0xffffffffu, (int)bad, o) != 0;
         if (lower ? fabsf(other) >= fabsf(top) : fabsf(other) > fabsf(top)) top = other;
     }
-    float d = Q8 ? __fdiv_rn(fabsf(top), 127.0f) : top * -0.125f;
+    float d = Q8 ? __fmul_rn(fabsf(top), 1.0f / 127.0f) : top * -0.125f;
     d = fminf(fmaxf(d, -65504.0f), 65504.0f);
     scale = bad ? NAN : d;
     const float inverse = bad || __half2float(__float2half_rn(d)) == 0.0f ? 0.0f : __fdiv_rn(1.0f, d);

@@ -12,7 +12,7 @@ def quantize(x, encoding):
     f = np.float32
     with np.errstate(all="ignore"):
         if encoding == enc.Q8_0:
-            d = (np.max(np.abs(b), axis=-1) / f(127)).astype(np.float32)
+            d = (np.max(np.abs(b), axis=-1) * (f(1) / f(127))).astype(np.float32)
         else:
             at = np.argmax(np.abs(b), axis=-1)
             d = (np.take_along_axis(b, at[..., None], -1)[..., 0] / f(-8)).astype(np.float32)
