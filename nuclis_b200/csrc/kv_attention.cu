@@ -522,46 +522,82 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 1) split_kernel(con
         const bool whole = n == count;
         const unsigned long long c0 = unit_begin / sh, c1 = (unit_begin + count - 1) / sh;  // the blocks that share the unit
         float *partial = p.partials + ((size_t)blockIdx.x * 2 + (skip == 0 && !whole)) * S::PARTIAL;  // a unit that starts here goes into the second place
-        for (uint32_t e = tid; e < ROWS * W; e += S::THREADS) {
-            const uint32_t r = e / W;
-            float top = -INFINITY, sum = 0.0f, acc = 0.0f;
-            for (uint32_t w = 0; w < used; ++w) top = fmaxf(top, join_m[w * ROWS + r]);
+        // a row's parts are weighted by 2^(their maximum - the row's): found once, by one thread a row
+        if (tid < ROWS) {
+            float top = -INFINITY, sum = 0.0f;
+            for (uint32_t w = 0; w < used; ++w) top = fmaxf(top, join_m[w * ROWS + tid]);
             const float ref = top == -INFINITY ? 0.0f : top;
             for (uint32_t w = 0; w < used; ++w) {
-                const float f = exp2f(join_m[w * ROWS + r] - ref);
-                sum += join_l[w * ROWS + r] * f;
-                acc += join[(w * ROWS + r) * W + e % W] * f;
+                const float f = exp2f(join_m[w * ROWS + tid] - ref);
+                sum += join_l[w * ROWS + tid] * f;
+                join_m[w * ROWS + tid] = f;
             }
             if (whole) {
-                const uint64_t out_row = (uint64_t)tile * ROWS + r;
-                if (out_row < live_rows)
-                    store_out(p, (rows0 + out_row / p.group) * p.out_stride + (size_t)(head * p.group + (uint32_t)(out_row % p.group)) * W + e % W, acc / sum);
+                row_scale[tid] = 1.0f / sum;
             } else {
-                partial[e] = acc;
-                if (e % W == 0) { partial[ROWS * W + r] = top; partial[ROWS * W + ROWS + r] = sum; }
+                partial[ROWS * W + tid] = top;
+                partial[ROWS * W + ROWS + tid] = sum;
             }
+        }
+        __syncthreads();
+        auto put = [&](uint32_t e, float4 x) {  // four values of a row of the result
+            const uint32_t r = e / W;
+            const uint64_t out_row = (uint64_t)tile * ROWS + r;
+            if (out_row >= live_rows) return;
+            const float f = row_scale[r];
+            const size_t i = (rows0 + out_row / p.group) * p.out_stride + (size_t)(head * p.group + (uint32_t)(out_row % p.group)) * W + e % W;
+            store_out(p, i, x.x * f);
+            store_out(p, i + 1, x.y * f);
+            store_out(p, i + 2, x.z * f);
+            store_out(p, i + 3, x.w * f);
+        };
+        for (uint32_t e = tid * 4; e < ROWS * W; e += S::THREADS * 4) {
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (uint32_t w = 0; w < used; ++w) {
+                const float f = join_m[w * ROWS + e / W];
+                const float4 x = *(const float4 *)(join + w * ROWS * W + e);
+                acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y); acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
+            }
+            if (whole) put(e, acc);
+            else *(float4 *)(partial + e) = acc;
         }
         if (!whole) {
             __threadfence();
             __syncthreads();
             if (tid == 0) *word = atomicAdd(p.counters + c0, 1u) == (uint32_t)(c1 - c0);
             __syncthreads();
-            if (*word) {
+            if (*word) {  // this block arrived last: the parts of all blocks, in their order
                 __threadfence();
-                for (uint32_t e = tid; e < ROWS * W; e += S::THREADS) {
-                    const uint32_t r = e / W;
-                    float top = -INFINITY, sum = 0.0f, acc = 0.0f;
-                    for (unsigned long long c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(p.partials + (c * 2 + (c == c0)) * S::PARTIAL + ROWS * W + r));
+                const uint32_t parts = (uint32_t)(c1 - c0) + 1;
+                const float *first_part = p.partials + (c0 * 2 + 1) * S::PARTIAL, *other = p.partials + (c0 + 1) * 2 * S::PARTIAL;
+                auto part = [&](uint32_t c) { return c ? other + (size_t)(c - 1) * 2 * S::PARTIAL : first_part; };
+                float *weight = join;  // [parts][ROWS], then the sums
+                for (uint32_t i = tid; i < parts * ROWS; i += S::THREADS) {
+                    weight[i] = __ldcg(part(i / ROWS) + ROWS * W + i % ROWS);
+                    weight[(parts + i / ROWS) * ROWS + i % ROWS] = __ldcg(part(i / ROWS) + ROWS * W + ROWS + i % ROWS);
+                }
+                __syncthreads();
+                if (tid < ROWS) {
+                    float top = -INFINITY, sum = 0.0f;
+                    for (uint32_t c = 0; c < parts; ++c) top = fmaxf(top, weight[c * ROWS + tid]);
                     const float ref = top == -INFINITY ? 0.0f : top;
-                    for (unsigned long long c = c0; c <= c1; ++c) {
-                        const float *x = p.partials + (c * 2 + (c == c0)) * S::PARTIAL;
-                        const float f = exp2f(__ldcg(x + ROWS * W + r) - ref);
-                        sum += __ldcg(x + ROWS * W + ROWS + r) * f;
-                        acc += __ldcg(x + e) * f;
+                    for (uint32_t c = 0; c < parts; ++c) {
+                        const float f = exp2f(weight[c * ROWS + tid] - ref);
+                        sum += weight[(parts + c) * ROWS + tid] * f;
+                        weight[c * ROWS + tid] = f;
                     }
-                    const uint64_t out_row = (uint64_t)tile * ROWS + r;
-                    if (out_row < live_rows)
-                        store_out(p, (rows0 + out_row / p.group) * p.out_stride + (size_t)(head * p.group + (uint32_t)(out_row % p.group)) * W + e % W, acc / sum);
+                    row_scale[tid] = 1.0f / sum;
+                }
+                __syncthreads();
+                for (uint32_t e = tid * 4; e < ROWS * W; e += S::THREADS * 4) {
+                    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+                    for (uint32_t c = 0; c < parts; ++c) {
+                        const float f = weight[c * ROWS + e / W];
+                        const float4 x = __ldcg((const float4 *)(part(c) + e));
+                        acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y); acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
+                    }
+                    put(e, acc);
                 }
                 if (tid == 0) p.counters[c0] = 0;
             }

@@ -49,151 +49,299 @@ __device__ __forceinline__ uint32_t quantize4(const float x[4], float &scale) {
     return codes;
 }
 
-struct WriteParams {
-    KvView c;
-    const KvSpan *spans;
-    uint32_t sequences, tokens, pieces;  // a piece: 128 consecutive values of a row, one warp's
-    const float *rows[2];                // keys, values
-    size_t stride[2];
-};
-
 __device__ __forceinline__ uint32_t nibbles(uint32_t bytes) { return (bytes & 15u) | (bytes >> 4 & 0xf0u) | (bytes >> 8 & 0xf00u) | (bytes >> 12 & 0xf000u); }
 
-template <bool VALUES, bool Q8>
-__device__ __forceinline__ void write_piece(const WriteParams &p, const float *row, uint32_t piece, uint32_t slot, uint32_t pos) {
-    const uint32_t lane = threadIdx.x & 31, e = piece * 128 + lane * 4, width = p.c.l.width;
-    const bool live = e < p.c.heads * width;  // blocks are whole: the eight lanes of one are live together
-    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (live) {
-        if ((uintptr_t)(row + e) % 16 == 0) {
-            const float4 v = *(const float4 *)(row + e);
-            x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = row[e + i];
-        }
-    }
-    float scale;
-    const uint32_t codes = quantize4<Q8>(x, scale);
-    const uint32_t head = e / width, dim = e % width, b = dim / 32, at = pos % KV_GRANULE;
-    uint8_t *g = live ? kv_head(p.c, slot, head) + (size_t)(pos / KV_GRANULE) * p.c.l.bytes : nullptr;
-    const uint32_t near = __shfl_xor_sync(0xffffffffu, codes, VALUES ? 2 : 1);  // keys: the other half of eight dimensions; values: the other nibbles
-    if (!live) return;
-    if (dim % 32 == 0) *(__half *)(g + (VALUES ? p.c.l.v_scales : p.c.l.k_scales) + (at * p.c.l.blocks + b) * 2) = __float2half_rn(scale);
-    if (VALUES) {
-        if (Q8) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) g[kv_value_byte(p.c.l, at, dim + i)] = (uint8_t)(codes >> (8 * i));
-        } else if (!(dim & 8)) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) g[kv_value_byte(p.c.l, at, dim + i)] = (uint8_t)((codes >> (8 * i) & 15u) | (near >> (8 * i) & 15u) << 4);
-        }
-    } else {
-        const uint32_t t = dim % 32 / 8, second = dim / 4 % 2;
-        if (Q8) {  // bytes 0,4,1,5 by the lane of dimensions 0..3, bytes 2,6,3,7 by the other
-            const uint32_t low = second ? near : codes, high = second ? codes : near;
-            *(uint32_t *)(g + kv_key_word(p.c.l, at, b, t, second)) = __byte_perm(low, high, second ? 0x7362 : 0x5140);
-        } else if (!second) {
-            *(uint32_t *)(g + kv_key_word(p.c.l, at, b, t, 0)) = nibbles(codes) | nibbles(near) << 16;
-        }
-    }
-}
-
-// One warp a piece of a row. Where two spans of a call cover the same position, the row of the later span is written.
-__global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(const WriteParams p) {
-    wait_for_previous_operator();
-    const uint32_t lane = threadIdx.x & 31;
-    const size_t item = (size_t)blockIdx.x * (KV_THREADS / 32) + threadIdx.x / 32;
-    const uint32_t which = (uint32_t)(item % 2), piece = (uint32_t)(item / 2 % p.pieces);
-    const size_t r = item / 2 / p.pieces;
-    if (r >= (size_t)p.sequences * p.tokens) return;
-    const uint32_t sequence = (uint32_t)(r / p.tokens), i = (uint32_t)(r % p.tokens);
-    const KvSpan span = kv_span(p.c, p.spans, sequence, p.tokens);
-    if (i >= span.count) return;
-    const uint32_t pos = span.first + i;
-    for (uint32_t later = sequence + 1; later < p.sequences; later += 32) {
-        bool covered = false;
-        if (later + lane < p.sequences) {
-            const KvSpan s = kv_span(p.c, p.spans, later + lane, p.tokens);
-            covered = s.slot == span.slot && pos >= s.first && pos - s.first < s.count;
-        }
-        if (__any_sync(0xffffffffu, covered)) return;
-    }
-    const float *row = p.rows[which] + r * p.stride[which];
-    if (which) {
-        if (p.c.l.v8) write_piece<true, true>(p, row, piece, span.slot, pos);
-        else write_piece<true, false>(p, row, piece, span.slot, pos);
-    } else {
-        if (p.c.l.k8) write_piece<false, true>(p, row, piece, span.slot, pos);
-        else write_piece<false, false>(p, row, piece, span.slot, pos);
-    }
-}
-
-struct ReadParams {
-    KvView c;
-    const KvSpan *spans;
-    uint32_t sequences, tokens, pieces;
-    void *rows[2];
-    size_t stride[2];
-    bool bf16;
+// Both kernels give one warp the share of a granule (16 positions) that a piece of up to 128 dimensions of one head's keys
+// or values has, of one sequence: the rows' side is then read or written in whole 512-byte runs, and so is the cache's,
+// whose order puts four positions into one word of the values. A granule that the span covers in part is written byte by
+// byte where a word has other positions in it.
+struct Item {
+    KvSpan span;
+    uint32_t sequence, granule, head, dim0, dims;  // dimensions [dim0, dim0 + dims) of the head
+    uint32_t which;                                // 0: keys, 1: values
+    uint32_t live;                                 // bit i: position i of the granule is in the span
 };
 
-// One warp a piece of a row, a lane four values of it.
-__global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const ReadParams p) {
-    wait_for_previous_operator();
-    const uint32_t lane = threadIdx.x & 31;
-    const size_t item = (size_t)blockIdx.x * (KV_THREADS / 32) + threadIdx.x / 32;
-    const uint32_t which = (uint32_t)(item % 2), piece = (uint32_t)(item / 2 % p.pieces);
-    const size_t r = item / 2 / p.pieces;
-    if (r >= (size_t)p.sequences * p.tokens) return;
-    const uint32_t sequence = (uint32_t)(r / p.tokens), i = (uint32_t)(r % p.tokens);
-    const KvSpan span = kv_span(p.c, p.spans, sequence, p.tokens);
-    const uint32_t e = piece * 128 + lane * 4, width = p.c.l.width;
-    if (i >= span.count || e >= p.c.heads * width) return;
-    const uint32_t pos = span.first + i, at = pos % KV_GRANULE, head = e / width, dim = e % width, b = dim / 32;
-    const uint8_t *g = kv_head(p.c, span.slot, head) + (size_t)(pos / KV_GRANULE) * p.c.l.bytes;
-    const float d = __half2float(*(const __half *)(g + (which ? p.c.l.v_scales : p.c.l.k_scales) + (at * p.c.l.blocks + b) * 2));
-    float x[4];
+struct RowsParams {
+    KvView c;
+    const KvSpan *spans;
+    uint32_t sequences, tokens, pieces;  // pieces of a head's width
+    uint32_t granules;                   // that a span of `tokens` rows can touch
+    void *rows[2];                       // keys, values
+    size_t stride[2];
+};
+
+__device__ __forceinline__ bool item_of(const RowsParams &p, size_t index, Item &it) {
+    it.which = (uint32_t)(index & 1);
+    index >>= 1;
+    it.dim0 = (uint32_t)(index % p.pieces) * 128;
+    index /= p.pieces;
+    it.head = (uint32_t)(index % p.c.heads);
+    index /= p.c.heads;
+    it.granule = (uint32_t)(index % p.granules);
+    it.sequence = (uint32_t)(index / p.granules);
+    if (it.sequence >= p.sequences) return false;
+    it.dims = min(128u, p.c.l.width - it.dim0);
+    it.span = kv_span(p.c, p.spans, it.sequence, p.tokens);
+    if (it.span.count == 0) return false;
+    it.granule += it.span.first / KV_GRANULE;
+    const uint32_t p0 = it.granule * KV_GRANULE, end = it.span.first + it.span.count;
+    if (p0 >= end) return false;
+    const uint32_t low = it.span.first > p0 ? it.span.first - p0 : 0, high = min(KV_GRANULE, end - p0);
+    it.live = (0xffffu >> (16 - high)) & (0xffffu << low);
+    return true;
+}
+
+// A 4 x 4 transposition of bytes: word i of the result has byte i of each of the four words, in their order.
+__device__ __forceinline__ void transpose_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t (&out)[4]) {
+    const uint32_t ab = __byte_perm(a, b, 0x5140), cd = __byte_perm(c, d, 0x5140), ab2 = __byte_perm(a, b, 0x7362), cd2 = __byte_perm(c, d, 0x7362);
+    out[0] = __byte_perm(ab, cd, 0x5410);
+    out[1] = __byte_perm(ab, cd, 0x7632);
+    out[2] = __byte_perm(ab2, cd2, 0x5410);
+    out[3] = __byte_perm(ab2, cd2, 0x7632);
+}
+
+constexpr int KV_WARPS = KV_THREADS / 32;
+
+template <bool VALUES, bool Q8>
+__device__ __forceinline__ void write_item(const RowsParams &p, const Item &it, uint32_t (&words)[512], __half (&scales)[64]) {
+    const KvLayout &l = p.c.l;
+    const uint32_t lane = threadIdx.x & 31, mine = lane * 4;
+    const bool live = mine < it.dims;  // blocks are whole: the eight lanes of one are live together
+    const uint32_t dim = it.dim0 + mine, b = dim / 32;
+    // row of position 0 of the granule, before the rows' start where the span begins inside it; only live positions are read
+    const float *row0 = (const float *)p.rows[VALUES] + ((ptrdiff_t)it.sequence * p.tokens + (ptrdiff_t)it.granule * KV_GRANULE - it.span.first) * (ptrdiff_t)p.stride[VALUES] +
+                        (size_t)it.head * l.width + dim;
+    uint8_t *g = kv_head(p.c, it.span.slot, it.head) + (size_t)it.granule * l.bytes;
+    const bool aligned = ((uintptr_t)row0 | p.stride[VALUES] * 4) % 16 == 0;
+    uint32_t codes[KV_GRANULE];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        int code;
-        if (which) {
-            const uint32_t byte = g[kv_value_byte(p.c.l, at, dim + k)];
-            code = p.c.l.v8 ? (int)byte - 128 : (int)(byte >> (dim & 8 ? 4 : 0) & 15u) - 8;
-        } else if (p.c.l.k8) {
-            const uint32_t w = *(const uint32_t *)(g + kv_key_word(p.c.l, at, b, dim % 32 / 8, k / 2));
-            code = (int)(w >> (8 * (k % 2 * 2 + dim / 4 % 2)) & 255u) - 128;
-        } else {
-            const uint32_t w = *(const uint32_t *)(g + kv_key_word(p.c.l, at, b, dim % 32 / 8, 0));
-            code = (int)(w >> (4 * (dim % 8 + k)) & 15u) - 8;
+    for (int half = 0; half < 2; ++half) {
+        float x[8][4];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int at = half * 8 + i;
+            x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.0f;
+            if ((it.live >> at & 1u) && live) {
+                const float *row = row0 + (ptrdiff_t)at * (ptrdiff_t)p.stride[VALUES];
+                if (aligned) {
+                    const float4 v = __ldcs((const float4 *)row);
+                    x[i][0] = v.x; x[i][1] = v.y; x[i][2] = v.z; x[i][3] = v.w;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) x[i][k] = row[k];
+                }
+            }
         }
-        x[k] = __fmul_rn(d, (float)code);
-    }
-    const size_t out = r * p.stride[which] + e;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        if (p.bf16) ((__nv_bfloat16 *)p.rows[which])[out + k] = __float2bfloat16_rn(x[k]);
-        else ((float *)p.rows[which])[out + k] = x[k];
+        for (int i = 0; i < 8; ++i) {
+            const int at = half * 8 + i;
+            codes[at] = 0;
+            if (!(it.live >> at & 1u)) continue;  // the same for the whole warp
+            float scale;
+            codes[at] = quantize4<Q8>(x[i], scale);
+            if (lane % 8 == 0 && live) scales[at * 4 + lane / 8] = __float2half_rn(scale);
+            if (!VALUES) {
+                const uint32_t near = __shfl_xor_sync(0xffffffffu, codes[at], 1);  // the other half of eight dimensions
+                const uint32_t t = dim % 32 / 8, second = dim / 4 % 2;
+                if (live && Q8) {  // bytes 0,4,1,5 by the lane of dimensions 0..3, bytes 2,6,3,7 by the other
+                    const uint32_t low = second ? near : codes[at], high = second ? codes[at] : near;
+                    *(uint32_t *)(g + kv_key_word(l, at, b, t, second)) = __byte_perm(low, high, second ? 0x7362 : 0x5140);
+                } else if (live && !second) {
+                    *(uint32_t *)(g + kv_key_word(l, at, b, t, 0)) = nibbles(codes[at]) | nibbles(near) << 16;
+                }
+            }
+        }
+    }
+    __syncwarp();
+    uint8_t *gs = g + (VALUES ? l.v_scales : l.k_scales);
+    const uint32_t blocks = it.dims / 32;
+    if (it.live == 0xffffu && l.blocks == 4) {
+        ((uint32_t *)gs)[lane] = ((const uint32_t *)scales)[lane];
+    } else {
+        for (uint32_t i = lane; i < KV_GRANULE * blocks; i += 32)
+            if (it.live >> (i / blocks) & 1u) ((__half *)gs)[i / blocks * l.blocks + it.dim0 / 32 + i % blocks] = scales[i / blocks * 4 + i % blocks];
+    }
+    if (!VALUES) return;
+
+    // this lane's words: four dimensions (four codes a byte of theirs, or with the partner's as nibbles), four groups of positions
+    const uint32_t per = Q8 ? it.dims / 8 : it.dims / 16;  // words of a lane slot
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        uint32_t c[4];
+        transpose_bytes(codes[2 * t], codes[2 * t + 1], codes[8 + 2 * t], codes[9 + 2 * t], c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t w = c[i];
+            if (!Q8) {
+                w = __byte_perm(w, 0, 0x3120);  // 2t, 8 + 2t, 2t + 1, 9 + 2t
+                w |= __shfl_xor_sync(0xffffffffu, w, 2) << 4;
+            }
+            const uint32_t word = mine / (Q8 ? 8 : 16), slot = ((mine + i) % 8) * 4 + t;
+            // vectors of four words a slot, as the cache keeps them
+            if (live && (Q8 || !(mine & 8))) words[word / 4 * 128 + slot * 4 + word % 4] = w;
+        }
+    }
+    __syncwarp();
+    const uint32_t word0 = Q8 ? it.dim0 / 8 : it.dim0 / 16;
+    if (it.live == 0xffffu && l.v_vec == 16 && per % 4 == 0) {
+        for (uint32_t v = 0; v < per / 4; ++v) *(uint4 *)(g + l.v_codes + (word0 / 4 + v) * 512 + lane * 16) = *(const uint4 *)&words[v * 128 + lane * 4];
+    } else {
+        const uint32_t t = lane % 4;
+        for (uint32_t w = 0; w < per; ++w) {
+            const uint32_t x = words[w / 4 * 128 + lane * 4 + w % 4];
+            uint8_t *dst = g + l.v_codes + kv_word(l.v_vec, lane, word0 + w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t at = Q8 ? 2 * t + (i & 1) + (i >> 1) * 8 : 2 * t + (i >> 1) + (i & 1) * 8;
+                if (it.live >> at & 1u) dst[i] = (uint8_t)(x >> (8 * i));
+            }
+        }
+    }
+}
+
+__global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(const RowsParams p) {
+    __shared__ __align__(16) uint32_t words[KV_WARPS][512];
+    __shared__ __align__(16) __half scales[KV_WARPS][64];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+    wait_for_previous_operator();
+    Item it;
+    if (!item_of(p, (size_t)blockIdx.x * KV_WARPS + warp, it)) return;
+    // where two spans of a call cover the same position, the row of the later span is written
+    for (uint32_t later = it.sequence + 1; later < p.sequences; later += 32) {
+        uint32_t covered = 0;
+        if (later + lane < p.sequences) {
+            const KvSpan s = kv_span(p.c, p.spans, later + lane, p.tokens);
+            if (s.count && s.slot == it.span.slot)
+                for (uint32_t i = 0; i < KV_GRANULE; ++i) covered |= (uint32_t)(it.granule * KV_GRANULE + i >= s.first && it.granule * KV_GRANULE + i - s.first < s.count) << i;
+        }
+        it.live &= ~__reduce_or_sync(0xffffffffu, covered);
+    }
+    if (it.which) {
+        if (p.c.l.v8) write_item<true, true>(p, it, words[warp], scales[warp]);
+        else write_item<true, false>(p, it, words[warp], scales[warp]);
+    } else {
+        if (p.c.l.k8) write_item<false, true>(p, it, words[warp], scales[warp]);
+        else write_item<false, false>(p, it, words[warp], scales[warp]);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ T out_value(float x);
+template <>
+__device__ __forceinline__ float out_value<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 out_value<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// Decoded rows of a piece, padded so that the values' scattered stores meet no bank twice.
+template <typename T>
+struct Staged {
+    static constexpr int ROW = 128 + 16 / sizeof(T);
+    T x[KV_GRANULE][ROW];
+};
+
+template <bool VALUES, bool Q8, typename T>
+__device__ __forceinline__ void read_item(const RowsParams &p, const Item &it, Staged<T> &st) {
+    const KvLayout &l = p.c.l;
+    const uint32_t lane = threadIdx.x & 31, slot = lane / 4, t = lane % 4, b0 = it.dim0 / 32;
+    const uint8_t *g = kv_head(p.c, it.span.slot, it.head) + (size_t)it.granule * l.bytes;
+    const __half *scales = (const __half *)(g + (VALUES ? l.v_scales : l.k_scales)) + b0;
+    if (VALUES) {
+        for (uint32_t b = 0; b < it.dims / 32; ++b) {
+            float d[4];  // of positions 2t, 2t + 1, 8 + 2t, 9 + 2t
+#pragma unroll
+            for (int i = 0; i < 4; ++i) d[i] = __half2float(scales[(2 * t + (i & 1) + (i >> 1) * 8) * l.blocks + b]);
+#pragma unroll
+            for (int w = 0; w < (Q8 ? 4 : 2); ++w) {
+                const uint32_t word = *(const uint32_t *)(g + l.v_codes + kv_word(l.v_vec, lane, (b0 + b) * (Q8 ? 4 : 2) + w));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t at = 2 * t + (i & 1) + (i >> 1) * 8;
+                    if (Q8) {
+                        st.x[at][b * 32 + w * 8 + slot] = out_value<T>(__fmul_rn(d[i], (float)((int)(word >> (8 * i) & 255u) - 128)));
+                    } else {
+                        const uint32_t byte = word >> (8 * ((i & 1) * 2 + (i >> 1)));
+                        st.x[at][b * 32 + w * 16 + slot] = out_value<T>(__fmul_rn(d[i], (float)((int)(byte & 15u) - 8)));
+                        st.x[at][b * 32 + w * 16 + 8 + slot] = out_value<T>(__fmul_rn(d[i], (float)((int)(byte >> 4 & 15u) - 8)));
+                    }
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t at = j * 8 + slot;
+            for (uint32_t b = 0; b < it.dims / 32; ++b) {
+                const float d = __half2float(scales[at * l.blocks + b]);
+                const uint32_t w0 = *(const uint32_t *)(g + kv_key_word(l, at, b0 + b, t, 0)), w1 = Q8 ? *(const uint32_t *)(g + kv_key_word(l, at, b0 + b, t, 1)) : 0u;
+                alignas(16) T x[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int code = Q8 ? (int)((i % 4 < 2 ? w0 : w1) >> (8 * (i % 2 * 2 + i / 4)) & 255u) - 128 : (int)(w0 >> (4 * i) & 15u) - 8;
+                    x[i] = out_value<T>(__fmul_rn(d, (float)code));
+                }
+#pragma unroll
+                for (int v = 0; v < (int)sizeof(x) / 16; ++v) *(uint4 *)((uint8_t *)&st.x[at][b * 32 + t * 8] + v * 16) = ((const uint4 *)x)[v];
+            }
+        }
+    }
+    __syncwarp();
+    // the rows, as whole runs
+    T *row0 = (T *)p.rows[VALUES] + ((ptrdiff_t)it.sequence * p.tokens + (ptrdiff_t)it.granule * KV_GRANULE - it.span.first) * (ptrdiff_t)p.stride[VALUES] +
+              (size_t)it.head * l.width + it.dim0;
+    constexpr uint32_t V = 16 / sizeof(T);
+    const uint32_t lanes = it.dims / V;  // vectors of a row
+    if (((uintptr_t)row0 | p.stride[VALUES] * sizeof(T)) % 16 == 0) {
+        for (uint32_t i = lane; i < KV_GRANULE * lanes; i += 32) {
+            const uint32_t at = i / lanes, v = i % lanes;
+            if (it.live >> at & 1u) *(uint4 *)(row0 + (ptrdiff_t)at * (ptrdiff_t)p.stride[VALUES] + v * V) = *(const uint4 *)&st.x[at][v * V];
+        }
+    } else {
+        for (uint32_t i = lane; i < KV_GRANULE * it.dims; i += 32) {
+            const uint32_t at = i / it.dims, d = i % it.dims;
+            if (it.live >> at & 1u) row0[(ptrdiff_t)at * (ptrdiff_t)p.stride[VALUES] + d] = st.x[at][d];
+        }
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const RowsParams p) {
+    __shared__ __align__(16) Staged<T> staged[KV_WARPS];
+    const uint32_t warp = threadIdx.x / 32;
+    wait_for_previous_operator();
+    Item it;
+    if (!item_of(p, (size_t)blockIdx.x * KV_WARPS + warp, it)) return;
+    if (it.which) {
+        if (p.c.l.v8) read_item<true, true, T>(p, it, staged[warp]);
+        else read_item<true, false, T>(p, it, staged[warp]);
+    } else {
+        if (p.c.l.k8) read_item<false, true, T>(p, it, staged[warp]);
+        else read_item<false, false, T>(p, it, staged[warp]);
     }
 }
 
 KvView view(const KvCacheJob &c) { return {c.base, kv_layout(c.width, c.k8, c.v8), c.slots, c.heads, c.capacity / KV_GRANULE, c.status}; }
 
+RowsParams rows_params(const KvCacheJob &c, const void *spans, uint32_t sequences, uint32_t tokens, void *keys, size_t key_stride, void *values, size_t value_stride) {
+    const uint32_t granules = (tokens + 2 * KV_GRANULE - 2) / KV_GRANULE;
+    return {view(c), (const KvSpan *)spans, sequences, tokens, (c.width + 127) / 128, granules, {keys, values}, {key_stride, value_stride}};
+}
+unsigned blocks_of(const RowsParams &p) { return (unsigned)(((size_t)p.sequences * p.granules * p.c.heads * p.pieces * 2 + KV_WARPS - 1) / KV_WARPS); }
+
 }  // namespace
 
 int launch_kv_write(cudaStream_t s, const KvCacheJob &c, const void *spans, uint32_t sequences, uint32_t tokens, const float *keys, size_t key_stride,
                     const float *values, size_t value_stride) {
-    WriteParams p{view(c), (const KvSpan *)spans, sequences, tokens, (c.heads * c.width + 127) / 128, {keys, values}, {key_stride, value_stride}};
-    const size_t items = (size_t)sequences * tokens * p.pieces * 2;
-    launch_after_previous(kv_write_kernel, dim3((unsigned)((items + KV_THREADS / 32 - 1) / (KV_THREADS / 32))), dim3(KV_THREADS), s, p);
+    const RowsParams p = rows_params(c, spans, sequences, tokens, (void *)keys, key_stride, (void *)values, value_stride);
+    launch_after_previous(kv_write_kernel, dim3(blocks_of(p)), dim3(KV_THREADS), s, p);
     return 1;
 }
 
 int launch_kv_read(cudaStream_t s, const KvCacheJob &c, const void *spans, uint32_t sequences, uint32_t tokens, void *keys, size_t key_stride, void *values,
                    size_t value_stride, bool bf16) {
-    ReadParams p{view(c), (const KvSpan *)spans, sequences, tokens, (c.heads * c.width + 127) / 128, {keys, values}, {key_stride, value_stride}, bf16};
-    const size_t items = (size_t)sequences * tokens * p.pieces * 2;
-    launch_after_previous(kv_read_kernel, dim3((unsigned)((items + KV_THREADS / 32 - 1) / (KV_THREADS / 32))), dim3(KV_THREADS), s, p);
+    const RowsParams p = rows_params(c, spans, sequences, tokens, keys, key_stride, values, value_stride);
+    if (bf16) launch_after_previous(kv_read_kernel<__nv_bfloat16>, dim3(blocks_of(p)), dim3(KV_THREADS), s, p);
+    else launch_after_previous(kv_read_kernel<float>, dim3(blocks_of(p)), dim3(KV_THREADS), s, p);
     return 1;
 }
 
