@@ -214,34 +214,118 @@ __device__ __forceinline__ float scale_of(const uint32_t (&w)[NB], int e, int b)
 
 template <int W, bool K8, bool V8>
 struct Split {
-    static constexpr int WARPS = 8, THREADS = WARPS * 32;
+    // Two blocks share a multiprocessor, so that one's prologue and join run under the other's main loop; a thread holds W/2
+    // accumulators, which leaves room for eight warps a block at 128 registers, or four at 255.
+    static constexpr int WARPS = W == 256 ? 4 : 8, THREADS = WARPS * 32, RESIDENT = 2;
     static constexpr int NB = W / 32, KT = W / 16, NT = W / 8;
     static constexpr KvLayout L = kv_layout(W, K8, V8);
-    static constexpr int SG = L.bytes <= 2560 ? 2 : 1;  // granules of a stage
+    static constexpr int SG = W == 64 ? 2 : 1;  // granules of a stage
     static constexpr int STAGE = SG * (int)L.bytes;
-    static constexpr int RING = 196 * 1024 / WARPS;
+    static constexpr int RING = (W == 256 ? 98 : 100) * 1024 / WARPS;
     static constexpr int STAGES = RING / STAGE < 8 ? RING / STAGE : 8;
     static constexpr int JOIN = WARPS * ROWS * W * 4;  // the warps' accumulators; takes the ring's place
     static constexpr int BUFFER = WARPS * STAGES * STAGE > JOIN ? WARPS * STAGES * STAGE : JOIN;
     static constexpr int FRAGMENTS = KT * 512;
     static constexpr int SMEM = BUFFER + FRAGMENTS + WARPS * STAGES * 8 + (WARPS * 2 + 1) * ROWS * 4 + 64;
     static constexpr int PARTIAL = ROWS * (W + 2);
+    // A second segment costs a block about 6 us of prologue and join; the bytes that its warps read in that time.
+    static constexpr uint32_t SEGMENT = 96 * 1024 / L.bytes;
     static_assert(STAGES >= 2, "a ring needs two stages");
+    static_assert(SMEM <= 113 * 1024, "two blocks share a multiprocessor");
 };
 
 // The granules that the rows of tile `tile` of a sequence see: [first, first + count).
 __device__ __forceinline__ void unit_range(const AttentionParams &p, const KvSpan &s, uint32_t tile, uint32_t &first, uint32_t &count) {
-    const uint64_t rows = (uint64_t)s.count * p.group, r0 = (uint64_t)tile * ROWS;
+    const uint32_t rows = s.count * p.group, r0 = tile * ROWS;  // below 2^31: the host's limit on a call's rows
     first = count = 0;
     if (r0 >= rows) return;
-    const uint64_t r1 = min(rows, r0 + ROWS) - 1;
-    const uint32_t low = s.first + (uint32_t)(r0 / p.group), high = s.first + (uint32_t)(r1 / p.group);
+    const uint32_t r1 = min(rows, r0 + ROWS) - 1;
+    const uint32_t low = s.first + r0 / p.group, high = s.first + r1 / p.group;
     first = (p.window && low >= p.window ? low - p.window + 1 : 0) / KV_GRANULE;
     count = high / KV_GRANULE + 1 - first;
 }
 
+// Where a block starts: which entry ((sequence, row tile), all of whose heads have the same granules) and how far into it.
+struct Plan {
+    bool even;                      // every block has one part of one unit; else an equal share of all granules
+    unsigned long long share, total;
+    uint32_t entry, in;             // in: blocks (even) or granules into the entry
+    bool idle;
+};
+
+// One warp's finding, the same in every warp: no barrier. Lanes take entries in turn.
+template <uint32_t SEGMENT>
+__device__ __forceinline__ Plan plan(const AttentionParams &p) {
+    const uint32_t lane = threadIdx.x & 31, entries = p.sequences * p.tiles, blocks = gridDim.x, heads = p.c.heads;
+    uint32_t first, one = 0;  // the granules of this lane's first entry
+    auto granules = [&](uint32_t e) {
+        uint32_t count = 0;
+        if (e < entries) unit_range(p, kv_span(p.c, p.spans, e / p.tiles, p.tokens), e % p.tiles, first, count);
+        return count;
+    };
+    auto cached = [&](uint32_t e) { return e < 32 ? one : granules(e); };
+    one = granules(lane);
+    unsigned long long total = 0, units = 0;
+    for (uint32_t e = lane; e < entries; e += 32) {
+        const uint32_t c = cached(e);
+        total += c;
+        units += c != 0;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        total += __shfl_xor_sync(0xffffffffu, total, o);
+        units += __shfl_xor_sync(0xffffffffu, units, o);
+    }
+    total *= heads;
+    units *= heads;
+    Plan r{};
+    r.total = total;
+    r.share = (total + blocks - 1) / blocks;
+    if (total == 0) { r.idle = true; return r; }
+    // Even parts: 1 + count * spare / total blocks for a unit of `count` granules, at most `blocks` together. Taken if the longest part
+    // is not much longer than an equal share, which costs most blocks a second segment.
+    const unsigned long long spare = units <= blocks ? blocks - units : 0;
+    auto parts = [&](uint32_t count) { return 1 + (uint32_t)((unsigned long long)count * spare / total); };
+    if (units <= blocks) {
+        uint32_t longest = 0;
+        for (uint32_t e = lane; e < entries; e += 32) {
+            const uint32_t c = cached(e), n = parts(c);
+            longest = max(longest, (c + n - 1) / n);
+        }
+        r.even = __reduce_max_sync(0xffffffffu, longest) <= r.share + SEGMENT;
+    }
+    const unsigned long long at = r.even ? blockIdx.x : blockIdx.x * r.share;
+    unsigned long long before = 0;
+    r.idle = true;
+    for (uint32_t e0 = 0; e0 < entries; e0 += 32) {
+        const uint32_t c = cached(e0 + lane);
+        const unsigned long long mine = c == 0 ? 0 : (unsigned long long)(r.even ? parts(c) : c) * heads;
+        unsigned long long upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned long long x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= (uint32_t)o) upto += x;
+        }
+        const uint32_t hit = __ballot_sync(0xffffffffu, at < before + upto);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            r.entry = e0 + l;
+            r.in = (uint32_t)(at - before - __shfl_sync(0xffffffffu, upto - mine, l));
+            r.idle = false;
+            break;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    if (r.even && !r.idle) {  // the unit's share: parts of one length
+        const uint32_t c = granules(r.entry), n = parts(c);
+        r.share = (c + n - 1) / n;
+        r.total = n;
+    }
+    return r;
+}
+
 template <int W, bool K8, bool V8>
-__global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 1) split_kernel(const __grid_constant__ AttentionParams p) {
+__global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(const __grid_constant__ AttentionParams p) {
     using S = Split<W, K8, V8>;
     constexpr int NB = S::NB, NT = S::NT, WARPS = S::WARPS, STAGES = S::STAGES, SG = S::SG;
     constexpr KvLayout L = S::L;
@@ -254,7 +338,6 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 1) split_kernel(con
     float *join_l = join_m + WARPS * ROWS;                              // [WARPS][ROWS]
     float *row_scale = join_l + WARPS * ROWS;                           // [ROWS]
     uint32_t *word = (uint32_t *)(row_scale + ROWS);                    // broadcast words
-    __shared__ unsigned long long sums[WARPS], start[2];
 
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid / 32, g = lane / 4, t = lane % 4;
     if (lane == 0)
@@ -263,61 +346,43 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 1) split_kernel(con
     __syncwarp();
     wait_for_previous_operator();
 
-    // ---- this block's share: granules [begin, end) of all units' laid end to end, unit = (sequence, tile, head) ----
-    const size_t entries = (size_t)p.sequences * p.tiles, per = (entries + S::THREADS - 1) / S::THREADS;
-    const size_t e0 = min(entries, tid * per), e1 = min(entries, e0 + per);
-    unsigned long long mine = 0;
-    for (size_t e = e0; e < e1; ++e) {
-        uint32_t first, count;
-        unit_range(p, kv_span(p.c, p.spans, (uint32_t)(e / p.tiles), p.tokens), (uint32_t)(e % p.tiles), first, count);
-        mine += (unsigned long long)count * p.c.heads;
-    }
-    unsigned long long before = mine;  // inclusive sum over the warp's lanes
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long x = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= (uint32_t)o) before += x;
-    }
-    if (lane == 31) sums[warp] = before;
-    __syncthreads();
-    unsigned long long total = 0;
-    for (int w = 0; w < WARPS; ++w) {
-        if (w == (int)warp) before += total;
-        total += sums[w];
-    }
-    before -= mine;
-    const unsigned long long sh = (total + gridDim.x - 1) / gridDim.x;
-    unsigned long long at = blockIdx.x * sh;
-    const unsigned long long end = min(total, at + sh);
-    if (at >= end) return;  // the whole block
-    if (at >= before && at < before + mine) {  // one thread
-        for (size_t e = e0; e < e1; ++e) {
-            uint32_t first, count;
-            unit_range(p, kv_span(p.c, p.spans, (uint32_t)(e / p.tiles), p.tokens), (uint32_t)(e % p.tiles), first, count);
-            const unsigned long long n = (unsigned long long)count * p.c.heads;
-            if (at < before + n) { start[0] = e; start[1] = before; break; }
-            before += n;
-        }
-    }
-    __syncthreads();
-    unsigned long long entry = start[0], entry_begin = start[1];  // the entry that `at` lies in, and where its granules begin
+    const Plan pl = plan<S::SEGMENT>(p);
+    if (pl.idle) return;  // the whole block
+    unsigned long long at = pl.even ? 0 : blockIdx.x * pl.share;
+    const unsigned long long end = pl.even ? 1 : min(pl.total, at + pl.share);  // even parts: one turn of the loop
+    unsigned long long entry_begin = at - pl.in;
+    uint32_t entry = pl.entry;
 
     uint32_t turn = 0;  // stages this warp has taken, over all segments: position and phase in the ring
     bool alive = true;
     while (at < end) {
-        // ---- the segment: granules [g0, g0 + n) of one unit ----
-        const KvSpan span = kv_span(p.c, p.spans, (uint32_t)(entry / p.tiles), p.tokens);
-        const uint32_t tile = (uint32_t)(entry % p.tiles);
-        uint32_t first, count;
+        // ---- the segment: granules [g0, g0 + n) of one unit, which the blocks c0 .. c1 share ----
+        const uint32_t sequence = entry / p.tiles, tile = entry % p.tiles;
+        const KvSpan span = kv_span(p.c, p.spans, sequence, p.tokens);
+        uint32_t first, count, head, skip, n, c0, c1;
         unit_range(p, span, tile, first, count);
-        if (at - entry_begin >= (unsigned long long)count * p.c.heads) {  // all its heads are done (or it has no rows)
-            entry_begin += (unsigned long long)count * p.c.heads;
-            ++entry;
-            continue;
+        if (pl.even) {
+            head = pl.in / (uint32_t)pl.total;
+            const uint32_t k = pl.in % (uint32_t)pl.total;
+            skip = k * (uint32_t)pl.share;
+            if (skip >= count) return;  // fewer parts than blocks: the whole block
+            n = min((uint32_t)pl.share, count - skip);
+            c0 = blockIdx.x - k;
+            c1 = c0 + (count - 1) / (uint32_t)pl.share;
+        } else {
+            if (at - entry_begin >= (unsigned long long)count * p.c.heads) {  // all its heads are done (or it has no rows)
+                entry_begin += (unsigned long long)count * p.c.heads;
+                ++entry;
+                continue;
+            }
+            head = (uint32_t)((at - entry_begin) / count);
+            const unsigned long long unit_begin = entry_begin + (unsigned long long)head * count;
+            skip = (uint32_t)(at - unit_begin);
+            n = (uint32_t)min((unsigned long long)(count - skip), end - at);
+            c0 = (uint32_t)(unit_begin / pl.share);
+            c1 = (uint32_t)((unit_begin + count - 1) / pl.share);
         }
-        const uint32_t head = (uint32_t)((at - entry_begin) / count);
-        const unsigned long long unit_begin = entry_begin + (unsigned long long)head * count;
-        const uint32_t skip = (uint32_t)(at - unit_begin), n = (uint32_t)min((unsigned long long)(count - skip), end - at), g0 = first + skip;
+        const uint32_t g0 = first + skip;
         const uint8_t *base = kv_head(p.c, span.slot, head) + (size_t)g0 * L.bytes;
         const uint32_t stages = (n + SG - 1) / SG, mystages = stages > warp ? (stages - warp + WARPS - 1) / WARPS : 0;
         auto request = [&](uint32_t i) {  // the warp's stage i of this segment
@@ -329,13 +394,13 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 1) split_kernel(con
             for (uint32_t i = 0; i < min(mystages, (uint32_t)STAGES); ++i) request(i);
 
         // ---- the rows, split into f16 halves after a power of two that brings each row's largest value to [1, 2) ----
-        const size_t rows0 = (size_t)(entry / p.tiles) * p.tokens;  // the sequence's first row in the call
-        const uint64_t live_rows = (uint64_t)span.count * p.group;
+        const size_t rows0 = (size_t)sequence * p.tokens;  // the sequence's first row in the call
+        const uint32_t live_rows = span.count * p.group;
         for (uint32_t r = warp; r < ROWS; r += WARPS) {
-            const uint64_t row = (uint64_t)tile * ROWS + r;
+            const uint32_t row = tile * ROWS + r;
             float x[8] = {};
             if (row < live_rows && lane < (uint32_t)W / 8) {
-                const float *q = p.q + (rows0 + row / p.group) * p.q_stride + (size_t)(head * p.group + (uint32_t)(row % p.group)) * W + lane * 8;
+                const float *q = p.q + (rows0 + row / p.group) * p.q_stride + (size_t)(head * p.group + row % p.group) * W + lane * 8;
                 if ((uintptr_t)q % 16 == 0) {
                     const float4 a = *(const float4 *)q, b = *(const float4 *)(q + 4);
                     x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
@@ -365,11 +430,11 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 1) split_kernel(con
         __syncthreads();
 
         // positions that this thread's row sees, and those that every row of the tile sees
-        const uint64_t row = (uint64_t)tile * ROWS + g;
-        const uint32_t pos = row < live_rows ? span.first + (uint32_t)(row / p.group) : 0;
+        const uint32_t row = tile * ROWS + g;
+        const uint32_t pos = row < live_rows ? span.first + row / p.group : 0;
         const uint32_t row_high = pos, row_low = row < live_rows ? (p.window && pos >= p.window ? pos - p.window + 1 : 0) : 1;  // a dead row sees nothing
-        const uint64_t last_row = min(live_rows, (uint64_t)tile * ROWS + ROWS) - 1;
-        const uint32_t tile_high = span.first + (uint32_t)(last_row / p.group), first_pos = span.first + (uint32_t)((uint64_t)tile * ROWS / p.group);
+        const uint32_t last_row = min(live_rows, tile * ROWS + ROWS) - 1;
+        const uint32_t tile_high = span.first + last_row / p.group, first_pos = span.first + tile * ROWS / p.group;
         const uint32_t tile_low = p.window && first_pos >= p.window ? first_pos - p.window + 1 : 0;   // some row sees [tile_low, tile_high]
         const uint32_t all_low = p.window && tile_high >= p.window ? tile_high - p.window + 1 : 0;    // every live row sees [all_low, first_pos]
         const float my_scale = row_scale[g];
@@ -393,27 +458,36 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 1) split_kernel(con
             const bool edge = key0 < all_low || key0 + SG * KV_GRANULE - 1 > first_pos || here < SG * KV_GRANULE;
 
             float s[SG * 2][2];
+            {
+                uint32_t codes[SG * 2][K8 ? 2 * NB : NB], scales[SG * 2][NB];
 #pragma unroll
-            for (int j = 0; j < SG * 2; ++j) {
-                const uint8_t *gran = stage + j / 2 * L.bytes;
-                uint32_t codes[K8 ? 2 * NB : NB], scales[NB];
-                load_words<K8 ? 2 * NB : NB, L.k_vec>(gran + j % 2 * (L.k_scales / 2), lane, codes);
-                load_scales<NB>(gran + L.k_scales, j % 2 * 8 + 2 * t, scales);
-                s[j][0] = s[j][1] = 0.0f;
+                for (int j = 0; j < SG * 2; ++j) {
+                    const uint8_t *gran = stage + j / 2 * L.bytes;
+                    load_words<K8 ? 2 * NB : NB, L.k_vec>(gran + j % 2 * (L.k_scales / 2), lane, codes[j]);
+                    load_scales<NB>(gran + L.k_scales, j % 2 * 8 + 2 * t, scales[j]);
+                    s[j][0] = s[j][1] = 0.0f;
+                }
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    if (K8) {
-                        mma(c, fragments[(2 * b) * 32 + lane], byte_codes(codes[2 * b], 0x4140), byte_codes(codes[2 * b], 0x4342));
-                        mma(c, fragments[(2 * b + 1) * 32 + lane], byte_codes(codes[2 * b + 1], 0x4140), byte_codes(codes[2 * b + 1], 0x4342));
-                    } else {
-                        const uint32_t w = codes[b], w8 = w >> 8;
-                        mma(c, fragments[(2 * b) * 32 + lane], low_codes(w), high_codes(w));
-                        mma(c, fragments[(2 * b + 1) * 32 + lane], low_codes(w8), high_codes(w8));
+                    const uint4 q0 = fragments[(2 * b) * 32 + lane], q1 = fragments[(2 * b + 1) * 32 + lane];
+#pragma unroll
+                    for (int j = 0; j < SG * 2; ++j) {
+                        float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        if (K8) {
+                            mma(c, q0, byte_codes(codes[j][2 * b], 0x4140), byte_codes(codes[j][2 * b], 0x4342));
+                            mma(c, q1, byte_codes(codes[j][2 * b + 1], 0x4140), byte_codes(codes[j][2 * b + 1], 0x4342));
+                        } else {
+                            const uint32_t w = codes[j][b], w8 = w >> 8;
+                            mma(c, q0, low_codes(w), high_codes(w));
+                            mma(c, q1, low_codes(w8), high_codes(w8));
+                        }
+                        s[j][0] = fmaf(scale_of<NB>(scales[j], 0, b), fmaf(c[2], LO, c[0]), s[j][0]);
+                        s[j][1] = fmaf(scale_of<NB>(scales[j], 1, b), fmaf(c[3], LO, c[1]), s[j][1]);
                     }
-                    s[j][0] = fmaf(scale_of<NB>(scales, 0, b), fmaf(c[2], LO, c[0]), s[j][0]);
-                    s[j][1] = fmaf(scale_of<NB>(scales, 1, b), fmaf(c[3], LO, c[1]), s[j][1]);
                 }
+            }
+#pragma unroll
+            for (int j = 0; j < SG * 2; ++j) {
                 s[j][0] *= my_scale;
                 s[j][1] *= my_scale;
                 if (edge) {
@@ -520,7 +594,6 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 1) split_kernel(con
         __syncthreads();
         const uint32_t used = min(stages, (uint32_t)WARPS);
         const bool whole = n == count;
-        const unsigned long long c0 = unit_begin / sh, c1 = (unit_begin + count - 1) / sh;  // the blocks that share the unit
         float *partial = p.partials + ((size_t)blockIdx.x * 2 + (skip == 0 && !whole)) * S::PARTIAL;  // a unit that starts here goes into the second place
         // a row's parts are weighted by 2^(their maximum - the row's): found once, by one thread a row
         if (tid < ROWS) {
@@ -542,10 +615,10 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 1) split_kernel(con
         __syncthreads();
         auto put = [&](uint32_t e, float4 x) {  // four values of a row of the result
             const uint32_t r = e / W;
-            const uint64_t out_row = (uint64_t)tile * ROWS + r;
+            const uint32_t out_row = tile * ROWS + r;
             if (out_row >= live_rows) return;
             const float f = row_scale[r];
-            const size_t i = (rows0 + out_row / p.group) * p.out_stride + (size_t)(head * p.group + (uint32_t)(out_row % p.group)) * W + e % W;
+            const size_t i = (rows0 + out_row / p.group) * p.out_stride + (size_t)(head * p.group + out_row % p.group) * W + e % W;
             store_out(p, i, x.x * f);
             store_out(p, i + 1, x.y * f);
             store_out(p, i + 2, x.z * f);
@@ -564,12 +637,12 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 1) split_kernel(con
         if (!whole) {
             __threadfence();
             __syncthreads();
-            if (tid == 0) *word = atomicAdd(p.counters + c0, 1u) == (uint32_t)(c1 - c0);
+            if (tid == 0) *word = atomicAdd(p.counters + c0, 1u) == (c1 - c0);
             __syncthreads();
             if (*word) {  // this block arrived last: the parts of all blocks, in their order
                 __threadfence();
-                const uint32_t parts = (uint32_t)(c1 - c0) + 1;
-                const float *first_part = p.partials + (c0 * 2 + 1) * S::PARTIAL, *other = p.partials + (c0 + 1) * 2 * S::PARTIAL;
+                const uint32_t parts = (c1 - c0) + 1;
+                const float *first_part = p.partials + ((size_t)c0 * 2 + 1) * S::PARTIAL, *other = p.partials + ((size_t)c0 + 1) * 2 * S::PARTIAL;
                 auto part = [&](uint32_t c) { return c ? other + (size_t)(c - 1) * 2 * S::PARTIAL : first_part; };
                 float *weight = join;  // [parts][ROWS], then the sums
                 for (uint32_t i = tid; i < parts * ROWS; i += S::THREADS) {
@@ -591,7 +664,7 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 1) split_kernel(con
                 __syncthreads();
                 for (uint32_t e = tid * 4; e < ROWS * W; e += S::THREADS * 4) {
                     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
+#pragma unroll 8
                     for (uint32_t c = 0; c < parts; ++c) {
                         const float f = weight[c * ROWS + e / W];
                         const float4 x = __ldcg((const float4 *)(part(c) + e));
@@ -615,7 +688,7 @@ bool configure() {
 template <int W, bool K8, bool V8>
 int launch(cudaStream_t s, const AttentionParams &p, int sm_count) {
     using S = Split<W, K8, V8>;
-    launch_after_previous_smem(split_kernel<W, K8, V8>, dim3(sm_count), dim3(S::THREADS), S::SMEM, s, p);
+    launch_after_previous_smem(split_kernel<W, K8, V8>, dim3(sm_count * S::RESIDENT), dim3(S::THREADS), S::SMEM, s, p);
     return 1;
 }
 #define NU_EVERY(F, W, ...) (k8 ? (v8 ? F<W, true, true>(__VA_ARGS__) : F<W, true, false>(__VA_ARGS__)) : (v8 ? F<W, false, true>(__VA_ARGS__) : F<W, false, false>(__VA_ARGS__)))
