@@ -6,14 +6,19 @@
 // on mma.sync.m16n8k16 without losing F32 accuracy:
 //
 //   * Codes are whole numbers of at most eight bits, so they are exact in f16; a block's scale is applied to the product, not
-//     to the codes. What is not exact in f16, the query and the probabilities, is split: x = hi + lo / 2048 with hi and lo in
+//     to the codes. What is not exact in f16, the query and the probabilities, is split: x = hi + lo with both in
 //     f16 (22 bits). The 16 rows of the A operand are the hi parts of eight query rows and their lo parts, so the split
 //     costs no second instruction, and the two sums of a row come out in the same thread.
-//   * q . k = sum_b d_b (q_b . c_b): one accumulator pair of instructions per block of 32, then one F32 FMA with d_b.
+//   * q . k = sum_b d_b (q_b . c_b): one accumulator pair of instructions per block of 32, then F32 FMAs with d_b. The key's code
+//     without sign is left where it lies in its word: as f16 that is code * 2^-24, a subnormal number (16 times that
+//     from a high nibble, which the query's fragment makes up for), so a pair of codes costs one logical operation. The
+//     offset (8 or 128) comes off the sum instead, sum_b d_b * sum(q_b): one more product with the scales as they lie. It is as
+//     large as the sums themselves, so nothing is lost; the values' sums run over the positions, where it would grow
+//     with their number, so their codes get their sign first.
 //   * p v = sum_j (p_j d_jb) c_j: the scale goes into the probability, once per block, before it is split. The products
-//     p d are kept near one by a power of two per warp (`bias`), raised when a larger scale comes by: f16's range is no limit, and what
-//     is lost of a position is below 2^-36 of the largest value seen.
-//   * The running maximum of a row is only raised when a score passes it by 8 (in log2): the accumulators are rarely rescaled.
+//     p d are kept near 2^11 by a power of two per warp (`bias`), lowered when a larger scale comes by: f16's range is no limit,
+//     and what is lost of a position is below 2^-36 of the largest value seen.
+//   * The running maximum of a row is only raised when a score passes it by 3 (in log2): the accumulators are rarely rescaled.
 //
 // Work split: the granules of all (sequence, row tile, head) units are laid end to end and every block takes the same
 // number of them, whatever the lengths are; they are counted on the device from the spans, so a recorded launch fits every
@@ -22,6 +27,8 @@
 //
 // generic_kernel: one warp per query row and head, any width up to 512; also what generic_only selects.
 #include <cuda_bf16.h>
+
+#include <type_traits>
 
 #include "kernels.hpp"
 #include "kv_layout.cuh"
@@ -159,22 +166,33 @@ __device__ __forceinline__ void mma(float c[4], const uint4 a, uint32_t b0, uint
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
+// The same onto an accumulator of zeros.
+__device__ __forceinline__ void mma_zero(float c[4], const uint4 a, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ uint32_t h2(__half2 x) { return *(const uint32_t *)&x; }
 __device__ __forceinline__ __half2 as_h2(uint32_t x) { return *(const __half2 *)&x; }
+// (w & mask) | high in one operation: `high` is a register the compiler cannot see into, as two constants do not fit one.
+__device__ __forceinline__ uint32_t mask_or(uint32_t w, uint32_t mask, uint32_t high) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "r"(mask), "r"(high));
+    return r;
+}
 // Four-bit codes in bits 0..3 / 4..7 of the bytes 0 and 2 of w, as whole numbers code - 8 in f16: the code is placed in the
 // low bits of 1024 (or, shifted by four, of 1024 = 64 * 16), which one exact operation takes off again.
-__device__ __forceinline__ uint32_t low_codes(uint32_t w) { return h2(__hsub2(as_h2((w & 0x000f000fu) | 0x64006400u), as_h2(0x64086408u))); }
-__device__ __forceinline__ uint32_t high_codes(uint32_t w) { return h2(__hfma2(as_h2((w & 0x00f000f0u) | 0x64006400u), as_h2(0x2c002c00u), as_h2(0xd480d480u))); }
+__device__ __forceinline__ uint32_t low_codes(uint32_t w, uint32_t k1024) { return h2(__hsub2(as_h2(mask_or(w, 0x000f000fu, k1024)), as_h2(0x64086408u))); }
+__device__ __forceinline__ uint32_t high_codes(uint32_t w, uint32_t k1024) { return h2(__hfma2(as_h2(mask_or(w, 0x00f000f0u, k1024)), as_h2(0x2c002c00u), as_h2(0xd480d480u))); }
 // Eight-bit codes in bytes 0, 1 (or 2, 3) of w, as code - 128.
 __device__ __forceinline__ uint32_t byte_codes(uint32_t w, uint32_t selector) { return h2(__hsub2(as_h2(__byte_perm(w, 0x64646464u, selector)), as_h2(0x64806480u))); }
 
 __device__ __forceinline__ uint32_t pack_hi_lo(float x, float y, uint32_t &lo) {
     const __half2 hi = __floats2half2_rn(x, y);
     const float2 f = __half22float2(hi);
-    lo = h2(__floats2half2_rn((x - f.x) * 2048.0f, (y - f.y) * 2048.0f));
+    lo = h2(__floats2half2_rn(x - f.x, y - f.y));
     return h2(hi);
 }
-constexpr float LO = 1.0f / 2048.0f;
 
 // N words of a lane's codes in a tile, kept in vectors.
 template <int N, int VEC>
@@ -226,7 +244,7 @@ struct Split {
     static constexpr int JOIN = WARPS * ROWS * W * 4;  // the warps' accumulators; takes the ring's place
     static constexpr int BUFFER = WARPS * STAGES * STAGE > JOIN ? WARPS * STAGES * STAGE : JOIN;
     static constexpr int FRAGMENTS = KT * 512;
-    static constexpr int SMEM = BUFFER + FRAGMENTS + WARPS * STAGES * 8 + (WARPS * 2 + 1) * ROWS * 4 + 64;
+    static constexpr int SMEM = BUFFER + FRAGMENTS + 256 + WARPS * STAGES * 8 + (WARPS * 2 + 1) * ROWS * 4 + 64;
     static constexpr int PARTIAL = ROWS * (W + 2);
     // A second segment costs a block about 6 us of prologue and join; the bytes that its warps read in that time.
     static constexpr uint32_t SEGMENT = 96 * 1024 / L.bytes;
@@ -333,7 +351,8 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
     uint8_t *ring = smem;
     float *join = (float *)smem;
     uint4 *fragments = (uint4 *)(smem + S::BUFFER);                     // [KT][32]
-    uint64_t *bars = (uint64_t *)(smem + S::BUFFER + S::FRAGMENTS);     // [WARPS][STAGES]
+    __half *block_sums = (__half *)(smem + S::BUFFER + S::FRAGMENTS);   // [hi, lo][ROWS][8]: sums of a row's blocks, for the offset
+    uint64_t *bars = (uint64_t *)(smem + S::BUFFER + S::FRAGMENTS + 256);  // [WARPS][STAGES]
     float *join_m = (float *)(bars + WARPS * STAGES);                   // [WARPS][ROWS]
     float *join_l = join_m + WARPS * ROWS;                              // [WARPS][ROWS]
     float *row_scale = join_l + WARPS * ROWS;                           // [ROWS]
@@ -393,7 +412,7 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
         if (lane == 0)
             for (uint32_t i = 0; i < min(mystages, (uint32_t)STAGES); ++i) request(i);
 
-        // ---- the rows, split into f16 halves after a power of two that brings each row's largest value to [1, 2) ----
+        // ---- the rows, split into f16 halves after a power of two that brings each row's largest value to [2^13, 2^14) ----
         const size_t rows0 = (size_t)sequence * p.tokens;  // the sequence's first row in the call
         const uint32_t live_rows = span.count * p.group;
         for (uint32_t r = warp; r < ROWS; r += WARPS) {
@@ -415,13 +434,30 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
             top = __reduce_max_sync(0xffffffffu, top);
             // 2^e: from the exponent's bits; rows of zeros and of subnormal values count as 2^-126
             const int e = (int)max(top >> 23, 1u) - 127;
-            const float down = top >= 0x7f800000u ? NAN : scalbnf(1.0f, -e);
-            if (lane == 0) row_scale[r] = scalbnf(p.scale, e);
+            const float down = top >= 0x7f800000u ? NAN : scalbnf(1.0f, -e), up = K8 ? 1.0f : 0.0625f;
+            if (lane == 0) row_scale[r] = scalbnf(p.scale, e - 13 + 24);  // the query's power of two, and the codes'
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i] = x[i] * down * 8192.0f;
+                sum += x[i];
+            }
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            if (lane % 4 == 0) {  // at most 32 * 2^14 * 2^-5
+                const float y = sum * 0.03125f;
+                const __half hi = __float2half_rn(y);
+                block_sums[r * 8 + lane / 4] = hi;
+                block_sums[(ROWS + r) * 8 + lane / 4] = __float2half_rn(y - __half2float(hi));
+            }
             if (lane < (uint32_t)W / 8) {
                 const uint32_t b = lane / 4, tt = lane % 4;
                 uint32_t hi[4], lo[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) hi[i] = pack_hi_lo(x[i] * down, x[i + 4] * down, lo[i]);
+                for (int i = 0; i < 4; ++i) {
+                    const float f = i % 2 ? up : 1.0f;  // Q4_0: dimensions 1, 5, 3, 7 meet high nibbles
+                    hi[i] = pack_hi_lo(x[i] * f, x[i + 4] * f, lo[i]);
+                }
                 // the pair of dimensions i, i + 4 of the eight is the k pair of step i / 2, half i % 2
                 fragments[(2 * b) * 32 + r * 4 + tt] = make_uint4(hi[0], lo[0], hi[1], lo[1]);
                 fragments[(2 * b + 1) * 32 + r * 4 + tt] = make_uint4(hi[2], lo[2], hi[3], lo[3]);
@@ -438,8 +474,11 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
         const uint32_t tile_low = p.window && first_pos >= p.window ? first_pos - p.window + 1 : 0;   // some row sees [tile_low, tile_high]
         const uint32_t all_low = p.window && tile_high >= p.window ? tile_high - p.window + 1 : 0;    // every live row sees [all_low, first_pos]
         const float my_scale = row_scale[g];
+        const uint4 sums = make_uint4(((const uint32_t *)block_sums)[lane], ((const uint32_t *)block_sums)[ROWS * 4 + lane], 0u, 0u);
+        uint32_t k1024 = 0x64006400u;
+        asm volatile("" : "+r"(k1024));
 
-        float m = -INFINITY, l = 0.0f, bias = 0x1p40f, o[NT][4];
+        float m = -INFINITY, l = 0.0f, bias = 0x1p40f, o[NT][4];  // the smallest scale is 2^-24
 #pragma unroll
         for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
 
@@ -455,7 +494,9 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
             const uint8_t *stage = ring + (warp * STAGES + slot) * S::STAGE;
             const uint32_t st = warp + i * WARPS, key0 = (g0 + st * SG) * KV_GRANULE;
             const uint32_t here = min((uint32_t)SG, n - st * SG) * KV_GRANULE;  // positions that were copied
-            const bool edge = key0 < all_low || key0 + SG * KV_GRANULE - 1 > first_pos || here < SG * KV_GRANULE;
+            const bool at_edge = key0 < all_low || key0 + SG * KV_GRANULE - 1 > first_pos || here < SG * KV_GRANULE;
+            auto take = [&](auto edge_tag) {
+            constexpr bool edge = decltype(edge_tag)::value;
 
             float s[SG * 2][2];
             {
@@ -465,24 +506,30 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
                     const uint8_t *gran = stage + j / 2 * L.bytes;
                     load_words<K8 ? 2 * NB : NB, L.k_vec>(gran + j % 2 * (L.k_scales / 2), lane, codes[j]);
                     load_scales<NB>(gran + L.k_scales, j % 2 * 8 + 2 * t, scales[j]);
-                    s[j][0] = s[j][1] = 0.0f;
+                    // what the codes' offset adds: sum_b d_b * offset * sum(q_b), in units of 2^-24; the sums carry 2^-5
+                    float c[4];
+                    const uint32_t pair = 2 * t < NB ? *(const uint32_t *)(gran + L.k_scales + ((j % 2 * 8 + g) * NB + 2 * t) * 2) : 0u;
+                    mma_zero(c, sums, pair, 0u);
+                    constexpr float OFFSET = -(K8 ? 128.0f : 8.0f) * 32.0f / 16777216.0f;
+                    s[j][0] = (c[0] + c[2]) * OFFSET;
+                    s[j][1] = (c[1] + c[3]) * OFFSET;
                 }
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
                     const uint4 q0 = fragments[(2 * b) * 32 + lane], q1 = fragments[(2 * b + 1) * 32 + lane];
 #pragma unroll
                     for (int j = 0; j < SG * 2; ++j) {
-                        float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        float c[4];
                         if (K8) {
-                            mma(c, q0, byte_codes(codes[j][2 * b], 0x4140), byte_codes(codes[j][2 * b], 0x4342));
-                            mma(c, q1, byte_codes(codes[j][2 * b + 1], 0x4140), byte_codes(codes[j][2 * b + 1], 0x4342));
+                            mma_zero(c, q0, __byte_perm(codes[j][2 * b], 0u, 0x4140), __byte_perm(codes[j][2 * b], 0u, 0x4342));
+                            mma(c, q1, __byte_perm(codes[j][2 * b + 1], 0u, 0x4140), __byte_perm(codes[j][2 * b + 1], 0u, 0x4342));
                         } else {
                             const uint32_t w = codes[j][b], w8 = w >> 8;
-                            mma(c, q0, low_codes(w), high_codes(w));
-                            mma(c, q1, low_codes(w8), high_codes(w8));
+                            mma_zero(c, q0, w & 0x000f000fu, w & 0x00f000f0u);
+                            mma(c, q1, w8 & 0x000f000fu, w8 & 0x00f000f0u);
                         }
-                        s[j][0] = fmaf(scale_of<NB>(scales[j], 0, b), fmaf(c[2], LO, c[0]), s[j][0]);
-                        s[j][1] = fmaf(scale_of<NB>(scales[j], 1, b), fmaf(c[3], LO, c[1]), s[j][1]);
+                        s[j][0] = fmaf(scale_of<NB>(scales[j], 0, b), c[0] + c[2], s[j][0]);
+                        s[j][1] = fmaf(scale_of<NB>(scales[j], 1, b), c[1] + c[3], s[j][1]);
                     }
                 }
             }
@@ -525,11 +572,11 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
             for (int j = 0; j < SG * 2; ++j) top = fmaxf(top, fmaxf(s[j][0], s[j][1]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            if (__any_sync(0xffffffffu, top > m + 8.0f || dmax * bias > 2.0f)) {
+            if (__any_sync(0xffffffffu, top > m + 3.0f || dmax * bias > 4096.0f)) {
                 float d = fmaxf(dmax, __shfl_xor_sync(0xffffffffu, dmax, 1));
                 d = fmaxf(d, __shfl_xor_sync(0xffffffffu, d, 2));
                 const float next = fmaxf(m, top);
-                const float bias_next = d * bias > 2.0f ? scalbnf(1.0f, 127 - (int)(__float_as_uint(fminf(d, 65504.0f)) >> 23)) : bias;
+                const float bias_next = d * bias > 4096.0f ? scalbnf(1.0f, 127 + 11 - (int)(__float_as_uint(fminf(d, 65504.0f)) >> 23)) : bias;
                 const float fl = m == -INFINITY ? 0.0f : exp2_approx(m - next), f = fl * (bias_next / bias);
                 bias = bias_next;
                 m = next;
@@ -571,12 +618,15 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
 #pragma unroll
                         for (int q = 0; q < 2; ++q) {
                             const uint32_t w = codes[2 * b + q], w8 = w >> 8;
-                            mma(o[4 * b + 2 * q], a, low_codes(w), low_codes(w8));
-                            mma(o[4 * b + 2 * q + 1], a, high_codes(w), high_codes(w8));
+                            mma(o[4 * b + 2 * q], a, low_codes(w, k1024), low_codes(w8, k1024));
+                            mma(o[4 * b + 2 * q + 1], a, high_codes(w, k1024), high_codes(w8, k1024));
                         }
                     }
                 }
             }
+            };
+            if (at_edge) take(std::true_type{});
+            else take(std::false_type{});
             __syncwarp();
             if (lane == 0 && i + STAGES < mystages) request(i + STAGES);
         }
@@ -590,7 +640,7 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
         const float back = 1.0f / bias;
 #pragma unroll
         for (int k = 0; k < NT; ++k)
-            *(float2 *)(join + (warp * ROWS + g) * W + k * 8 + 2 * t) = make_float2(fmaf(o[k][2], LO, o[k][0]) * back, fmaf(o[k][3], LO, o[k][1]) * back);
+            *(float2 *)(join + (warp * ROWS + g) * W + k * 8 + 2 * t) = make_float2((o[k][0] + o[k][2]) * back, (o[k][1] + o[k][3]) * back);
         __syncthreads();
         const uint32_t used = min(stages, (uint32_t)WARPS);
         const bool whole = n == count;

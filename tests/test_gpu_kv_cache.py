@@ -280,11 +280,11 @@ def test_values_and_queries_of_all_sizes(backend, gain, encoding):
         want = kv_oracle.attention(q, k[0], v[0], 298, 2)
         got = attend(b, held, cache, shape, [(0, 298, 2)], 2, q, 4)
         # scores of some hundred (the last head): their F32 rounding, 2^-24 of the score for each of the 4 blocks, is that of the probability.
-        # The split of x = p d bias into f16 halves has an absolute end as well: lo = 2048 (x - hi) is rounded to a multiple of 2^-24 at
-        # its smallest, half a step of which is 2^-36 of x. bias d < 2 for every scale d seen and bias dmax >= 1, so that is at most 2^-36 dmax
-        # of p d and, the largest code of a block times its scale being its largest value, 2^-36 max|v| a position of the result (the sum
-        # of the p, by which it is divided, is at least 1). It shows where the row's likeliest positions hold zeros: values of 1e-6, whose Q8_0
-        # scales vanish in f16 for some blocks and not for others.
+        # The split of x = p d bias into f16 halves has an absolute end as well: lo = x - hi is rounded to a multiple of 2^-24 at its smallest,
+        # half a step of which is 2^-25. The largest scale seen has bias dmax >= 2^11, so that is at most 2^-36 dmax of p d and, the largest
+        # code of a block times its scale being its largest value, 2^-36 max|v| a position of the result (the sum of the p, by which it is
+        # divided, is at least 1). It shows where the row's likeliest positions hold zeros: values of 1e-6, whose Q8_0 scales vanish in f16
+        # for some blocks and not for others.
         lost = 300 * 2.0 ** -36 * np.abs(v).max() * np.sqrt(want[:, 0].size)
         for h in range(4):
             assert np.linalg.norm(got[:, h] - want[:, h]) <= (1e-5 if h < 3 else 1e-4) * np.linalg.norm(want[:, h]) + lost, h
