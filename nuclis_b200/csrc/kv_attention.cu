@@ -26,46 +26,16 @@
 // Within a block the warps take turns at stages of one or two granules, each through its own ring of bulk copies.
 //
 // generic_kernel: one warp per query row and head, any width up to 512; also what generic_only selects.
-#include <cuda_bf16.h>
-
 #include <type_traits>
 
-#include "kernels.hpp"
-#include "kv_layout.cuh"
+#include "kv_attention.cuh"
 #include "launch.cuh"
 
 namespace nu {
 
+using namespace attn;
+
 namespace {
-
-constexpr uint32_t SPIN_LIMIT = 1u << 22;
-
-struct AttentionParams {
-    KvView c;
-    const KvSpan *spans;
-    uint32_t sequences, tokens;
-    const float *q;
-    size_t q_stride;
-    uint32_t group;  // query heads of a key/value head
-    uint32_t tiles;  // row tiles of a (sequence, head): ceil(tokens * group / 8)
-    void *out;
-    size_t out_stride;
-    bool bf16;
-    float scale;     // times log2(e)
-    uint32_t window; // 0: none
-    float *partials;      // [block][2][rows * (width + 2)]
-    uint32_t *counters;   // one a block, zero between launches
-};
-
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ void store_out(const AttentionParams &p, size_t index, float v) {
-    if (p.bf16) ((__nv_bfloat16 *)p.out)[index] = __float2bfloat16_rn(v);
-    else ((float *)p.out)[index] = v;
-}
 
 // ---- any width ---------------------------------------------------------------------------------------------------------
 
@@ -142,21 +112,6 @@ __global__ void __launch_bounds__(GENERIC_WARPS * 32) generic_kernel(const Atten
 
 constexpr int ROWS = 8;  // query rows of a unit
 
-__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
-    for (uint32_t i = 0; i < SPIN_LIMIT; ++i) {
-        uint32_t done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(done)
-            : "r"(bar), "r"(parity)
-            : "memory");
-        if (done) return true;
-    }
-    return false;
-}
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
@@ -172,21 +127,6 @@ __device__ __forceinline__ void mma_zero(float c[4], const uint4 a, uint32_t b0,
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
         : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.0f));
 }
-__device__ __forceinline__ uint32_t h2(__half2 x) { return *(const uint32_t *)&x; }
-__device__ __forceinline__ __half2 as_h2(uint32_t x) { return *(const __half2 *)&x; }
-// (w & mask) | high in one operation: `high` is a register the compiler cannot see into, as two constants do not fit one.
-__device__ __forceinline__ uint32_t mask_or(uint32_t w, uint32_t mask, uint32_t high) {
-    uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "r"(mask), "r"(high));
-    return r;
-}
-// Four-bit codes in bits 0..3 / 4..7 of the bytes 0 and 2 of w, as whole numbers code - 8 in f16: the code is placed in the
-// low bits of 1024 (or, shifted by four, of 1024 = 64 * 16), which one exact operation takes off again.
-__device__ __forceinline__ uint32_t low_codes(uint32_t w, uint32_t k1024) { return h2(__hsub2(as_h2(mask_or(w, 0x000f000fu, k1024)), as_h2(0x64086408u))); }
-__device__ __forceinline__ uint32_t high_codes(uint32_t w, uint32_t k1024) { return h2(__hfma2(as_h2(mask_or(w, 0x00f000f0u, k1024)), as_h2(0x2c002c00u), as_h2(0xd480d480u))); }
-// Eight-bit codes in bytes 0, 1 (or 2, 3) of w, as code - 128.
-__device__ __forceinline__ uint32_t byte_codes(uint32_t w, uint32_t selector) { return h2(__hsub2(as_h2(__byte_perm(w, 0x64646464u, selector)), as_h2(0x64806480u))); }
-
 __device__ __forceinline__ uint32_t pack_hi_lo(float x, float y, uint32_t &lo) {
     const __half2 hi = __floats2half2_rn(x, y);
     const float2 f = __half22float2(hi);
@@ -252,96 +192,6 @@ struct Split {
     static_assert(SMEM <= 113 * 1024, "two blocks share a multiprocessor");
 };
 
-// The granules that the rows of tile `tile` of a sequence see: [first, first + count).
-__device__ __forceinline__ void unit_range(const AttentionParams &p, const KvSpan &s, uint32_t tile, uint32_t &first, uint32_t &count) {
-    const uint32_t rows = s.count * p.group, r0 = tile * ROWS;  // below 2^31: the host's limit on a call's rows
-    first = count = 0;
-    if (r0 >= rows) return;
-    const uint32_t r1 = min(rows, r0 + ROWS) - 1;
-    const uint32_t low = s.first + r0 / p.group, high = s.first + r1 / p.group;
-    first = (p.window && low >= p.window ? low - p.window + 1 : 0) / KV_GRANULE;
-    count = high / KV_GRANULE + 1 - first;
-}
-
-// Where a block starts: which entry ((sequence, row tile), all of whose heads have the same granules) and how far into it.
-struct Plan {
-    bool even;                      // every block has one part of one unit; else an equal share of all granules
-    unsigned long long share, total;
-    uint32_t entry, in;             // in: blocks (even) or granules into the entry
-    bool idle;
-};
-
-// One warp's finding, the same in every warp: no barrier. Lanes take entries in turn.
-template <uint32_t SEGMENT>
-__device__ __forceinline__ Plan plan(const AttentionParams &p) {
-    const uint32_t lane = threadIdx.x & 31, entries = p.sequences * p.tiles, blocks = gridDim.x, heads = p.c.heads;
-    uint32_t first, one = 0;  // the granules of this lane's first entry
-    auto granules = [&](uint32_t e) {
-        uint32_t count = 0;
-        if (e < entries) unit_range(p, kv_span(p.c, p.spans, e / p.tiles, p.tokens), e % p.tiles, first, count);
-        return count;
-    };
-    auto cached = [&](uint32_t e) { return e < 32 ? one : granules(e); };
-    one = granules(lane);
-    unsigned long long total = 0, units = 0;
-    for (uint32_t e = lane; e < entries; e += 32) {
-        const uint32_t c = cached(e);
-        total += c;
-        units += c != 0;
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        total += __shfl_xor_sync(0xffffffffu, total, o);
-        units += __shfl_xor_sync(0xffffffffu, units, o);
-    }
-    total *= heads;
-    units *= heads;
-    Plan r{};
-    r.total = total;
-    r.share = (total + blocks - 1) / blocks;
-    if (total == 0) { r.idle = true; return r; }
-    // Even parts: 1 + count * spare / total blocks for a unit of `count` granules, at most `blocks` together. Taken if the longest part
-    // is not much longer than an equal share, which costs most blocks a second segment.
-    const unsigned long long spare = units <= blocks ? blocks - units : 0;
-    auto parts = [&](uint32_t count) { return 1 + (uint32_t)((unsigned long long)count * spare / total); };
-    if (units <= blocks) {
-        uint32_t longest = 0;
-        for (uint32_t e = lane; e < entries; e += 32) {
-            const uint32_t c = cached(e), n = parts(c);
-            longest = max(longest, (c + n - 1) / n);
-        }
-        r.even = __reduce_max_sync(0xffffffffu, longest) <= r.share + SEGMENT;
-    }
-    const unsigned long long at = r.even ? blockIdx.x : blockIdx.x * r.share;
-    unsigned long long before = 0;
-    r.idle = true;
-    for (uint32_t e0 = 0; e0 < entries; e0 += 32) {
-        const uint32_t c = cached(e0 + lane);
-        const unsigned long long mine = c == 0 ? 0 : (unsigned long long)(r.even ? parts(c) : c) * heads;
-        unsigned long long upto = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const unsigned long long x = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= (uint32_t)o) upto += x;
-        }
-        const uint32_t hit = __ballot_sync(0xffffffffu, at < before + upto);
-        if (hit) {
-            const int l = __ffs(hit) - 1;
-            r.entry = e0 + l;
-            r.in = (uint32_t)(at - before - __shfl_sync(0xffffffffu, upto - mine, l));
-            r.idle = false;
-            break;
-        }
-        before += __shfl_sync(0xffffffffu, upto, 31);
-    }
-    if (r.even && !r.idle) {  // the unit's share: parts of one length
-        const uint32_t c = granules(r.entry), n = parts(c);
-        r.share = (c + n - 1) / n;
-        r.total = n;
-    }
-    return r;
-}
-
 template <int W, bool K8, bool V8>
 __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(const __grid_constant__ AttentionParams p) {
     using S = Split<W, K8, V8>;
@@ -365,43 +215,17 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
     __syncwarp();
     wait_for_previous_operator();
 
-    const Plan pl = plan<S::SEGMENT>(p);
-    if (pl.idle) return;  // the whole block
-    unsigned long long at = pl.even ? 0 : blockIdx.x * pl.share;
-    const unsigned long long end = pl.even ? 1 : min(pl.total, at + pl.share);  // even parts: one turn of the loop
-    unsigned long long entry_begin = at - pl.in;
-    uint32_t entry = pl.entry;
+    const Plan pl = plan<ROWS, KV_GRANULE, S::SEGMENT>(p);
+    Walk<ROWS, KV_GRANULE> walk(pl);
+    Segment sg;
 
     uint32_t turn = 0;  // stages this warp has taken, over all segments: position and phase in the ring
     bool alive = true;
-    while (at < end) {
+    while (walk.next(p, pl, sg)) {
         // ---- the segment: granules [g0, g0 + n) of one unit, which the blocks c0 .. c1 share ----
-        const uint32_t sequence = entry / p.tiles, tile = entry % p.tiles;
-        const KvSpan span = kv_span(p.c, p.spans, sequence, p.tokens);
-        uint32_t first, count, head, skip, n, c0, c1;
-        unit_range(p, span, tile, first, count);
-        if (pl.even) {
-            head = pl.in / (uint32_t)pl.total;
-            const uint32_t k = pl.in % (uint32_t)pl.total;
-            skip = k * (uint32_t)pl.share;
-            if (skip >= count) return;  // fewer parts than blocks: the whole block
-            n = min((uint32_t)pl.share, count - skip);
-            c0 = blockIdx.x - k;
-            c1 = c0 + (count - 1) / (uint32_t)pl.share;
-        } else {
-            if (at - entry_begin >= (unsigned long long)count * p.c.heads) {  // all its heads are done (or it has no rows)
-                entry_begin += (unsigned long long)count * p.c.heads;
-                ++entry;
-                continue;
-            }
-            head = (uint32_t)((at - entry_begin) / count);
-            const unsigned long long unit_begin = entry_begin + (unsigned long long)head * count;
-            skip = (uint32_t)(at - unit_begin);
-            n = (uint32_t)min((unsigned long long)(count - skip), end - at);
-            c0 = (uint32_t)(unit_begin / pl.share);
-            c1 = (uint32_t)((unit_begin + count - 1) / pl.share);
-        }
-        const uint32_t g0 = first + skip;
+        const KvSpan &span = sg.span;
+        const uint32_t sequence = sg.sequence, tile = sg.tile, head = sg.head, count = sg.count, skip = sg.skip, n = sg.n, c0 = sg.c0, c1 = sg.c1;
+        const uint32_t g0 = sg.first + skip;
         const uint8_t *base = kv_head(p.c, span.slot, head) + (size_t)g0 * L.bytes;
         const uint32_t stages = (n + SG - 1) / SG, mystages = stages > warp ? (stages - warp + WARPS - 1) / WARPS : 0;
         auto request = [&](uint32_t i) {  // the warp's stage i of this segment
@@ -725,7 +549,6 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
                 if (tid == 0) p.counters[c0] = 0;
             }
         }
-        at += n;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the ring's bytes go back to the copies
         __syncthreads();
     }
@@ -751,7 +574,7 @@ bool attention_configure() {
         const bool k8 = i & 1, v8 = i & 2;
         ok = ok && NU_EVERY(configure, 64) && NU_EVERY(configure, 128) && NU_EVERY(configure, 256);
     }
-    return ok;
+    return ok && attention_tile_configure();
 }
 
 int launch_attention(cudaStream_t s, const AttentionJob &j) {
@@ -768,6 +591,7 @@ int launch_attention(cudaStream_t s, const AttentionJob &j) {
     p.scale = j.scale * 1.4426950408889634f;
     p.window = j.window;
     p.partials = j.partials; p.counters = j.counters;
+    if (!j.generic && attention_tile_supported(j)) return launch_attention_tile(s, j, p);
     if (!j.generic && width == 64) return NU_EVERY(launch, 64, s, p, j.sm_count);
     if (!j.generic && width == 128) return NU_EVERY(launch, 128, s, p, j.sm_count);
     if (!j.generic && width == 256) return NU_EVERY(launch, 256, s, p, j.sm_count);

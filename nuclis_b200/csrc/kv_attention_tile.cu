@@ -1,0 +1,681 @@
+// Attention over the quantized cache for many query rows, to BF16: the products on the 5th-generation tensor cores.
+//
+// One block a multiprocessor walks its share of all (sequence, row tile, head) units, as the kernel for few rows does
+// (kv_attention.cu), in steps of 128 keys (64 at width 256). A unit's row tile is 256 query rows, two M = 128 tiles that share every key
+// step (one tile at width 256, whose accumulator alone takes half the tensor memory).
+//   * warps 8..11 decode: a step's keys and values become f16 in shared memory, in the 128-byte-swizzled K-major layout of
+//     the tensor core: keys as rows of dimensions, values transposed as rows of positions. The dimensions of a key's eight
+//     stand in the order 0,4,1,5,2,6,3,7 that unpacking gives, and the queries are laid out alike.
+//   * warp 12 (one thread) issues S = Q K^T and O += P V, in an order that keeps one tile's softmax under the other's products.
+//   * warps 0..7 are the softmax: a thread has a row; it reads S from tensor memory, writes P = 2^(S scale - m) as f16 over it, and
+//     the tensor core takes P from there. The maximum m is only moved when a score passes it by 8 (log2), so O is rarely rescaled.
+//
+// Range: a step's keys and values are brought near f16's upper end by a power of two each (their largest scale's), a row's query
+// by one of its own; the score's factor takes the first and last back, P that of the values relative to the largest so far. So f16's
+// 11 bits hold for every magnitude a cache can store; products are exact and sums F32. Against 64 bits the result is off by
+// its own BF16 rounding and little else (1.7e-3 relative).
+//
+// A value's scale that is NaN would reach rows that do not see its position (0 * NaN), so it is decoded as zeros and marked, and
+// the rows that do see it write NaN in its block's dimensions.
+//
+// Every wait is bounded: a thread whose wait runs out raises the block's flag, all waits then fall through, and the block
+// ends as ever with the status word raised.
+#include "kv_attention.cuh"
+#include "launch.cuh"
+
+namespace nu {
+
+using namespace attn;
+
+namespace {
+
+template <int W, bool K8, bool V8>
+struct Tile {
+    static constexpr int QT = W == 256 ? 1 : 2;    // M = 128 tiles
+    static constexpr int ROWS = QT * 128;
+    static constexpr int KT = W == 256 ? 64 : 128; // keys of a step
+    static constexpr int NB = W / 32;
+    static constexpr KvLayout L = kv_layout(W, K8, V8);
+    static constexpr int SOFT = 8, PROD = 4, THREADS = (SOFT + PROD + 1) * 32;
+    static constexpr int PARTS = 128 / KT;         // decoding threads of a key
+    static constexpr int NBT = NB / PARTS;         // a key's blocks of a thread
+    // shared memory
+    static constexpr int Q_TILE = 128 * W * 2, Q = 0, K_BYTES = KT * W * 2, K = Q + QT * Q_TILE, V = K + 2 * K_BYTES, TABLE = V + 2 * K_BYTES;
+    static constexpr int NANS = TABLE + 2 * NB * KT * 2, EXCHANGE = NANS + 4 * 2 * 128, SMALL = EXCHANGE + 3 * 256 * 4, BARS = SMALL + 128, BYTES = BARS + 32 * 8 + 1024;
+    // tensor memory columns
+    static constexpr int S_COLS = KT, O_COL = 2 * KT;
+    static constexpr int PARTIAL = ROWS * (W + 2);
+    static constexpr uint32_t SEGMENT = 6;         // steps that a block decodes in the time that a second segment costs it
+};
+
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// Bounded; falls through at once when a thread of the block has given up.
+__device__ __forceinline__ void wait_or_give_up(uint32_t bar, uint32_t parity, volatile uint32_t *abort_flag) {
+    for (uint32_t i = 0; i < SPIN_LIMIT; ++i) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (done) return;
+        if (i % 64 == 63 && *abort_flag) return;
+    }
+    *abort_flag = 1;
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// K-major f16 tile in the 128-byte swizzle: rows of 128 bytes, groups of eight rows 1024 bytes apart (version 1, swizzle mode 2).
+__device__ __forceinline__ uint64_t descriptor(uint32_t addr) {
+    return (uint64_t)((addr & 0x3ffffu) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// kind::f16, D f32, A and B f16, K-major.
+constexpr uint32_t instruction(int m, int n) { return 1u << 4 | (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24; }
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]),
+          "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]),
+          "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]),
+        "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]),
+        "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+template <int ID, int N>
+__device__ __forceinline__ void named_barrier() { asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N) : "memory"); }
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+// Byte of the 16-byte chunk `chunk` (of all a row's) of row `row` in a swizzled tile of `rows` rows.
+__device__ __forceinline__ uint32_t swizzled(uint32_t rows, uint32_t row, uint32_t chunk) {
+    return chunk / 8 * rows * 128 + row / 8 * 1024 + row % 8 * 128 + ((chunk % 8) ^ (row % 8)) * 16;
+}
+__device__ __forceinline__ uint32_t times(uint32_t codes, __half2 d) { return h2(__hmul2(as_h2(codes), d)); }
+
+template <int W, bool K8, bool V8>
+__global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const __grid_constant__ AttentionParams p) {
+    using T = Tile<W, K8, V8>;
+    constexpr int QT = T::QT, ROWS = T::ROWS, KT = T::KT, NB = T::NB;
+    constexpr KvLayout L = T::L;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    __half *table = (__half *)(smem + T::TABLE);                    // [2][NB][KT]: the values' scales of a step
+    uint8_t *nans = smem + T::NANS;                                 // [4][2][128]: blocks of a key's values with a NaN scale
+    float *exchange = (float *)(smem + T::EXCHANGE);                // [2][256] row maxima and sums between the two halves of a row (width 256), [256] row scales
+    float *row_scale = exchange + 512;
+    int *exponents = (int *)(smem + T::SMALL);                      // [4][2] of a step's keys and values
+    uint32_t *largest = (uint32_t *)(smem + T::SMALL) + 8;          // [4][2] their largest scale's bits
+    uint32_t *any_nan = largest + 8;                                // [4]
+    uint32_t *tmem_slot = any_nan + 4, *last = tmem_slot + 1;
+    volatile uint32_t *abort_flag = last + 1;
+    const uint32_t bars = smem_u32(smem + T::BARS);
+    auto bar = [&](int i) { return bars + i * 8; };
+    constexpr int K_FULL = 0, K_EMPTY = 2, V_FULL = 4, V_EMPTY = 6, S_FULL = 8, P_FULL = 10, PV_DONE = 12, Q_FULL = 14;
+    const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
+
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(bar(K_FULL + i), T::PROD);
+            mbar_init(bar(V_FULL + i), T::PROD);
+            mbar_init(bar(K_EMPTY + i), 1);
+            mbar_init(bar(V_EMPTY + i), 1);
+            mbar_init(bar(S_FULL + i), 1);
+            mbar_init(bar(P_FULL + i), T::SOFT / QT);
+            mbar_init(bar(PV_DONE + i), 1);
+        }
+        mbar_init(bar(Q_FULL), T::SOFT);
+        for (int i = 0; i < 8; ++i) largest[i] = 0;
+        for (int i = 0; i < 4; ++i) any_nan[i] = 0;
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == T::SOFT + T::PROD) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *tmem_slot;
+    wait_for_previous_operator();
+
+    const Plan pl = plan<ROWS, KT, T::SEGMENT>(p);
+    Walk<ROWS, KT> walk(pl);
+    Segment sg;
+
+    if (warp < T::SOFT) {
+        // ---- softmax: thread = row `row` of M tile `q` (width 256: columns `half` of the only tile) ----
+        const uint32_t group = warp / 4, q = QT == 2 ? group : 0, row = warp % 4 * 32 + lane;
+        const uint32_t lanes = (warp % 4 * 32) << 16;
+        constexpr int COLS = QT == 2 ? KT : KT / 2;  // of S, a thread's
+        constexpr int OCOLS = QT == 2 ? W : W / 2;   // of O
+        const uint32_t ocol = tmem + lanes + T::O_COL + (QT == 2 ? q * W : group * OCOLS);
+        uint32_t step = 0;  // over all segments
+        while (walk.next(p, pl, sg)) {
+            // the queries: a row's largest value is brought to [1, 2) by a power of two
+            const uint32_t live_rows = sg.span.count * p.group, tile_row0 = sg.tile * ROWS;
+            const size_t rows0 = (size_t)sg.sequence * p.tokens;
+            {
+                constexpr uint32_t LPR = W / 8, RPI = 32 / LPR;  // lanes a row, rows a turn
+                constexpr uint32_t MINE = ROWS / T::SOFT;        // rows of this warp: those of its threads
+                const uint32_t base = QT == 2 ? warp * 32 : warp % 4 * 32 + group * 16, chunk = lane % LPR;
+#pragma unroll 4
+                for (uint32_t i = 0; i < MINE / RPI; ++i) {
+                    const uint32_t r = base + i * RPI + lane / LPR, all = tile_row0 + r;
+                    float x[8] = {};
+                    if (all < live_rows) {
+                        const float *src = p.q + (rows0 + all / p.group) * p.q_stride + (size_t)(sg.head * p.group + all % p.group) * W + chunk * 8;
+                        if ((uintptr_t)src % 16 == 0) {
+                            const float4 a = *(const float4 *)src, b = *(const float4 *)(src + 4);
+                            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) x[k] = src[k];
+                        }
+                    }
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(x[k]) & 0x7fffffffu);
+#pragma unroll
+                    for (uint32_t o = 1; o < LPR; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    const int e = top == 0 ? 0 : min((int)max(top >> 23, 1u) - 127, 126);
+                    const bool bad = top >= 0x7f800000u;
+                    const float down = power_of_two(-e);
+                    if (chunk == 0) row_scale[r] = bad ? NAN : p.scale * power_of_two(e);
+                    uint4 out;
+                    out.x = h2(__floats2half2_rn(x[0] * down, x[4] * down));
+                    out.y = h2(__floats2half2_rn(x[1] * down, x[5] * down));
+                    out.z = h2(__floats2half2_rn(x[2] * down, x[6] * down));
+                    out.w = h2(__floats2half2_rn(x[3] * down, x[7] * down));
+                    if (bad) out = make_uint4(0u, 0u, 0u, 0u);
+                    *(uint4 *)(smem + T::Q + r / 128 * T::Q_TILE + swizzled(128, r % 128, chunk)) = out;
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(Q_FULL));
+            if (QT == 1) named_barrier<1, 256>();  // the two halves of a row share its scale
+            const uint32_t all = tile_row0 + q * 128 + row;
+            const bool live = all < live_rows;
+            const uint32_t pos = live ? sg.span.first + all / p.group : 0;
+            const uint32_t low = live ? (p.window && pos >= p.window ? pos - p.window + 1 : 0) : 1;  // sees [low, pos]; a dead row nothing
+            const uint32_t first_pos = sg.span.first + tile_row0 / p.group, last_pos = sg.span.first + (min(live_rows, tile_row0 + ROWS) - 1) / p.group;
+            const uint32_t all_low = p.window && last_pos >= p.window ? last_pos - p.window + 1 : 0;  // every live row sees [all_low, first_pos]
+            const float rs = row_scale[q * 128 + row];
+            float m = -INFINITY, l = 0.0f;
+            int big = 0;            // exponent that O carries
+            uint32_t nan_blocks = 0;
+
+            for (uint32_t i = 0; i < sg.n; ++i, ++step) {
+                const uint32_t buffer = QT == 2 ? q : step & 1u, ring = step & 3u;
+                const uint32_t key0 = (sg.first + sg.skip + i) * KT + (QT == 1 ? group * COLS : 0);
+                const bool edge = key0 < all_low || key0 + COLS - 1 > first_pos;
+                wait_or_give_up(bar(S_FULL + buffer), (QT == 2 ? step : step >> 1) & 1u, abort_flag);
+                fence_after();
+                const int ek = exponents[ring * 2], ev = exponents[ring * 2 + 1];
+                float factor = rs * power_of_two(ek);
+                factor = factor < 1.2e-38f ? 1.2e-38f : factor;  // a masked score is minus infinity times this
+                const uint32_t scol = tmem + lanes + buffer * T::S_COLS;
+                uint32_t v[32];
+                auto hide = [&](int c0) {
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) {
+                        const uint32_t key = key0 + c0 + c;
+                        if (key < low || key > pos) v[c] = 0xff800000u;
+                    }
+                };
+                float top = -INFINITY;
+#pragma unroll
+                for (int c0 = 0; c0 < COLS; c0 += 32) {
+                    tmem_load32(scol + (QT == 1 ? group * COLS : 0) + c0, v);
+                    tmem_load_wait();
+                    if (edge) hide(c0);
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) top = fmaxf(top, __uint_as_float(v[c]));
+                }
+                top *= factor;
+                if (QT == 1) {  // both halves have S in registers now: P may take its place
+                    exchange[(step & 1u) * 256 + tid] = top;
+                    named_barrier<1, 256>();
+                    top = fmaxf(top, exchange[(step & 1u) * 256 + (tid ^ 128u)]);
+                }
+                bool waited = i == 0;
+                if (i == 0) {
+                    m = top;
+                    big = ev;
+                } else if (__any_sync(0xffffffffu, top > m + 8.0f) || ev > big) {
+                    const float next = fmaxf(m, top), fl = m == -INFINITY ? 0.0f : exp2_approx(m - next);
+                    const int next_big = max(big, ev);
+                    const float f = fl * power_of_two(max(big - next_big, -126));
+                    m = next;
+                    l *= fl;
+                    big = next_big;
+                    wait_or_give_up(bar(PV_DONE + q), (step - 1) & 1u, abort_flag);
+                    waited = true;
+                    fence_after();
+#pragma unroll 1
+                    for (int c0 = 0; c0 < OCOLS; c0 += 32) {
+                        uint32_t o[32];
+                        tmem_load32(ocol + c0, o);
+                        tmem_load_wait();
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
+                        tmem_store32(ocol + c0, o);
+                    }
+                    tmem_store_wait();
+                }
+                const int shift = max(ev - big, -100);
+                const float offset = (float)shift - (m == -INFINITY ? 0.0f : m);
+                float sum = 0.0f;
+#pragma unroll
+                for (int c0 = 0; c0 < COLS; c0 += 32) {
+                    if (QT == 2) {
+                        tmem_load32(scol + c0, v);
+                        tmem_load_wait();
+                        if (edge) hide(c0);
+                    }
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int c = 0; c < 32; c += 2) {
+                        const float a = exp2_approx(fmaf(__uint_as_float(v[c]), factor, offset)), b = exp2_approx(fmaf(__uint_as_float(v[c + 1]), factor, offset));
+                        sum += a + b;
+                        pk[c / 2] = h2(__floats2half2_rn(a, b));
+                        v[c] = __float_as_uint(a);
+                        v[c + 1] = __float_as_uint(b);
+                    }
+                    tmem_store16(scol + ((QT == 1 ? group * COLS : 0) + c0) / 2, pk);
+                    if (any_nan[ring]) {
+                        const uint32_t k0 = (QT == 1 ? group * COLS : 0) + c0;
+#pragma unroll 1
+                        for (int c = 0; c < 32; ++c) {
+                            float w = 0.0f;
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) w = k == c ? __uint_as_float(v[k]) : w;
+                            if (w > 0.0f) nan_blocks |= nans[ring * 256 + k0 + c] | nans[ring * 256 + 128 + k0 + c];
+                        }
+                    }
+                }
+                l += sum * power_of_two(-shift);
+                tmem_store_wait();
+                if (!waited) wait_or_give_up(bar(PV_DONE + q), (step - 1) & 1u, abort_flag);
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(P_FULL + q));
+            }
+
+            // ---- the result, or this block's part of it ----
+            wait_or_give_up(bar(PV_DONE + q), (step - 1) & 1u, abort_flag);
+            fence_after();
+            if (QT == 1) {  // every thread has read the last maxima: the product that was waited for has all their rows
+                exchange[tid] = l;
+                exchange[256 + tid] = __uint_as_float(nan_blocks);
+                named_barrier<1, 256>();
+                l += exchange[tid ^ 128u];
+                nan_blocks |= __float_as_uint(exchange[256 + (tid ^ 128u)]);
+                named_barrier<1, 256>();
+            }
+            const bool whole = sg.n == sg.count;
+            const float up = power_of_two(max(min(big, 127), -126)) * (whole ? 1.0f / l : 1.0f);
+            float *partial = p.partials + ((size_t)blockIdx.x * 2 + (sg.skip == 0)) * T::PARTIAL;  // a unit that starts here goes into the second place
+            const uint32_t dim0 = QT == 2 ? 0 : group * OCOLS;
+#pragma unroll 1
+            for (int c0 = 0; c0 < OCOLS; c0 += 32) {
+                uint32_t o[32];
+                tmem_load32(ocol + c0, o);
+                tmem_load_wait();
+                const bool nan = nan_blocks >> ((dim0 + c0) / 32) & 1u;
+#pragma unroll
+                for (int c = 0; c < 32; ++c) o[c] = nan ? 0x7fffffffu : __float_as_uint(__uint_as_float(o[c]) * up);
+                if (!whole) {
+                    float4 *dst = (float4 *)(partial + (size_t)(q * 128 + row) * W + dim0 + c0);
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) dst[c] = make_float4(__uint_as_float(o[c * 4]), __uint_as_float(o[c * 4 + 1]), __uint_as_float(o[c * 4 + 2]), __uint_as_float(o[c * 4 + 3]));
+                } else if (live) {
+                    __nv_bfloat16 *dst = (__nv_bfloat16 *)p.out + (rows0 + all / p.group) * p.out_stride + (size_t)(sg.head * p.group + all % p.group) * W + dim0 + c0;
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) {
+                        const __nv_bfloat162 pair = __floats2bfloat162_rn(__uint_as_float(o[2 * c]), __uint_as_float(o[2 * c + 1]));
+                        pk[c] = *(const uint32_t *)&pair;
+                    }
+                    if ((uintptr_t)dst % 16 == 0) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) ((uint4 *)dst)[c] = make_uint4(pk[c * 4], pk[c * 4 + 1], pk[c * 4 + 2], pk[c * 4 + 3]);
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) dst[c] = __ushort_as_bfloat16((unsigned short)(pk[c / 2] >> (c % 2 * 16)));
+                    }
+                }
+            }
+            if (!whole) {
+                if (QT == 2 || group == 0) {
+                    partial[ROWS * W + q * 128 + row] = m;
+                    partial[ROWS * W + ROWS + q * 128 + row] = l;
+                }
+                __threadfence();
+                named_barrier<1, 256>();
+                if (tid == 0) *last = atomicAdd(p.counters + sg.c0, 1u) == sg.c1 - sg.c0;
+                named_barrier<1, 256>();
+                if (*last) {  // this block arrived last: the parts of all blocks, in their order; a warp takes a row at a time
+                    __threadfence();
+                    const uint32_t parts = sg.c1 - sg.c0 + 1;
+                    auto part = [&](uint32_t c) { return p.partials + ((size_t)(sg.c0 + c) * 2 + (c == 0)) * T::PARTIAL; };
+                    for (uint32_t r = warp; r < (uint32_t)ROWS; r += T::SOFT) {
+                        const uint32_t to = tile_row0 + r;
+                        if (to >= live_rows) break;
+                        float mm = -INFINITY, ll = 0.0f;
+                        for (uint32_t c = 0; c < parts; ++c) mm = fmaxf(mm, __ldcg(part(c) + ROWS * W + r));
+                        const float ref = mm == -INFINITY ? 0.0f : mm;
+                        constexpr int EACH = W / 32;
+                        float acc[EACH] = {};
+#pragma unroll 4
+                        for (uint32_t c = 0; c < parts; ++c) {
+                            const float f = exp2_approx(__ldcg(part(c) + ROWS * W + r) - ref);
+                            ll += __ldcg(part(c) + ROWS * W + ROWS + r) * f;
+#pragma unroll
+                            for (int k = 0; k < EACH; ++k) {
+                                const float x = __ldcg(part(c) + (size_t)r * W + k * 32 + lane);
+                                acc[k] = f > 0.0f ? fmaf(x, f, acc[k]) : acc[k];  // a part that the row does not see may hold anything
+                            }
+                        }
+                        __nv_bfloat16 *dst = (__nv_bfloat16 *)p.out + (rows0 + to / p.group) * p.out_stride + (size_t)(sg.head * p.group + to % p.group) * W;
+                        const float inv = 1.0f / ll;
+#pragma unroll
+                        for (int k = 0; k < EACH; ++k) dst[k * 32 + lane] = __float2bfloat16_rn(acc[k] * inv);
+                    }
+                    if (tid == 0) p.counters[sg.c0] = 0;
+                }
+            }
+        }
+        fence_before();
+    } else if (warp < T::SOFT + T::PROD) {
+        // ---- decoding: thread = (key, part of its blocks) for the keys, (granule, dimension mod 8, part) for the values ----
+        const uint32_t t = tid - T::SOFT * 32, key = t % KT, part = t / KT;
+        constexpr int KW = (K8 ? 2 : 1) * T::NBT;                        // a lane slot's words of the key, of this thread
+        constexpr int KVEC = L.k_vec, KVECS = KW * 4 / KVEC;
+        constexpr int VPARTS = 128 / (KT / 16 * 8);                      // threads of a (granule, dimension mod 8)
+        constexpr int VW = (V8 ? W / 8 : W / 16) / VPARTS;               // words of a lane slot, of this thread
+        constexpr int VBLOCKS = VW / (V8 ? 4 : 2);                       // blocks they belong to
+        const uint32_t vg = t / 8 % (KT / 16), vdim = t % 8, vpart = t / (KT / 2);
+        uint32_t step = 0;
+        while (walk.next(p, pl, sg)) {
+            const uint32_t live_rows = sg.span.count * p.group;
+            const uint32_t first_row = sg.tile * ROWS, last_row = min(live_rows, first_row + ROWS) - 1;
+            const uint32_t first_pos = sg.span.first + first_row / p.group, high = sg.span.first + last_row / p.group;
+            const uint32_t low = p.window && first_pos >= p.window ? first_pos - p.window + 1 : 0;   // some row sees [low, high]
+            const uint8_t *base = kv_head(p.c, sg.span.slot, sg.head);
+            uint32_t kw[4][KW], vw[4][VW], ks[T::NBT / 2], vs[T::NBT / 2];
+            // granules past `high` may lie past the slot's end: they are not read
+            auto load_keys = [&](uint32_t key0) {
+                const uint32_t at = key0 + key;
+                const uint8_t *g = base + (size_t)(at / KV_GRANULE) * L.bytes;
+                const bool in = at / KV_GRANULE <= high / KV_GRANULE;
+#pragma unroll
+                for (int i = 0; i < T::NBT / 2; ++i) {
+                    ks[i] = in ? *(const uint32_t *)(g + L.k_scales + (at % KV_GRANULE * NB + part * T::NBT) * 2 + i * 4) : 0u;
+                    vs[i] = in ? *(const uint32_t *)(g + L.v_scales + (at % KV_GRANULE * NB + part * T::NBT) * 2 + i * 4) : 0u;
+                }
+#pragma unroll
+                for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+                    for (int v = 0; v < KVECS; ++v) {
+                        const uint8_t *src = g + at % KV_GRANULE / 8 * (L.k_scales / 2) + (part * KVECS + v) * 32 * KVEC + (at % 8 * 4 + tt) * KVEC;
+                        if (KVEC == 16) {
+                            const uint4 x = in ? __ldg((const uint4 *)src) : make_uint4(0u, 0u, 0u, 0u);
+                            kw[tt][v * 4] = x.x; kw[tt][v * 4 + 1] = x.y; kw[tt][v * 4 + 2] = x.z; kw[tt][v * 4 + 3] = x.w;
+                        } else {
+                            const uint2 x = in ? __ldg((const uint2 *)src) : make_uint2(0u, 0u);
+                            kw[tt][v * 2] = x.x; kw[tt][v * 2 + 1] = x.y;
+                        }
+                    }
+            };
+            auto load_values = [&](uint32_t key0) {
+                const uint32_t gran = key0 / KV_GRANULE + vg;
+                const uint8_t *g = base + (size_t)gran * L.bytes + L.v_codes;
+                const bool in = gran <= high / KV_GRANULE;
+#pragma unroll
+                for (int tt = 0; tt < 4; ++tt) {
+#pragma unroll
+                    for (int v = 0; v < (VW + 3) / 4; ++v) {
+                        const uint32_t w0 = vpart * VW + v * 4;
+                        const uint8_t *src = g + w0 / 4 * 512 + (vdim * 4 + tt) * 16 + w0 % 4 * 4;
+                        if (VW % 4 == 0) {
+                            const uint4 x = in ? __ldg((const uint4 *)src) : make_uint4(0u, 0u, 0u, 0u);
+                            vw[tt][v * 4] = x.x; vw[tt][v * 4 + 1] = x.y; vw[tt][v * 4 + 2] = x.z; vw[tt][v * 4 + 3] = x.w;
+                        } else {
+                            const uint2 x = in ? __ldg((const uint2 *)src) : make_uint2(0u, 0u);
+                            vw[tt][0] = x.x; vw[tt][1] = x.y;
+                        }
+                    }
+                }
+            };
+            const uint32_t begin = (sg.first + sg.skip) * KT;
+            load_keys(begin);
+            load_values(begin);
+            for (uint32_t i = 0; i < sg.n; ++i, ++step) {
+                const uint32_t key0 = begin + i * KT, stage = step & 1u, ring = step & 3u, parity = (step >> 1) & 1u;
+                // the scales: what no row of the tile sees counts as zero, the largest sets the step's power of two
+                const bool seen = key0 + key >= low && key0 + key <= high;
+                float dk[T::NBT], dv[T::NBT], kmax = 0.0f, vmax = 0.0f;
+                uint32_t nan_mask = 0;
+#pragma unroll
+                for (int b = 0; b < T::NBT; ++b) {
+                    dk[b] = seen ? __half2float(__ushort_as_half((unsigned short)(ks[b / 2] >> (b % 2 * 16)))) : 0.0f;
+                    dv[b] = seen ? __half2float(__ushort_as_half((unsigned short)(vs[b / 2] >> (b % 2 * 16)))) : 0.0f;
+                    if (dv[b] != dv[b]) {
+                        nan_mask |= 1u << (part * T::NBT + b);
+                        dv[b] = 0.0f;
+                    }
+                    kmax = fmaxf(kmax, fabsf(dk[b]));
+                    vmax = fmaxf(vmax, fabsf(dv[b]));
+                }
+                const uint32_t kbits = __reduce_max_sync(0xffffffffu, __float_as_uint(kmax)), vbits = __reduce_max_sync(0xffffffffu, __float_as_uint(vmax));
+                if (lane == 0) {
+                    atomicMax(largest + ring * 2, kbits);
+                    atomicMax(largest + ring * 2 + 1, vbits);
+                }
+                nans[ring * 256 + part * 128 + key] = (uint8_t)nan_mask;
+                if (KT == 128) nans[ring * 256 + 128 + key] = 0;
+                if (nan_mask) any_nan[ring] = 1;
+                named_barrier<2, 128>();
+                // the largest product of a scale and a code comes below 2^15
+                const int ek = (int)max(largest[ring * 2] >> 23, 64u) - 127 + (K8 ? 7 : 3) - 14, ev = (int)max(largest[ring * 2 + 1] >> 23, 64u) - 127 + (V8 ? 7 : 3) - 14;
+                const float fk = power_of_two(-ek), fv = power_of_two(-ev);
+#pragma unroll
+                for (int b = 0; b < T::NBT; ++b) table[(stage * NB + part * T::NBT + b) * KT + key] = __float2half_rn(dv[b] * fv);
+                if (t == 0) {
+                    exponents[ring * 2] = ek;
+                    exponents[ring * 2 + 1] = ev;
+                    const uint32_t later = (step + 1) & 3u;  // last used by step - 3, whose products are done: a stage of the values has been refilled since
+                    largest[later * 2] = 0;
+                    largest[later * 2 + 1] = 0;
+                    any_nan[later] = 0;
+                }
+                named_barrier<2, 128>();
+
+                // keys
+                if (step >= 2) wait_or_give_up(bar(K_EMPTY + stage), parity ^ 1u, abort_flag);
+                uint8_t *kt = smem + T::K + stage * T::K_BYTES;
+#pragma unroll
+                for (int b = 0; b < T::NBT; ++b) {
+                    const __half2 d = __float2half2_rn(dk[b] * fk);
+#pragma unroll
+                    for (int tt = 0; tt < 4; ++tt) {
+                        uint4 x;
+                        if (K8) {
+                            const uint32_t w0 = kw[tt][2 * b], w1 = kw[tt][2 * b + 1];
+                            x = make_uint4(times(byte_codes(w0, 0x4140), d), times(byte_codes(w0, 0x4342), d), times(byte_codes(w1, 0x4140), d), times(byte_codes(w1, 0x4342), d));
+                        } else {
+                            const uint32_t w = kw[tt][b], w8 = w >> 8;
+                            x = make_uint4(times(low_codes(w, 0x64006400u), d), times(high_codes(w, 0x64006400u), d), times(low_codes(w8, 0x64006400u), d),
+                                           times(high_codes(w8, 0x64006400u), d));
+                        }
+                        *(uint4 *)(kt + swizzled(KT, key, (part * T::NBT + b) * 4 + tt)) = x;
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(K_FULL + stage));
+                if (i + 1 < sg.n) load_keys(key0 + KT);
+
+                // values
+                if (step >= 2) wait_or_give_up(bar(V_EMPTY + stage), parity ^ 1u, abort_flag);
+                uint8_t *vt = smem + T::V + stage * T::K_BYTES;
+#pragma unroll
+                for (int b = 0; b < VBLOCKS; ++b) {
+                    const uint32_t block = vpart * VBLOCKS + b;
+                    uint4 d[2];  // of the granule's 16 positions
+                    d[0] = *(const uint4 *)(table + (stage * NB + block) * KT + vg * 16);
+                    d[1] = *(const uint4 *)(table + (stage * NB + block) * KT + vg * 16 + 8);
+                    const uint32_t d0[4] = {d[0].x, d[0].y, d[0].z, d[0].w}, d1[4] = {d[1].x, d[1].y, d[1].z, d[1].w};
+#pragma unroll
+                    for (int w = 0; w < VW / VBLOCKS; ++w) {
+                        uint32_t a[2][4], c[2][4];  // [dimension][positions 2t, 2t + 1] of the granule's first and second half
+#pragma unroll
+                        for (int tt = 0; tt < 4; ++tt) {
+                            const uint32_t x = vw[tt][b * (VW / VBLOCKS) + w], x8 = x >> 8;
+                            if (V8) {
+                                a[0][tt] = times(byte_codes(x, 0x4140), as_h2(d0[tt]));
+                                c[0][tt] = times(byte_codes(x, 0x4342), as_h2(d1[tt]));
+                            } else {
+                                a[0][tt] = times(low_codes(x, 0x64006400u), as_h2(d0[tt]));
+                                c[0][tt] = times(low_codes(x8, 0x64006400u), as_h2(d1[tt]));
+                                a[1][tt] = times(high_codes(x, 0x64006400u), as_h2(d0[tt]));
+                                c[1][tt] = times(high_codes(x8, 0x64006400u), as_h2(d1[tt]));
+                            }
+                        }
+                        const uint32_t word = vpart * VW + b * (VW / VBLOCKS) + w;
+#pragma unroll
+                        for (int h = 0; h < (V8 ? 1 : 2); ++h) {
+                            const uint32_t dim = (V8 ? word * 8 : word * 16 + h * 8) + vdim;
+                            *(uint4 *)(vt + swizzled(W, dim, vg * 2)) = make_uint4(a[h][0], a[h][1], a[h][2], a[h][3]);
+                            *(uint4 *)(vt + swizzled(W, dim, vg * 2 + 1)) = make_uint4(c[h][0], c[h][1], c[h][2], c[h][3]);
+                        }
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(V_FULL + stage));
+                if (i + 1 < sg.n) load_values(key0 + KT);
+            }
+        }
+    } else if (lane == 0) {
+        // ---- the products ----
+        constexpr uint32_t s_desc = instruction(128, KT), o_desc = instruction(128, W);
+        uint32_t step = 0, segment = 0;
+        const uint32_t q_addr = smem_u32(smem + T::Q), k_addr = smem_u32(smem + T::K), v_addr = smem_u32(smem + T::V);
+        auto scores = [&](uint32_t q, uint32_t at) {  // S of step `at`
+            const uint32_t buffer = QT == 2 ? q : at & 1u, k = k_addr + (at & 1u) * T::K_BYTES;
+#pragma unroll
+            for (int s = 0; s < W / 16; ++s)
+                mma_ss(tmem + buffer * T::S_COLS, descriptor(q_addr + q * T::Q_TILE + s / 4 * 128 * 128 + s % 4 * 32), descriptor(k + s / 4 * KT * 128 + s % 4 * 32), s_desc, s != 0);
+            commit(bar(S_FULL + buffer));
+        };
+        while (walk.next(p, pl, sg)) {
+            wait_or_give_up(bar(Q_FULL), segment & 1u, abort_flag);
+            wait_or_give_up(bar(K_FULL + (step & 1u)), (step >> 1) & 1u, abort_flag);
+            fence_after();
+            for (uint32_t q = 0; q < QT; ++q) scores(q, step);
+            commit(bar(K_EMPTY + (step & 1u)));
+            for (uint32_t i = 0; i < sg.n; ++i, ++step) {
+                const uint32_t next = step + 1;
+                const bool more = i + 1 < sg.n;
+                if (more) {
+                    wait_or_give_up(bar(K_FULL + (next & 1u)), (next >> 1) & 1u, abort_flag);
+                    fence_after();
+                    if (QT == 1) {
+                        scores(0, next);
+                        commit(bar(K_EMPTY + (next & 1u)));
+                    }
+                }
+                for (uint32_t q = 0; q < QT; ++q) {
+                    wait_or_give_up(bar(P_FULL + q), step & 1u, abort_flag);
+                    if (q == 0) wait_or_give_up(bar(V_FULL + (step & 1u)), (step >> 1) & 1u, abort_flag);
+                    fence_after();
+                    const uint32_t pcol = tmem + (QT == 2 ? q : step & 1u) * T::S_COLS, v = v_addr + (step & 1u) * T::K_BYTES;
+#pragma unroll
+                    for (int s = 0; s < KT / 16; ++s)
+                        mma_ts(tmem + T::O_COL + q * W, pcol + s * 8, descriptor(v + s / 4 * W * 128 + s % 4 * 32), o_desc, i != 0 || s != 0);
+                    commit(bar(PV_DONE + q));
+                    if (QT == 2 && more) scores(q, next);
+                }
+                commit(bar(V_EMPTY + (step & 1u)));
+                if (QT == 2 && more) commit(bar(K_EMPTY + (next & 1u)));
+            }
+            ++segment;
+        }
+    }
+    __syncwarp();
+    __syncthreads();
+    if (warp == T::SOFT + T::PROD) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+    if (tid == 0 && *abort_flag) *(volatile uint32_t *)p.c.status = 1u;
+}
+
+template <int W, bool K8, bool V8>
+bool configure() {
+    return cudaFuncSetAttribute(tile_kernel<W, K8, V8>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<W, K8, V8>::BYTES) == cudaSuccess;
+}
+template <int W, bool K8, bool V8>
+int launch(cudaStream_t s, AttentionParams p, int sm_count) {
+    using T = Tile<W, K8, V8>;
+    p.tiles = (uint32_t)(((uint64_t)p.tokens * p.group + T::ROWS - 1) / T::ROWS);
+    launch_after_previous_smem(tile_kernel<W, K8, V8>, dim3(sm_count), dim3(T::THREADS), T::BYTES, s, p);
+    return 1;
+}
+#define NU_EVERY(F, W, ...) (k8 ? (v8 ? F<W, true, true>(__VA_ARGS__) : F<W, true, false>(__VA_ARGS__)) : (v8 ? F<W, false, true>(__VA_ARGS__) : F<W, false, false>(__VA_ARGS__)))
+
+}  // namespace
+
+bool attention_tile_configure() {
+    bool ok = true;
+    for (int i = 0; i < 4; ++i) {
+        const bool k8 = i & 1, v8 = i & 2;
+        ok = ok && NU_EVERY(configure, 64) && NU_EVERY(configure, 128) && NU_EVERY(configure, 256);
+    }
+    return ok;
+}
+
+bool attention_tile_supported(const AttentionJob &j) {
+    const uint32_t w = j.cache.width;
+    return j.bf16 && (w == 64 || w == 128 || w == 256) && (uint64_t)j.tokens * (j.heads / j.cache.heads) >= 64;
+}
+
+int launch_attention_tile(cudaStream_t s, const AttentionJob &j, AttentionParams p) {
+    const bool k8 = j.cache.k8, v8 = j.cache.v8;
+    const uint32_t w = j.cache.width;
+    if (w == 64) return NU_EVERY(launch, 64, s, p, j.sm_count);
+    if (w == 128) return NU_EVERY(launch, 128, s, p, j.sm_count);
+    return NU_EVERY(launch, 256, s, p, j.sm_count);
+}
+
+}  // namespace nu

@@ -225,6 +225,104 @@ def test_attention_against_64_bits(backend, kenc, venc, width, group, rows, leng
         assert rel_l2(plain, want) <= 1e-5
 
 
+# many rows to BF16: the tensor-core kernel's tiles of 256 rows (128 at width 256) and steps of 128 keys (64)
+PROMPTS = [(128, 1, 64, 64, 0), (128, 5, 13, 13, 0), (128, 5, 60, 300, 0), (128, 8, 33, 1000, 0), (128, 1, 300, 300, 0), (128, 2, 200, 777, 130), (64, 1, 70, 500, 0),
+           (64, 4, 100, 129, 0), (64, 16, 20, 2000, 5), (256, 4, 16, 16, 0), (256, 5, 50, 700, 0), (256, 1, 200, 260, 64), (256, 3, 129, 400, 0)]
+
+
+@pytest.mark.parametrize("width,group,rows,length,window", PROMPTS)
+@pytest.mark.parametrize("kenc,venc", PAIRS)
+def test_many_rows_to_bf16(backend, kenc, venc, width, group, rows, length, window):
+    """16-bit operands: q, k, v and p are rounded to 11 bits once each (2^-11 of a term at most, 4 x 2^-12 / sqrt(3) of random sign: 6e-4 of the
+    result and less), the result to BF16's 8 (2^-8 at most): relative L2 within one half step, 2^-8."""
+    b = backend
+    heads = 2
+    shape = KvCache(2, (length + 15) // 16 * 16, heads, width, kenc, venc)
+    with Held(b) as held:
+        cache, k, v, rng = case(b, held, shape, [5, length], length + width + rows)
+        q = rng.standard_normal((rows, heads * group, width)) * 1.5
+        spans = [(1, length - rows, rows)]
+        want = kv_oracle.attention(q.astype(np.float32), k[1], v[1], length - rows, group, window=window)
+        got = attend(b, held, cache, shape, spans, rows, q, heads * group, window=window, dtype=enc.BF16)
+        assert rel_l2(got, want) <= 2.0 ** -8
+        np.testing.assert_array_equal(got, attend(b, held, cache, shape, spans, rows, q, heads * group, window=window, pad=3, dtype=enc.BF16))
+
+
+@pytest.mark.parametrize("width", [64, 128, 256])
+def test_many_rows_of_a_batch_to_bf16(backend, width):
+    b = backend
+    group, rows = 3, 90
+    lengths = [90, 91, 300, 1, 650, 40]
+    shape = KvCache(len(lengths), 656, 2, width, enc.Q8_0, enc.Q4_0)
+    with Held(b) as held:
+        cache, k, v, rng = case(b, held, shape, lengths, 78)
+        q = rng.standard_normal((len(lengths) * rows, 2 * group, width)).astype(np.float32)
+        spans = [(0, 0, 90), (1, 1, 90), (2, 230, 70), (3, 0, 1), (4, 0, 0), (4, 600, 50)]
+        for window in (0, 33):
+            got = attend(b, held, cache, shape, spans, rows, q, 2 * group, window=window, dtype=enc.BF16).reshape(len(spans), rows, 2 * group, width)
+            for s, (slot, first, count) in enumerate(spans):
+                if count:
+                    want = kv_oracle.attention(q[s * rows: s * rows + count], k[slot], v[slot], first, group, window=window)
+                    assert rel_l2(got[s, :count], want) <= 2.0 ** -8, s
+                assert np.all(got[s, count:].view(np.uint32) == 0xc1c10000), s  # padding rows are left as they were
+
+
+@pytest.mark.parametrize("kenc,venc", PAIRS[:2])
+@pytest.mark.parametrize("width", [64, 128, 256])
+def test_many_rows_beside_values_they_do_not_see(backend, width, kenc, venc):
+    """NaN and huge values ahead of a window and behind the last position, a NaN that some rows of the call see, queries of all sizes."""
+    b = backend
+    group, rows, length, window = 2, 100, 400, 200
+    shape = KvCache(1, 480, 1, width, kenc, venc)
+    with Held(b) as held:
+        cache, k, v, rng = case(b, held, shape, [length], 15)
+        bad = np.full((60, 1, width), np.nan, np.float32)
+        huge = np.full((60, 1, width), 3e38, np.float32)
+        write(b, held, cache, shape, [(0, length, 40)], 60, bad, bad)
+        write(b, held, cache, shape, [(0, length + 40, 10)], 60, huge, huge)
+        write(b, held, cache, shape, [(0, 0, 55)], 60, bad, huge)
+        q = (rng.standard_normal((rows, group, width)) * np.array([1e-30, 2.0])[:, None]).astype(np.float32)
+        q[7, 0] = 0
+        spans = [(0, length - rows, rows)]
+        want = kv_oracle.attention(q, k[0], v[0], length - rows, group, window=window)
+        got = attend(b, held, cache, shape, spans, rows, q, group, window=window, dtype=enc.BF16)
+        assert rel_l2(got[:, 0], want[:, 0]) <= 2.0 ** -8 and rel_l2(got[:, 1], want[:, 1]) <= 2.0 ** -8
+        # position 350 (row 50): NaN keys for every row that sees it
+        write(b, held, cache, shape, [(0, 350, 1)], 1, bad[:1], v[0, 350:351].astype(np.float32))
+        got = attend(b, held, cache, shape, spans, rows, q, group, window=window, dtype=enc.BF16)
+        assert rel_l2(got[:50], want[:50]) <= 2.0 ** -8 and np.all(np.isnan(got[50:]))
+        # a NaN block of its values: those dimensions of the rows that see it
+        one = v[0, 350:351].astype(np.float32)
+        one[0, 0, 40] = np.nan
+        write(b, held, cache, shape, [(0, 350, 1)], 1, k[0, 350:351].astype(np.float32), one)
+        got = attend(b, held, cache, shape, spans, rows, q, group, window=window, dtype=enc.BF16)
+        assert rel_l2(got[:50], want[:50]) <= 2.0 ** -8
+        assert np.all(np.isnan(got[50:, :, 32:64])) and np.all(np.isfinite(np.delete(got[50:], np.s_[32:64], 2)))
+        # a NaN query stays in its row
+        q[3, 1, 5] = np.nan
+        got = attend(b, held, cache, shape, spans, rows, q, group, window=window, dtype=enc.BF16)
+        assert np.all(np.isnan(got[3, 1])) and np.all(np.isfinite(got[3, 0])) and rel_l2(got[10:50], want[10:50]) <= 2.0 ** -8
+
+
+@pytest.mark.parametrize("gain", [1e-6, 1e4])
+@pytest.mark.parametrize("venc", [enc.Q8_0, enc.Q4_0])
+def test_many_rows_and_values_of_all_sizes(backend, gain, venc):
+    """Scales that rise and fall by orders of magnitude along the sequence, beyond what f16 holds of the values themselves."""
+    b = backend
+    shape = KvCache(1, 912, 1, 128, enc.Q4_0, venc)
+    rng = np.random.default_rng(12)
+    k, v = (rng.standard_normal((900, 1, 128)).astype(np.float32) for _ in range(2))
+    v *= np.exp(rng.uniform(-3, 3, (900, 1, 1))).astype(np.float32) * np.float32(gain)
+    k *= np.float32(gain)
+    with Held(b) as held:
+        cache = held.new(shape.bytes)
+        write(b, held, cache, shape, [(0, 0, 900)], 900, k, v)
+        q = (rng.standard_normal((150, 2, 128)) / gain).astype(np.float32)
+        sk, sv = kv_oracle.stored(k, enc.Q4_0), kv_oracle.stored(v, venc)
+        want = kv_oracle.attention(q, sk, sv, 750, 2)
+        assert rel_l2(attend(b, held, cache, shape, [(0, 750, 150)], 150, q, 2, dtype=enc.BF16), want) <= 2.0 ** -8
+
+
 @pytest.mark.parametrize("width", [64, 128, 256, 96])
 def test_a_batch_of_unlike_sequences(backend, width):
     """Lengths from one position to many, an absent sequence, padding rows, two sequences on one slot."""
