@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
     wait_for_previous_operator();
 
     const Plan pl = plan<ROWS, KV_GRANULE, S::SEGMENT>(p);
-    Walk<ROWS, KV_GRANULE> walk(pl);
+    Walk<ROWS, KV_GRANULE, S::SEGMENT> walk(pl);
     Segment sg;
 
     uint32_t turn = 0;  // stages this warp has taken, over all segments: position and phase in the ring

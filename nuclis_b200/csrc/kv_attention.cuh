@@ -80,9 +80,12 @@ __device__ __forceinline__ void unit_range(const AttentionParams &p, const KvSpa
     count = high / STEP + 1 - first;
 }
 
+// A unit costs its block SEGMENT steps before and after its own (queries, join, result): an equal share counts them as steps, ahead of
+// the unit's.
+//
 // Where a block starts: which entry ((sequence, row tile), all of whose heads have the same steps) and how far into it.
 struct Plan {
-    bool even;                      // every block has one part of one unit; else an equal share of all steps
+    bool even;                      // every block has one part of one unit; else an equal share of all steps (and segments)
     unsigned long long share, total;
     uint32_t entry, in;             // in: blocks (even) or steps into the entry
     bool idle;
@@ -114,8 +117,8 @@ __device__ __forceinline__ Plan plan(const AttentionParams &p) {
     total *= heads;
     units *= heads;
     Plan r{};
-    r.total = total;
-    r.share = (total + blocks - 1) / blocks;
+    r.total = total + units * SEGMENT;
+    r.share = (r.total + blocks - 1) / blocks;
     if (total == 0) { r.idle = true; return r; }
     // Even parts: 1 + count * spare / total blocks for a unit of `count` steps, at most `blocks` together. Taken if the longest part
     // is not much longer than an equal share, which costs most blocks a second segment.
@@ -134,7 +137,7 @@ __device__ __forceinline__ Plan plan(const AttentionParams &p) {
     r.idle = true;
     for (uint32_t e0 = 0; e0 < entries; e0 += 32) {
         const uint32_t c = cached(e0 + lane);
-        const unsigned long long mine = c == 0 ? 0 : (unsigned long long)(r.even ? parts(c) : c) * heads;
+        const unsigned long long mine = c == 0 ? 0 : (unsigned long long)(r.even ? parts(c) : c + SEGMENT) * heads;
         unsigned long long upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -166,7 +169,7 @@ struct Segment {
 };
 
 // Walks a block's plan; the same in every thread that walks it.
-template <uint32_t ROWS, uint32_t STEP>
+template <uint32_t ROWS, uint32_t STEP, uint32_t SEGMENT>
 struct Walk {
     unsigned long long at, end, entry_begin;
     uint32_t entry;
@@ -193,19 +196,22 @@ struct Walk {
                 s.c1 = s.c0 + (s.count - 1) / share;
                 return true;
             }
-            const unsigned long long all = (unsigned long long)s.count * p.c.heads;
+            const uint32_t cost = s.count ? s.count + SEGMENT : 0;
+            const unsigned long long all = (unsigned long long)cost * p.c.heads;
             if (at - entry_begin >= all) {  // all its heads are done (or it has no rows)
                 entry_begin += all;
                 ++entry;
                 continue;
             }
-            s.head = (uint32_t)((at - entry_begin) / s.count);
-            const unsigned long long unit_begin = entry_begin + (unsigned long long)s.head * s.count;
-            s.skip = (uint32_t)(at - unit_begin);
-            s.n = (uint32_t)min((unsigned long long)(s.count - s.skip), end - at);
-            s.c0 = (uint32_t)(unit_begin / pl.share);
-            s.c1 = (uint32_t)((unit_begin + s.count - 1) / pl.share);
-            at += s.n;
+            s.head = (uint32_t)((at - entry_begin) / cost);
+            const unsigned long long unit_begin = entry_begin + (unsigned long long)s.head * cost;
+            const uint32_t from = (uint32_t)(at - unit_begin), to = (uint32_t)min((unsigned long long)cost, end - unit_begin);
+            at += to - from;
+            if (to <= SEGMENT) continue;  // the share ends ahead of the unit's first step
+            s.skip = max(from, SEGMENT) - SEGMENT;
+            s.n = to - SEGMENT - s.skip;
+            s.c0 = (uint32_t)((unit_begin + SEGMENT) / pl.share);
+            s.c1 = (uint32_t)((unit_begin + cost - 1) / pl.share);
             return true;
         }
         return false;

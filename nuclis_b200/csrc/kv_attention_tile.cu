@@ -36,7 +36,10 @@ struct Tile {
     static constexpr int KT = W == 256 ? 64 : 128; // keys of a step
     static constexpr int NB = W / 32;
     static constexpr KvLayout L = kv_layout(W, K8, V8);
-    static constexpr int SOFT = 8, PROD = 4, THREADS = (SOFT + PROD + 1) * 32;
+    static constexpr int SOFT = 8, PROD = 4, THREADS = (SOFT + PROD + 4) * 32;  // + the warpgroup of the warp that issues
+    // Registers a thread of the three kinds: together the 128 x 512 that the block starts with
+    static constexpr int SOFT_REGS = 176, PROD_REGS = 104, MMA_REGS = 56;
+    static_assert(SOFT * SOFT_REGS + PROD * PROD_REGS + 4 * MMA_REGS <= 16 * 128, "more registers than the block has");
     static constexpr int PARTS = 128 / KT;         // decoding threads of a key
     static constexpr int NBT = NB / PARTS;         // a key's blocks of a thread
     // shared memory
@@ -69,23 +72,59 @@ __device__ __forceinline__ void wait_or_give_up(uint32_t bar, uint32_t parity, v
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar) : "memory");
 }
-// K-major f16 tile in the 128-byte swizzle: rows of 128 bytes, groups of eight rows 1024 bytes apart (version 1, swizzle mode 2).
-__device__ __forceinline__ uint64_t descriptor(uint32_t addr) {
-    return (uint64_t)((addr & 0x3ffffu) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+template <int N>
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+// Two F32 operations at once.
+__device__ __forceinline__ uint64_t two(float a, float b) { return (uint64_t)__float_as_uint(a) | (uint64_t)__float_as_uint(b) << 32; }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
 }
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float low_of(uint64_t x) { return __uint_as_float((uint32_t)x); }
+__device__ __forceinline__ float high_of(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
+// Shared-memory descriptor of a K-major f16 tile in the 128-byte swizzle: rows of 128 bytes, groups of eight rows 1024 bytes
+// apart (version 1, swizzle mode 2). The high word is the same for all; the low one has the address.
+constexpr uint32_t DESC_HIGH = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t descriptor(uint32_t addr) { return (addr & 0x3ffffu) >> 4 | 1u << 16; }
 // kind::f16, D f32, A and B f16, K-major.
 constexpr uint32_t instruction(int m, int n) { return 1u << 4 | (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24; }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-                 : "memory");
+// Four steps of 16 along K, one swizzle atom: 32 bytes, two units of a descriptor, further each. The whole warp comes here, so that
+// the operands stay in uniform registers, and one lane issues: with a lane alone in a branch every operand had to be moved there,
+// some 130 cycles a product that itself takes 32 to 64.
+__device__ __forceinline__ void mma_ss4(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred e, p, q;\n\t.reg .b64 a, b;\n\t.reg .b32 x, y;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.eq.u32 q, %4, %4;\n\t"
+        "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t"
+        "add.u32 x, %1, 2;\n\tadd.u32 y, %2, 2;\n\tmov.b64 a, {x, %5};\n\tmov.b64 b, {y, %5};\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, q;\n\t"
+        "add.u32 x, %1, 4;\n\tadd.u32 y, %2, 4;\n\tmov.b64 a, {x, %5};\n\tmov.b64 b, {y, %5};\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, q;\n\t"
+        "add.u32 x, %1, 6;\n\tadd.u32 y, %2, 6;\n\tmov.b64 a, {x, %5};\n\tmov.b64 b, {y, %5};\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, q;\n\t}"
+        ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(DESC_HIGH)
+        : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
-                 : "memory");
+// The same with A in tensor memory: 16 f16 along K are eight columns.
+__device__ __forceinline__ void mma_ts4(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred e, p, q;\n\t.reg .b64 b;\n\t.reg .b32 x, y;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.eq.u32 q, %4, %4;\n\t"
+        "mov.b64 b, {%2, %5};\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t"
+        "add.u32 x, %1, 8;\n\tadd.u32 y, %2, 2;\n\tmov.b64 b, {y, %5};\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, q;\n\t"
+        "add.u32 x, %1, 16;\n\tadd.u32 y, %2, 4;\n\tmov.b64 b, {y, %5};\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, q;\n\t"
+        "add.u32 x, %1, 24;\n\tadd.u32 y, %2, 6;\n\tmov.b64 b, {y, %5};\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, q;\n\t}"
+        ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(DESC_HIGH)
+        : "memory");
 }
-__device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&v)[32]) {
+__device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t *v) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
         "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -167,10 +206,11 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
     wait_for_previous_operator();
 
     const Plan pl = plan<ROWS, KT, T::SEGMENT>(p);
-    Walk<ROWS, KT> walk(pl);
+    Walk<ROWS, KT, T::SEGMENT> walk(pl);
     Segment sg;
 
     if (warp < T::SOFT) {
+        more_registers<T::SOFT_REGS>();
         // ---- softmax: thread = row `row` of M tile `q` (width 256: columns `half` of the only tile) ----
         const uint32_t group = warp / 4, q = QT == 2 ? group : 0, row = warp % 4 * 32 + lane;
         const uint32_t lanes = (warp % 4 * 32) << 16;
@@ -186,36 +226,55 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                 constexpr uint32_t LPR = W / 8, RPI = 32 / LPR;  // lanes a row, rows a turn
                 constexpr uint32_t MINE = ROWS / T::SOFT;        // rows of this warp: those of its threads
                 const uint32_t base = QT == 2 ? warp * 32 : warp % 4 * 32 + group * 16, chunk = lane % LPR;
-#pragma unroll 4
-                for (uint32_t i = 0; i < MINE / RPI; ++i) {
-                    const uint32_t r = base + i * RPI + lane / LPR, all = tile_row0 + r;
-                    float x[8] = {};
-                    if (all < live_rows) {
-                        const float *src = p.q + (rows0 + all / p.group) * p.q_stride + (size_t)(sg.head * p.group + all % p.group) * W + chunk * 8;
-                        if ((uintptr_t)src % 16 == 0) {
-                            const float4 a = *(const float4 *)src, b = *(const float4 *)(src + 4);
-                            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-                        } else {
+                constexpr uint32_t TURNS = MINE / RPI, BATCH = TURNS < 8 ? TURNS : 8;
+                const bool aligned = ((uintptr_t)p.q | p.q_stride * 4) % 16 == 0;
+                auto source = [&](uint32_t r) -> const float * {
+                    const uint32_t all = tile_row0 + r;
+                    return all < live_rows ? p.q + (rows0 + all / p.group) * p.q_stride + (size_t)(sg.head * p.group + all % p.group) * W + chunk * 8 : nullptr;
+                };
+#pragma unroll 1
+                for (uint32_t i0 = 0; i0 < TURNS; i0 += BATCH) {
+                    float x[BATCH][8];
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) x[k] = src[k];
+                    for (uint32_t i = 0; i < BATCH; ++i) {
+                        const float *src = source(base + (i0 + i) * RPI + lane / LPR);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) x[i][k] = 0.0f;
+                        if (src && aligned) {
+                            const float4 a = *(const float4 *)src, b = *(const float4 *)(src + 4);
+                            x[i][0] = a.x; x[i][1] = a.y; x[i][2] = a.z; x[i][3] = a.w; x[i][4] = b.x; x[i][5] = b.y; x[i][6] = b.z; x[i][7] = b.w;
                         }
                     }
-                    uint32_t top = 0;
+                    if (!aligned) {
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(x[k]) & 0x7fffffffu);
+                        for (uint32_t i = 0; i < BATCH; ++i) {
+                            const float *src = source(base + (i0 + i) * RPI + lane / LPR);
+                            if (src) {
 #pragma unroll
-                    for (uint32_t o = 1; o < LPR; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-                    const int e = top == 0 ? 0 : min((int)max(top >> 23, 1u) - 127, 126);
-                    const bool bad = top >= 0x7f800000u;
-                    const float down = power_of_two(-e);
-                    if (chunk == 0) row_scale[r] = bad ? NAN : p.scale * power_of_two(e);
-                    uint4 out;
-                    out.x = h2(__floats2half2_rn(x[0] * down, x[4] * down));
-                    out.y = h2(__floats2half2_rn(x[1] * down, x[5] * down));
-                    out.z = h2(__floats2half2_rn(x[2] * down, x[6] * down));
-                    out.w = h2(__floats2half2_rn(x[3] * down, x[7] * down));
-                    if (bad) out = make_uint4(0u, 0u, 0u, 0u);
-                    *(uint4 *)(smem + T::Q + r / 128 * T::Q_TILE + swizzled(128, r % 128, chunk)) = out;
+                                for (int k = 0; k < 8; ++k) x[i][k] = src[k];
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (uint32_t i = 0; i < BATCH; ++i) {
+                        const uint32_t r = base + (i0 + i) * RPI + lane / LPR;
+                        uint32_t top = 0;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(x[i][k]) & 0x7fffffffu);
+#pragma unroll
+                        for (uint32_t o = 1; o < LPR; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                        const int e = top == 0 ? 0 : min((int)max(top >> 23, 1u) - 127, 126);
+                        const bool bad = top >= 0x7f800000u;
+                        const float down = power_of_two(-e);
+                        if (chunk == 0) row_scale[r] = bad ? NAN : p.scale * power_of_two(e);
+                        uint4 out;
+                        out.x = h2(__floats2half2_rn(x[i][0] * down, x[i][4] * down));
+                        out.y = h2(__floats2half2_rn(x[i][1] * down, x[i][5] * down));
+                        out.z = h2(__floats2half2_rn(x[i][2] * down, x[i][6] * down));
+                        out.w = h2(__floats2half2_rn(x[i][3] * down, x[i][7] * down));
+                        if (bad) out = make_uint4(0u, 0u, 0u, 0u);
+                        *(uint4 *)(smem + T::Q + r / 128 * T::Q_TILE + swizzled(128, r % 128, chunk)) = out;
+                    }
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -243,23 +302,23 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                 float factor = rs * power_of_two(ek);
                 factor = factor < 1.2e-38f ? 1.2e-38f : factor;  // a masked score is minus infinity times this
                 const uint32_t scol = tmem + lanes + buffer * T::S_COLS;
-                uint32_t v[32];
-                auto hide = [&](int c0) {
+                uint32_t v[COLS];
 #pragma unroll
-                    for (int c = 0; c < 32; ++c) {
-                        const uint32_t key = key0 + c0 + c;
-                        if (key < low || key > pos) v[c] = 0xff800000u;
-                    }
-                };
-                float top = -INFINITY;
+                for (int c0 = 0; c0 < COLS; c0 += 32) tmem_load32(scol + (QT == 1 ? group * COLS : 0) + c0, v + c0);
+                tmem_load_wait();
+                if (edge) {
+                    // columns [from, to] of this thread's are seen
+                    const int to = pos < key0 ? -1 : (int)min(pos - key0, (uint32_t)COLS), from = low > key0 ? (int)min(low - key0, (uint32_t)COLS) : 0;
 #pragma unroll
-                for (int c0 = 0; c0 < COLS; c0 += 32) {
-                    tmem_load32(scol + (QT == 1 ? group * COLS : 0) + c0, v);
-                    tmem_load_wait();
-                    if (edge) hide(c0);
-#pragma unroll
-                    for (int c = 0; c < 32; ++c) top = fmaxf(top, __uint_as_float(v[c]));
+                    for (int c = 0; c < COLS; ++c)
+                        if (c > to || c < from) v[c] = 0xff800000u;
                 }
+                float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < COLS; c += 8)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) tops[k] = fmaxf(tops[k], fmaxf(__uint_as_float(v[c + k]), __uint_as_float(v[c + 4 + k])));
+                float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
                 top *= factor;
                 if (QT == 1) {  // both halves have S in registers now: P may take its place
                     exchange[(step & 1u) * 256 + tid] = top;
@@ -293,35 +352,28 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                 }
                 const int shift = max(ev - big, -100);
                 const float offset = (float)shift - (m == -INFINITY ? 0.0f : m);
-                float sum = 0.0f;
+                const uint64_t factor2 = two(factor, factor), offset2 = two(offset, offset);
+                uint64_t sums[4] = {0, 0, 0, 0};
 #pragma unroll
                 for (int c0 = 0; c0 < COLS; c0 += 32) {
-                    if (QT == 2) {
-                        tmem_load32(scol + c0, v);
-                        tmem_load_wait();
-                        if (edge) hide(c0);
-                    }
                     uint32_t pk[16];
 #pragma unroll
                     for (int c = 0; c < 32; c += 2) {
-                        const float a = exp2_approx(fmaf(__uint_as_float(v[c]), factor, offset)), b = exp2_approx(fmaf(__uint_as_float(v[c + 1]), factor, offset));
-                        sum += a + b;
+                        const uint64_t z = fma2((uint64_t)v[c0 + c] | (uint64_t)v[c0 + c + 1] << 32, factor2, offset2);
+                        const float a = exp2_approx(low_of(z)), b = exp2_approx(high_of(z));
+                        sums[c / 2 % 4] = add2(sums[c / 2 % 4], two(a, b));
                         pk[c / 2] = h2(__floats2half2_rn(a, b));
-                        v[c] = __float_as_uint(a);
-                        v[c + 1] = __float_as_uint(b);
                     }
                     tmem_store16(scol + ((QT == 1 ? group * COLS : 0) + c0) / 2, pk);
-                    if (any_nan[ring]) {
+                    if (any_nan[ring]) {  // the blocks that are NaN at a position this row has weight on
                         const uint32_t k0 = (QT == 1 ? group * COLS : 0) + c0;
-#pragma unroll 1
-                        for (int c = 0; c < 32; ++c) {
-                            float w = 0.0f;
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) w = k == c ? __uint_as_float(v[k]) : w;
-                            if (w > 0.0f) nan_blocks |= nans[ring * 256 + k0 + c] | nans[ring * 256 + 128 + k0 + c];
-                        }
+                        for (int c = 0; c < 32; ++c)
+                            if (pk[c / 2] >> (c % 2 * 16) & 0xffffu) nan_blocks |= nans[ring * 256 + k0 + c] | nans[ring * 256 + 128 + k0 + c];
                     }
                 }
+                sums[0] = add2(add2(sums[0], sums[1]), add2(sums[2], sums[3]));
+                const float sum = low_of(sums[0]) + high_of(sums[0]);
                 l += sum * power_of_two(-shift);
                 tmem_store_wait();
                 if (!waited) wait_or_give_up(bar(PV_DONE + q), (step - 1) & 1u, abort_flag);
@@ -357,22 +409,38 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                     float4 *dst = (float4 *)(partial + (size_t)(q * 128 + row) * W + dim0 + c0);
 #pragma unroll
                     for (int c = 0; c < 8; ++c) dst[c] = make_float4(__uint_as_float(o[c * 4]), __uint_as_float(o[c * 4 + 1]), __uint_as_float(o[c * 4 + 2]), __uint_as_float(o[c * 4 + 3]));
-                } else if (live) {
-                    __nv_bfloat16 *dst = (__nv_bfloat16 *)p.out + (rows0 + all / p.group) * p.out_stride + (size_t)(sg.head * p.group + all % p.group) * W + dim0 + c0;
+                } else {  // to this warp's rows of the queries' place: no product reads them any more
                     uint32_t pk[16];
 #pragma unroll
                     for (int c = 0; c < 16; ++c) {
                         const __nv_bfloat162 pair = __floats2bfloat162_rn(__uint_as_float(o[2 * c]), __uint_as_float(o[2 * c + 1]));
                         pk[c] = *(const uint32_t *)&pair;
                     }
-                    if ((uintptr_t)dst % 16 == 0) {
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) ((uint4 *)dst)[c] = make_uint4(pk[c * 4], pk[c * 4 + 1], pk[c * 4 + 2], pk[c * 4 + 3]);
+                    for (int c = 0; c < 4; ++c)
+                        *(uint4 *)(smem + T::Q + q * T::Q_TILE + swizzled(128, row, (dim0 + c0) / 8 + c)) = make_uint4(pk[c * 4], pk[c * 4 + 1], pk[c * 4 + 2], pk[c * 4 + 3]);
+                }
+            }
+            if (whole) {  // and on, whole runs of a row at a time
+                __syncwarp();
+                constexpr uint32_t CHUNKS = OCOLS / 8;
+                const bool aligned = ((uintptr_t)p.out | p.out_stride * 2) % 16 == 0;
+#pragma unroll 4
+                for (uint32_t i = lane; i < 32 * CHUNKS; i += 32) {
+                    const uint32_t r = warp % 4 * 32 + i / CHUNKS, chunk = dim0 / 8 + i % CHUNKS, to = tile_row0 + q * 128 + r;
+                    if (to >= live_rows) continue;
+                    const uint4 x = *(const uint4 *)(smem + T::Q + q * T::Q_TILE + swizzled(128, r, chunk));
+                    __nv_bfloat16 *dst = (__nv_bfloat16 *)p.out + (rows0 + to / p.group) * p.out_stride + (size_t)(sg.head * p.group + to % p.group) * W + chunk * 8;
+                    if (aligned) {
+                        *(uint4 *)dst = x;
                     } else {
+                        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                        for (int c = 0; c < 32; ++c) dst[c] = __ushort_as_bfloat16((unsigned short)(pk[c / 2] >> (c % 2 * 16)));
+                        for (int c = 0; c < 8; ++c) dst[c] = __ushort_as_bfloat16((unsigned short)(w[c / 2] >> (c % 2 * 16)));
                     }
                 }
+                if (QT == 1) named_barrier<1, 256>();  // a row's next queries are written by either half
+                else __syncwarp();
             }
             if (!whole) {
                 if (QT == 2 || group == 0) {
@@ -416,6 +484,7 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
         }
         fence_before();
     } else if (warp < T::SOFT + T::PROD) {
+        fewer_registers<T::PROD_REGS>();
         // ---- decoding: thread = (key, part of its blocks) for the keys, (granule, dimension mod 8, part) for the values ----
         const uint32_t t = tid - T::SOFT * 32, key = t % KT, part = t / KT;
         constexpr int KW = (K8 ? 2 : 1) * T::NBT;                        // a lane slot's words of the key, of this thread
@@ -586,27 +655,30 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                 if (i + 1 < sg.n) load_values(key0 + KT);
             }
         }
-    } else if (lane == 0) {
-        // ---- the products ----
+    } else {
+        // ---- the products: the first warp of the last warpgroup ----
+        fewer_registers<T::MMA_REGS>();
         constexpr uint32_t s_desc = instruction(128, KT), o_desc = instruction(128, W);
         uint32_t step = 0, segment = 0;
-        const uint32_t q_addr = smem_u32(smem + T::Q), k_addr = smem_u32(smem + T::K), v_addr = smem_u32(smem + T::V);
+        const uint32_t base = __reduce_max_sync(0xffffffffu, tmem);  // (a uniform register)
+        const uint32_t q_desc = descriptor(smem_u32(smem + T::Q)), k_desc = descriptor(smem_u32(smem + T::K)), v_desc = descriptor(smem_u32(smem + T::V));
         auto scores = [&](uint32_t q, uint32_t at) {  // S of step `at`
-            const uint32_t buffer = QT == 2 ? q : at & 1u, k = k_addr + (at & 1u) * T::K_BYTES;
+            const uint32_t buffer = QT == 2 ? q : at & 1u, k = k_desc + (at & 1u) * (T::K_BYTES / 16);
 #pragma unroll
-            for (int s = 0; s < W / 16; ++s)
-                mma_ss(tmem + buffer * T::S_COLS, descriptor(q_addr + q * T::Q_TILE + s / 4 * 128 * 128 + s % 4 * 32), descriptor(k + s / 4 * KT * 128 + s % 4 * 32), s_desc, s != 0);
+            for (int s = 0; s < W / 64; ++s) mma_ss4(base + buffer * T::S_COLS, q_desc + (q * T::Q_TILE + s * 128 * 128) / 16, k + s * KT * 128 / 16, s_desc, s != 0);
             commit(bar(S_FULL + buffer));
         };
-        while (walk.next(p, pl, sg)) {
+        while (warp == T::SOFT + T::PROD && walk.next(p, pl, sg)) {
+            const uint32_t n = __reduce_max_sync(0xffffffffu, sg.n);
             wait_or_give_up(bar(Q_FULL), segment & 1u, abort_flag);
             wait_or_give_up(bar(K_FULL + (step & 1u)), (step >> 1) & 1u, abort_flag);
             fence_after();
+#pragma unroll
             for (uint32_t q = 0; q < QT; ++q) scores(q, step);
             commit(bar(K_EMPTY + (step & 1u)));
-            for (uint32_t i = 0; i < sg.n; ++i, ++step) {
+            for (uint32_t i = 0; i < n; ++i, ++step) {
                 const uint32_t next = step + 1;
-                const bool more = i + 1 < sg.n;
+                const bool more = i + 1 < n;
                 if (more) {
                     wait_or_give_up(bar(K_FULL + (next & 1u)), (next >> 1) & 1u, abort_flag);
                     fence_after();
@@ -615,14 +687,14 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                         commit(bar(K_EMPTY + (next & 1u)));
                     }
                 }
+#pragma unroll
                 for (uint32_t q = 0; q < QT; ++q) {
                     wait_or_give_up(bar(P_FULL + q), step & 1u, abort_flag);
                     if (q == 0) wait_or_give_up(bar(V_FULL + (step & 1u)), (step >> 1) & 1u, abort_flag);
                     fence_after();
-                    const uint32_t pcol = tmem + (QT == 2 ? q : step & 1u) * T::S_COLS, v = v_addr + (step & 1u) * T::K_BYTES;
+                    const uint32_t pcol = base + (QT == 2 ? q : step & 1u) * T::S_COLS, v = v_desc + (step & 1u) * (T::K_BYTES / 16);
 #pragma unroll
-                    for (int s = 0; s < KT / 16; ++s)
-                        mma_ts(tmem + T::O_COL + q * W, pcol + s * 8, descriptor(v + s / 4 * W * 128 + s % 4 * 32), o_desc, i != 0 || s != 0);
+                    for (int s = 0; s < KT / 64; ++s) mma_ts4(base + T::O_COL + q * W, pcol + s * 32, v + s * W * 128 / 16, o_desc, i != 0 || s != 0);
                     commit(bar(PV_DONE + q));
                     if (QT == 2 && more) scores(q, next);
                 }
