@@ -10,7 +10,7 @@
 //   * warps 0..7 are the softmax: a thread has a row; it reads S from tensor memory, writes P = 2^(S scale - m) as f16 over it, and
 //     the tensor core takes P from there. The maximum m is only moved when a score passes it by 8 (log2), so O is rarely rescaled.
 //
-// Range: a step's keys and values are brought near f16's upper end by a power of two each (their largest scale's), a row's query
+// Range: a step's keys and values are brought into f16's range by a power of two each (their largest scale's), a row's query
 // by one of its own; the score's factor takes the first and last back, P that of the values relative to the largest so far. So f16's
 // 11 bits hold for every magnitude a cache can store; products are exact and sums F32. Against 64 bits the result is off by
 // its own BF16 rounding and little else (1.7e-3 relative).
@@ -37,14 +37,14 @@ struct Tile {
     static constexpr int NB = W / 32;
     static constexpr KvLayout L = kv_layout(W, K8, V8);
     static constexpr int SOFT = 8, PROD = 4, THREADS = (SOFT + PROD + 4) * 32;  // + the warpgroup of the warp that issues
-    // Registers a thread of the three kinds: together the 128 x 512 that the block starts with
-    static constexpr int SOFT_REGS = 176, PROD_REGS = 104, MMA_REGS = 56;
-    static_assert(SOFT * SOFT_REGS + PROD * PROD_REGS + 4 * MMA_REGS <= 16 * 128, "more registers than the block has");
+    // Registers a thread, of the 128 x 512 that the block starts with: the softmax keeps its 128, the issuing warpgroup gives to the decoding one
+    static constexpr int PROD_REGS = 168, MMA_REGS = 88;
+    static_assert(SOFT * 128 + PROD * PROD_REGS + 4 * MMA_REGS <= 16 * 128, "more registers than the block has");
     static constexpr int PARTS = 128 / KT;         // decoding threads of a key
     static constexpr int NBT = NB / PARTS;         // a key's blocks of a thread
     // shared memory
     static constexpr int Q_TILE = 128 * W * 2, Q = 0, K_BYTES = KT * W * 2, K = Q + QT * Q_TILE, V = K + 2 * K_BYTES, TABLE = V + 2 * K_BYTES;
-    static constexpr int NANS = TABLE + 2 * NB * KT * 2, EXCHANGE = NANS + 4 * 2 * 128, SMALL = EXCHANGE + 3 * 256 * 4, BARS = SMALL + 128, BYTES = BARS + 32 * 8 + 1024;
+    static constexpr int NANS = TABLE + 6 * NB * KT * 2, EXCHANGE = NANS + 4 * 2 * 128, SMALL = EXCHANGE + 3 * 256 * 4, BARS = SMALL + 128, BYTES = BARS + 32 * 8 + 1024;
     // tensor memory columns
     static constexpr int S_COLS = KT, O_COL = 2 * KT;
     static constexpr int PARTIAL = ROWS * (W + 2);
@@ -151,12 +151,31 @@ __device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::l
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 template <int ID, int N>
 __device__ __forceinline__ void named_barrier() { asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N) : "memory"); }
+// A barrier of the decoding warps that returns whether any of their threads says yes.
+__device__ __forceinline__ bool barrier_or(bool mine) {
+    uint32_t any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(any) : "r"((uint32_t)mine) : "memory");
+    return any != 0;
+}
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+// The 16-byte chunk that eight dimensions 32 b + 8 t .. of a row are kept in: an order in which the lanes (g, t) of a tile of keys, eight at
+// a time, meet no bank twice.
+__host__ __device__ constexpr uint32_t chunk_of(uint32_t b, uint32_t t) { return b / 2 * 8 + 2 * t + b % 2; }
 // Byte of the 16-byte chunk `chunk` (of all a row's) of row `row` in a swizzled tile of `rows` rows.
 __device__ __forceinline__ uint32_t swizzled(uint32_t rows, uint32_t row, uint32_t chunk) {
     return chunk / 8 * rows * 128 + row / 8 * 1024 + row % 8 * 128 + ((chunk % 8) ^ (row % 8)) * 16;
 }
-__device__ __forceinline__ uint32_t times(uint32_t codes, __half2 d) { return h2(__hmul2(as_h2(codes), d)); }
+// A code without sign, left where it lies in its word, is the f16 code * 2^-24 (16 times that from a high nibble): times 2^24 of
+// the scale, less the offset's share, is the value in one operation. All of it is kept 2^24 / (the largest scale's power of two) up.
+__device__ __forceinline__ uint32_t value2(uint32_t codes, uint32_t d, uint32_t c) { return h2(__hfma2(as_h2(codes), as_h2(d), as_h2(c))); }
+template <bool Q8>
+struct Scale {  // of a block, twice
+    uint32_t low, high, offset;
+    __device__ __forceinline__ explicit Scale(uint32_t d) : low(d) {
+        high = Q8 ? d : h2(__hmul2(as_h2(d), __float2half2_rn(0.0625f)));
+        offset = h2(__hmul2(as_h2(d), __float2half2_rn(Q8 ? -128.0f / 16777216.0f : -8.0f / 16777216.0f)));
+    }
+};
 
 template <int W, bool K8, bool V8>
 __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const __grid_constant__ AttentionParams p) {
@@ -164,8 +183,10 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
     constexpr int QT = T::QT, ROWS = T::ROWS, KT = T::KT, NB = T::NB;
     constexpr KvLayout L = T::L;
     extern __shared__ uint8_t smem_raw[];
-    uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    __half *table = (__half *)(smem + T::TABLE);                    // [2][NB][KT]: the values' scales of a step
+    uint8_t *smem = smem_raw + ((0u - smem_u32(smem_raw)) & 1023u);  // (an offset, so that the pointer stays one to shared memory)
+    __half *value_scales = (__half *)(smem + T::TABLE);             // [2][NB][KT] of a step
+    __half *value_offsets = value_scales + 2 * NB * KT;             // [2][NB][KT]: what their codes' offset takes off
+    __half *key_scales = value_offsets + 2 * NB * KT;               // [2][KT][NB]
     uint8_t *nans = smem + T::NANS;                                 // [4][2][128]: blocks of a key's values with a NaN scale
     float *exchange = (float *)(smem + T::EXCHANGE);                // [2][256] row maxima and sums between the two halves of a row (width 256), [256] row scales
     float *row_scale = exchange + 512;
@@ -191,7 +212,6 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
         }
         mbar_init(bar(Q_FULL), T::SOFT);
         for (int i = 0; i < 8; ++i) largest[i] = 0;
-        for (int i = 0; i < 4; ++i) any_nan[i] = 0;
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -210,7 +230,6 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
     Segment sg;
 
     if (warp < T::SOFT) {
-        more_registers<T::SOFT_REGS>();
         // ---- softmax: thread = row `row` of M tile `q` (width 256: columns `half` of the only tile) ----
         const uint32_t group = warp / 4, q = QT == 2 ? group : 0, row = warp % 4 * 32 + lane;
         const uint32_t lanes = (warp % 4 * 32) << 16;
@@ -273,7 +292,7 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                         out.z = h2(__floats2half2_rn(x[i][2] * down, x[i][6] * down));
                         out.w = h2(__floats2half2_rn(x[i][3] * down, x[i][7] * down));
                         if (bad) out = make_uint4(0u, 0u, 0u, 0u);
-                        *(uint4 *)(smem + T::Q + r / 128 * T::Q_TILE + swizzled(128, r % 128, chunk)) = out;
+                        *(uint4 *)(smem + T::Q + r / 128 * T::Q_TILE + swizzled(128, r % 128, chunk_of(chunk / 4, chunk % 4))) = out;
                     }
                 }
             }
@@ -302,22 +321,31 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                 float factor = rs * power_of_two(ek);
                 factor = factor < 1.2e-38f ? 1.2e-38f : factor;  // a masked score is minus infinity times this
                 const uint32_t scol = tmem + lanes + buffer * T::S_COLS;
-                uint32_t v[COLS];
+                // S in chunks of 32 columns, the next on its way while one is worked on; twice, first for the maximum (at width 256 a
+                // thread's one chunk stays)
+                constexpr int CHUNKS = COLS / 32;
+                const uint32_t sfirst = scol + (QT == 1 ? group * COLS : 0);
+                uint32_t v[QT][32];
+                // columns [from, to] of this thread's are seen
+                const int to = pos < key0 ? -1 : (int)min(pos - key0, (uint32_t)COLS), from = low > key0 ? (int)min(low - key0, (uint32_t)COLS) : 0;
+                auto hide = [&](uint32_t (&x)[32], int c0) {
 #pragma unroll
-                for (int c0 = 0; c0 < COLS; c0 += 32) tmem_load32(scol + (QT == 1 ? group * COLS : 0) + c0, v + c0);
-                tmem_load_wait();
-                if (edge) {
-                    // columns [from, to] of this thread's are seen
-                    const int to = pos < key0 ? -1 : (int)min(pos - key0, (uint32_t)COLS), from = low > key0 ? (int)min(low - key0, (uint32_t)COLS) : 0;
-#pragma unroll
-                    for (int c = 0; c < COLS; ++c)
-                        if (c > to || c < from) v[c] = 0xff800000u;
-                }
+                    for (int c = 0; c < 32; ++c)
+                        if (c > to - c0 || c < from - c0) x[c] = 0xff800000u;
+                };
                 float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                tmem_load32(sfirst, v[0]);
 #pragma unroll
-                for (int c = 0; c < COLS; c += 8)
+                for (int k = 0; k < CHUNKS; ++k) {
+                    uint32_t (&x)[32] = v[k % QT];
+                    tmem_load_wait();
+                    if (QT == 2) tmem_load32(sfirst + (k + 1) % CHUNKS * 32, v[(k + 1) % QT]);
+                    if (edge) hide(x, k * 32);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) tops[k] = fmaxf(tops[k], fmaxf(__uint_as_float(v[c + k]), __uint_as_float(v[c + 4 + k])));
+                    for (int c = 0; c < 32; c += 8)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) tops[j] = fmaxf(tops[j], fmaxf(__uint_as_float(x[c + j]), __uint_as_float(x[c + 4 + j])));
+                }
                 float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
                 top *= factor;
                 if (QT == 1) {  // both halves have S in registers now: P may take its place
@@ -355,18 +383,32 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                 const uint64_t factor2 = two(factor, factor), offset2 = two(offset, offset);
                 uint64_t sums[4] = {0, 0, 0, 0};
 #pragma unroll
-                for (int c0 = 0; c0 < COLS; c0 += 32) {
+                for (int k = 0; k < CHUNKS; ++k) {
+                    uint32_t (&x)[32] = v[k % QT];
+                    if (QT == 2) {
+                        tmem_load_wait();
+                        if (k + 1 < CHUNKS) tmem_load32(sfirst + (k + 1) * 32, v[(k + 1) % QT]);
+                        if (edge) hide(x, k * 32);
+                    }
                     uint32_t pk[16];
 #pragma unroll
                     for (int c = 0; c < 32; c += 2) {
-                        const uint64_t z = fma2((uint64_t)v[c0 + c] | (uint64_t)v[c0 + c + 1] << 32, factor2, offset2);
-                        const float a = exp2_approx(low_of(z)), b = exp2_approx(high_of(z));
-                        sums[c / 2 % 4] = add2(sums[c / 2 % 4], two(a, b));
-                        pk[c / 2] = h2(__floats2half2_rn(a, b));
+                        const uint64_t z = fma2((uint64_t)x[c] | (uint64_t)x[c + 1] << 32, factor2, offset2);
+                        x[c] = (uint32_t)z;
+                        x[c + 1] = (uint32_t)(z >> 32);
                     }
-                    tmem_store16(scol + ((QT == 1 ? group * COLS : 0) + c0) / 2, pk);
+                    // all of a chunk's powers ahead of their first use: the unit that makes them takes 8 cycles a warp and answers after some 20
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+r"(x[c]));
+#pragma unroll
+                    for (int c = 0; c < 32; c += 2) {
+                        sums[c / 2 % 4] = add2(sums[c / 2 % 4], (uint64_t)x[c] | (uint64_t)x[c + 1] << 32);
+                        pk[c / 2] = h2(__floats2half2_rn(__uint_as_float(x[c]), __uint_as_float(x[c + 1])));
+                    }
+                    // over S: half as wide, so over columns that have been read
+                    tmem_store16(scol + ((QT == 1 ? group * COLS : 0) + k * 32) / 2, pk);
                     if (any_nan[ring]) {  // the blocks that are NaN at a position this row has weight on
-                        const uint32_t k0 = (QT == 1 ? group * COLS : 0) + c0;
+                        const uint32_t k0 = (QT == 1 ? group * COLS : 0) + k * 32;
 #pragma unroll
                         for (int c = 0; c < 32; ++c)
                             if (pk[c / 2] >> (c % 2 * 16) & 0xffffu) nan_blocks |= nans[ring * 256 + k0 + c] | nans[ring * 256 + 128 + k0 + c];
@@ -484,15 +526,16 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
         }
         fence_before();
     } else if (warp < T::SOFT + T::PROD) {
-        fewer_registers<T::PROD_REGS>();
-        // ---- decoding: thread = (key, part of its blocks) for the keys, (granule, dimension mod 8, part) for the values ----
-        const uint32_t t = tid - T::SOFT * 32, key = t % KT, part = t / KT;
-        constexpr int KW = (K8 ? 2 : 1) * T::NBT;                        // a lane slot's words of the key, of this thread
-        constexpr int KVEC = L.k_vec, KVECS = KW * 4 / KVEC;
-        constexpr int VPARTS = 128 / (KT / 16 * 8);                      // threads of a (granule, dimension mod 8)
-        constexpr int VW = (V8 ? W / 8 : W / 16) / VPARTS;               // words of a lane slot, of this thread
-        constexpr int VBLOCKS = VW / (V8 ? 4 : 2);                       // blocks they belong to
-        const uint32_t vg = t / 8 % (KT / 16), vdim = t % 8, vpart = t / (KT / 2);
+        more_registers<T::PROD_REGS>();
+        // ---- decoding: a warp has KT / 64 granules of a step. Keys: lane (g, t) its own vectors of a tile of eight; values: lane (half, words w,
+        // g) the four lanes' words of two neighbouring words, which are eight positions each of a dimension and (Q4_0) the one eight on ----
+        const uint32_t t = tid - T::SOFT * 32, key = t % KT, part = t / KT, pw = warp - T::SOFT, g8 = lane / 4, t4 = lane % 4;
+        constexpr int GRANULES = KT / 64;                                      // of a warp
+        constexpr int KVEC = L.k_vec, KWORDS = KVEC / 4;                       // words of a vector
+        constexpr int KVECS = (K8 ? 2 : 1) * NB / KWORDS, KITEMS = 2 * GRANULES * KVECS;  // vectors of a tile of eight keys; of a warp in a step
+        constexpr int VVECS = W / (V8 ? 8 : 16) / 4, VITEMS = GRANULES * VVECS / 2;       // vectors of a granule; a half warp's in a step
+        const uint32_t half = lane / 16, vpair = lane / 8 % 2, vg = lane % 8;
+        const uint32_t vgran = GRANULES == 2 ? half : 0, vskip = GRANULES == 2 ? 0 : half, vturn = GRANULES == 2 ? 1 : 2;  // vector i * vturn + vskip of granule vgran
         uint32_t step = 0;
         while (walk.next(p, pl, sg)) {
             const uint32_t live_rows = sg.span.count * p.group;
@@ -500,60 +543,54 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
             const uint32_t first_pos = sg.span.first + first_row / p.group, high = sg.span.first + last_row / p.group;
             const uint32_t low = p.window && first_pos >= p.window ? first_pos - p.window + 1 : 0;   // some row sees [low, high]
             const uint8_t *base = kv_head(p.c, sg.span.slot, sg.head);
-            uint32_t kw[4][KW], vw[4][VW], ks[T::NBT / 2], vs[T::NBT / 2];
-            // granules past `high` may lie past the slot's end: they are not read
-            auto load_keys = [&](uint32_t key0) {
+            const uint32_t last_granule = high / KV_GRANULE;  // what is behind it may lie past the slot's end: it is not read
+            uint32_t kw[KITEMS][KWORDS], vw[VITEMS][4][2], ks[T::NBT / 2], vs[T::NBT / 2];
+            auto load_scales = [&](uint32_t key0) {
                 const uint32_t at = key0 + key;
-                const uint8_t *g = base + (size_t)(at / KV_GRANULE) * L.bytes;
-                const bool in = at / KV_GRANULE <= high / KV_GRANULE;
+                const uint8_t *g = base + (size_t)(at / KV_GRANULE) * L.bytes + (at % KV_GRANULE * NB + part * T::NBT) * 2;
+                const bool in = at / KV_GRANULE <= last_granule;
 #pragma unroll
                 for (int i = 0; i < T::NBT / 2; ++i) {
-                    ks[i] = in ? *(const uint32_t *)(g + L.k_scales + (at % KV_GRANULE * NB + part * T::NBT) * 2 + i * 4) : 0u;
-                    vs[i] = in ? *(const uint32_t *)(g + L.v_scales + (at % KV_GRANULE * NB + part * T::NBT) * 2 + i * 4) : 0u;
+                    ks[i] = in ? *(const uint32_t *)(g + L.k_scales + i * 4) : 0u;
+                    vs[i] = in ? *(const uint32_t *)(g + L.v_scales + i * 4) : 0u;
                 }
+            };
+            auto load_keys = [&](uint32_t key0) {
+                const uint32_t gran = key0 / KV_GRANULE + pw * GRANULES;
+                const uint8_t *g = base + (size_t)gran * L.bytes + lane * KVEC;
 #pragma unroll
-                for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-                    for (int v = 0; v < KVECS; ++v) {
-                        const uint8_t *src = g + at % KV_GRANULE / 8 * (L.k_scales / 2) + (part * KVECS + v) * 32 * KVEC + (at % 8 * 4 + tt) * KVEC;
-                        if (KVEC == 16) {
-                            const uint4 x = in ? __ldg((const uint4 *)src) : make_uint4(0u, 0u, 0u, 0u);
-                            kw[tt][v * 4] = x.x; kw[tt][v * 4 + 1] = x.y; kw[tt][v * 4 + 2] = x.z; kw[tt][v * 4 + 3] = x.w;
-                        } else {
-                            const uint2 x = in ? __ldg((const uint2 *)src) : make_uint2(0u, 0u);
-                            kw[tt][v * 2] = x.x; kw[tt][v * 2 + 1] = x.y;
-                        }
+                for (int i = 0; i < KITEMS; ++i) {
+                    const int tile = i / KVECS, v = i % KVECS;
+                    const uint8_t *src = g + tile / 2 * L.bytes + tile % 2 * (L.k_scales / 2) + v * 32 * KVEC;
+                    if (KVEC == 16) {
+                        const uint4 x = gran + tile / 2 <= last_granule ? __ldg((const uint4 *)src) : make_uint4(0u, 0u, 0u, 0u);
+                        kw[i][0] = x.x; kw[i][1] = x.y; kw[i][KWORDS - 2] = x.z; kw[i][KWORDS - 1] = x.w;
+                    } else {
+                        const uint2 x = gran + tile / 2 <= last_granule ? __ldg((const uint2 *)src) : make_uint2(0u, 0u);
+                        kw[i][0] = x.x; kw[i][1] = x.y;
                     }
+                }
             };
             auto load_values = [&](uint32_t key0) {
-                const uint32_t gran = key0 / KV_GRANULE + vg;
-                const uint8_t *g = base + (size_t)gran * L.bytes + L.v_codes;
-                const bool in = gran <= high / KV_GRANULE;
+                const uint32_t gran = key0 / KV_GRANULE + pw * GRANULES + vgran;
+                const bool in = gran <= last_granule;
+                const uint8_t *g = base + (size_t)gran * L.bytes + L.v_codes + vskip * 512 + vg * 64 + vpair * 8;
 #pragma unroll
-                for (int tt = 0; tt < 4; ++tt) {
+                for (int i = 0; i < VITEMS; ++i)
 #pragma unroll
-                    for (int v = 0; v < (VW + 3) / 4; ++v) {
-                        const uint32_t w0 = vpart * VW + v * 4;
-                        const uint8_t *src = g + w0 / 4 * 512 + (vdim * 4 + tt) * 16 + w0 % 4 * 4;
-                        if (VW % 4 == 0) {
-                            const uint4 x = in ? __ldg((const uint4 *)src) : make_uint4(0u, 0u, 0u, 0u);
-                            vw[tt][v * 4] = x.x; vw[tt][v * 4 + 1] = x.y; vw[tt][v * 4 + 2] = x.z; vw[tt][v * 4 + 3] = x.w;
-                        } else {
-                            const uint2 x = in ? __ldg((const uint2 *)src) : make_uint2(0u, 0u);
-                            vw[tt][0] = x.x; vw[tt][1] = x.y;
-                        }
+                    for (int tt = 0; tt < 4; ++tt) {
+                        const uint2 x = in ? __ldg((const uint2 *)(g + i * vturn * 512 + tt * 16)) : make_uint2(0u, 0u);
+                        vw[i][tt][0] = x.x; vw[i][tt][1] = x.y;
                     }
-                }
             };
             const uint32_t begin = (sg.first + sg.skip) * KT;
-            load_keys(begin);
-            load_values(begin);
-            for (uint32_t i = 0; i < sg.n; ++i, ++step) {
-                const uint32_t key0 = begin + i * KT, stage = step & 1u, ring = step & 3u, parity = (step >> 1) & 1u;
-                // the scales: what no row of the tile sees counts as zero, the largest sets the step's power of two
+            float dk[T::NBT], dv[T::NBT];
+            uint32_t nan_mask = 0;
+            // the scales of the step at key0 (global step `of`): what no row of the tile sees counts as zero; the largest of all sets the step's power of two
+            auto rate = [&](uint32_t key0, uint32_t of) {
                 const bool seen = key0 + key >= low && key0 + key <= high;
-                float dk[T::NBT], dv[T::NBT], kmax = 0.0f, vmax = 0.0f;
-                uint32_t nan_mask = 0;
+                float kmax = 0.0f, vmax = 0.0f;
+                nan_mask = 0;
 #pragma unroll
                 for (int b = 0; b < T::NBT; ++b) {
                     dk[b] = seen ? __half2float(__ushort_as_half((unsigned short)(ks[b / 2] >> (b % 2 * 16)))) : 0.0f;
@@ -567,92 +604,123 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                 }
                 const uint32_t kbits = __reduce_max_sync(0xffffffffu, __float_as_uint(kmax)), vbits = __reduce_max_sync(0xffffffffu, __float_as_uint(vmax));
                 if (lane == 0) {
-                    atomicMax(largest + ring * 2, kbits);
-                    atomicMax(largest + ring * 2 + 1, vbits);
+                    atomicMax(largest + (of & 3u) * 2, kbits);
+                    atomicMax(largest + (of & 3u) * 2 + 1, vbits);
                 }
-                nans[ring * 256 + part * 128 + key] = (uint8_t)nan_mask;
-                if (KT == 128) nans[ring * 256 + 128 + key] = 0;
-                if (nan_mask) any_nan[ring] = 1;
-                named_barrier<2, 128>();
-                // the largest product of a scale and a code comes below 2^15
-                const int ek = (int)max(largest[ring * 2] >> 23, 64u) - 127 + (K8 ? 7 : 3) - 14, ev = (int)max(largest[ring * 2 + 1] >> 23, 64u) - 127 + (V8 ? 7 : 3) - 14;
-                const float fk = power_of_two(-ek), fv = power_of_two(-ev);
+                nans[(of & 3u) * 256 + part * 128 + key] = (uint8_t)nan_mask;
+                if (KT == 128) nans[(of & 3u) * 256 + 128 + key] = 0;
+            };
+            // behind the barrier that follows: the powers of two, and the scales times them
+            auto publish = [&](uint32_t of, bool nan) {
+                const uint32_t ring = of & 3u;
+                const int xk = (int)max(largest[ring * 2] >> 23, 64u) - 127, xv = (int)max(largest[ring * 2 + 1] >> 23, 64u) - 127;
+                const float fk = power_of_two(14 - xk), fv = power_of_two(14 - xv);  // the largest scale to [2^14, 2^15)
 #pragma unroll
-                for (int b = 0; b < T::NBT; ++b) table[(stage * NB + part * T::NBT + b) * KT + key] = __float2half_rn(dv[b] * fv);
-                if (t == 0) {
-                    exponents[ring * 2] = ek;
-                    exponents[ring * 2 + 1] = ev;
-                    const uint32_t later = (step + 1) & 3u;  // last used by step - 3, whose products are done: a stage of the values has been refilled since
-                    largest[later * 2] = 0;
-                    largest[later * 2 + 1] = 0;
-                    any_nan[later] = 0;
+                for (int b = 0; b < T::NBT; b += 2)
+                    *(__half2 *)(key_scales + ((of & 1u) * KT + key) * NB + part * T::NBT + b) = __floats2half2_rn(dk[b] * fk, dk[b + 1] * fk);
+#pragma unroll
+                for (int b = 0; b < T::NBT; ++b) {
+                    const float d = dv[b] * fv;
+                    value_scales[((of & 1u) * NB + part * T::NBT + b) * KT + key] = __float2half_rn(d);
+                    value_offsets[((of & 1u) * NB + part * T::NBT + b) * KT + key] = __float2half_rn(d * (V8 ? -128.0f / 16777216.0f : -8.0f / 16777216.0f));
                 }
-                named_barrier<2, 128>();
-
+                if (t == 0) {
+                    exponents[ring * 2] = xk + 10;
+                    exponents[ring * 2 + 1] = xv + 10;
+                    any_nan[ring] = nan;
+                    largest[((of + 2) & 3u) * 2] = 0;  // next used two barriers on
+                    largest[((of + 2) & 3u) * 2 + 1] = 0;
+                }
+            };
+            load_scales(begin);
+            load_keys(begin);
+            load_values(begin);
+            rate(begin, step);
+            publish(step, barrier_or(nan_mask != 0));
+            named_barrier<2, 128>();
+            for (uint32_t i = 0; i < sg.n; ++i, ++step) {
+                const uint32_t key0 = begin + i * KT, stage = step & 1u, parity = (step >> 1) & 1u;
+                const bool more = i + 1 < sg.n;
+                if (more) load_scales(key0 + KT);
                 // keys
                 if (step >= 2) wait_or_give_up(bar(K_EMPTY + stage), parity ^ 1u, abort_flag);
                 uint8_t *kt = smem + T::K + stage * T::K_BYTES;
 #pragma unroll
-                for (int b = 0; b < T::NBT; ++b) {
-                    const __half2 d = __float2half2_rn(dk[b] * fk);
+                for (int j = 0; j < KITEMS; ++j) {
+                    const uint32_t row = pw * (KT / 4) + j / KVECS * 8 + g8, v = j % KVECS;
+                    constexpr int BLOCKS = KWORDS / (K8 ? 2 : 1);
+                    const uint32_t b0 = v * BLOCKS;
+                    uint32_t pairs[BLOCKS / 2];
+                    const __half *d16 = key_scales + (stage * KT + row) * NB + b0;
+                    if (BLOCKS == 4) {
+                        const uint2 x = *(const uint2 *)d16;
+                        pairs[0] = x.x; pairs[BLOCKS / 2 - 1] = x.y;
+                    } else {
+                        pairs[0] = *(const uint32_t *)d16;
+                    }
 #pragma unroll
-                    for (int tt = 0; tt < 4; ++tt) {
+                    for (int b = 0; b < BLOCKS; ++b) {
+                        const Scale<K8> d(__byte_perm(pairs[b / 2], 0u, b % 2 ? 0x3232 : 0x1010));
                         uint4 x;
                         if (K8) {
-                            const uint32_t w0 = kw[tt][2 * b], w1 = kw[tt][2 * b + 1];
-                            x = make_uint4(times(byte_codes(w0, 0x4140), d), times(byte_codes(w0, 0x4342), d), times(byte_codes(w1, 0x4140), d), times(byte_codes(w1, 0x4342), d));
+                            const uint32_t w0 = kw[j][2 * b % KWORDS], w1 = kw[j][(2 * b + 1) % KWORDS];
+                            x = make_uint4(value2(__byte_perm(w0, 0u, 0x4140), d.low, d.offset), value2(__byte_perm(w0, 0u, 0x4342), d.low, d.offset),
+                                           value2(__byte_perm(w1, 0u, 0x4140), d.low, d.offset), value2(__byte_perm(w1, 0u, 0x4342), d.low, d.offset));
                         } else {
-                            const uint32_t w = kw[tt][b], w8 = w >> 8;
-                            x = make_uint4(times(low_codes(w, 0x64006400u), d), times(high_codes(w, 0x64006400u), d), times(low_codes(w8, 0x64006400u), d),
-                                           times(high_codes(w8, 0x64006400u), d));
+                            const uint32_t w = kw[j][b], w8 = w >> 8;
+                            x = make_uint4(value2(w & 0x000f000fu, d.low, d.offset), value2(w & 0x00f000f0u, d.high, d.offset), value2(w8 & 0x000f000fu, d.low, d.offset),
+                                           value2(w8 & 0x00f000f0u, d.high, d.offset));
                         }
-                        *(uint4 *)(kt + swizzled(KT, key, (part * T::NBT + b) * 4 + tt)) = x;
+                        *(uint4 *)(kt + swizzled(KT, row, chunk_of(b0 + b, t4))) = x;
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(K_FULL + stage));
-                if (i + 1 < sg.n) load_keys(key0 + KT);
+                if (more) {
+                    load_keys(key0 + KT);
+                    rate(key0 + KT, step + 1);
+                }
+                const bool nan = barrier_or(nan_mask != 0);  // the next step's scales are rated
 
                 // values
                 if (step >= 2) wait_or_give_up(bar(V_EMPTY + stage), parity ^ 1u, abort_flag);
                 uint8_t *vt = smem + T::V + stage * T::K_BYTES;
 #pragma unroll
-                for (int b = 0; b < VBLOCKS; ++b) {
-                    const uint32_t block = vpart * VBLOCKS + b;
-                    uint4 d[2];  // of the granule's 16 positions
-                    d[0] = *(const uint4 *)(table + (stage * NB + block) * KT + vg * 16);
-                    d[1] = *(const uint4 *)(table + (stage * NB + block) * KT + vg * 16 + 8);
-                    const uint32_t d0[4] = {d[0].x, d[0].y, d[0].z, d[0].w}, d1[4] = {d[1].x, d[1].y, d[1].z, d[1].w};
+                for (int j = 0; j < VITEMS; ++j) {
+                    const uint32_t v = j * vturn + vskip, gran = pw * GRANULES + vgran, word = v * 4 + vpair * 2, block = word / (V8 ? 4 : 2);
 #pragma unroll
-                    for (int w = 0; w < VW / VBLOCKS; ++w) {
-                        uint32_t a[2][4], c[2][4];  // [dimension][positions 2t, 2t + 1] of the granule's first and second half
+                    for (int h = 0; h < 2; ++h) {  // eight positions of the granule: 2t, 2t + 1 of every t
+                        const uint4 d4 = *(const uint4 *)(value_scales + (stage * NB + block) * KT + gran * 16 + h * 8);
+                        const uint4 c4 = *(const uint4 *)(value_offsets + (stage * NB + block) * KT + gran * 16 + h * 8);
+                        const uint32_t d[4] = {d4.x, d4.y, d4.z, d4.w}, c[4] = {c4.x, c4.y, c4.z, c4.w};
 #pragma unroll
-                        for (int tt = 0; tt < 4; ++tt) {
-                            const uint32_t x = vw[tt][b * (VW / VBLOCKS) + w], x8 = x >> 8;
-                            if (V8) {
-                                a[0][tt] = times(byte_codes(x, 0x4140), as_h2(d0[tt]));
-                                c[0][tt] = times(byte_codes(x, 0x4342), as_h2(d1[tt]));
-                            } else {
-                                a[0][tt] = times(low_codes(x, 0x64006400u), as_h2(d0[tt]));
-                                c[0][tt] = times(low_codes(x8, 0x64006400u), as_h2(d1[tt]));
-                                a[1][tt] = times(high_codes(x, 0x64006400u), as_h2(d0[tt]));
-                                c[1][tt] = times(high_codes(x8, 0x64006400u), as_h2(d1[tt]));
+                        for (int w = 0; w < 2; ++w) {
+                            uint32_t x[4], y[4];  // a dimension's eight positions; Q4_0: the dimension eight on
+#pragma unroll
+                            for (int tt = 0; tt < 4; ++tt) {
+                                const uint32_t z = vw[j][tt][w];
+                                if (V8) {
+                                    x[tt] = value2(__byte_perm(z, 0u, h ? 0x4342 : 0x4140), d[tt], c[tt]);
+                                } else {
+                                    x[tt] = value2((h ? z >> 8 : z) & 0x000f000fu, d[tt], c[tt]);
+                                    y[tt] = value2((h ? z >> 12 : z >> 4) & 0x000f000fu, d[tt], c[tt]);
+                                }
                             }
-                        }
-                        const uint32_t word = vpart * VW + b * (VW / VBLOCKS) + w;
-#pragma unroll
-                        for (int h = 0; h < (V8 ? 1 : 2); ++h) {
-                            const uint32_t dim = (V8 ? word * 8 : word * 16 + h * 8) + vdim;
-                            *(uint4 *)(vt + swizzled(W, dim, vg * 2)) = make_uint4(a[h][0], a[h][1], a[h][2], a[h][3]);
-                            *(uint4 *)(vt + swizzled(W, dim, vg * 2 + 1)) = make_uint4(c[h][0], c[h][1], c[h][2], c[h][3]);
+                            const uint32_t dim = (word + w) * (V8 ? 8 : 16) + vg;
+                            *(uint4 *)(vt + swizzled(W, dim, gran * 2 + h)) = make_uint4(x[0], x[1], x[2], x[3]);
+                            if (!V8) *(uint4 *)(vt + swizzled(W, dim + 8, gran * 2 + h)) = make_uint4(y[0], y[1], y[2], y[3]);
                         }
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(V_FULL + stage));
-                if (i + 1 < sg.n) load_values(key0 + KT);
+                if (more) {
+                    load_values(key0 + KT);
+                    publish(step + 1, nan);
+                    named_barrier<2, 128>();  // the next step's scales are there
+                }
             }
         }
     } else {
