@@ -72,7 +72,9 @@ Backend *Backend::create(int device, std::string &error) {
     ok = ok && cudaMalloc(&b->partials_, kPartialsFloats * sizeof(float)) == cudaSuccess;
     ok = ok && cudaMalloc(&b->counters_, (kCounters + 3) * sizeof(uint32_t)) == cudaSuccess;
     ok = ok && cudaMemset(b->counters_, 0, (kCounters + 3) * sizeof(uint32_t)) == cudaSuccess;
-    ok = ok && cudaMallocHost(&b->status_host_, sizeof(uint32_t)) == cudaSuccess;
+    ok = ok && cudaHostAlloc(&b->status_host_, sizeof(uint32_t), cudaHostAllocMapped) == cudaSuccess;
+    ok = ok && cudaHostGetDevicePointer(&b->status_device_, b->status_host_, 0) == cudaSuccess;
+    if (ok) *b->status_host_ = 0;
     ok = ok && cudaMalloc(&b->argmax_records_, (128 * 4 + 4) * sizeof(float)) == cudaSuccess;
     ok = ok && cudaMemset(b->argmax_records_, 0, (128 * 4 + 4) * sizeof(float)) == cudaSuccess;
     if (!ok) {
@@ -324,13 +326,13 @@ int Backend::finishCapture(cudaGraphExec_t *exec) {
     return cuda(e, "commit: instantiate");
 }
 
-// Waits for everything enqueued so far and reads the kernels' status word: into pinned memory, so that the copy runs behind the
-// kernels and one wait serves both (a copy to pageable memory after the wait cost a second one, 8 us a replay).
+// Waits for everything enqueued so far and reads the kernels' status word. It lies in host memory that the kernels that have something to
+// report write to themselves, so a replay copies nothing back for it (a copy and a second wait cost 10 us of a replay's 37).
 int Backend::checkKernelStatus() {
-    if (int rc = cuda(cudaMemcpyAsync(status_host_, counters_ + counters_len_, sizeof *status_host_, cudaMemcpyDeviceToHost, stream_), "status read")) return rc;
     if (int rc = cuda(cudaStreamSynchronize(stream_), "launch: wait")) return rc;
-    const uint32_t status = *status_host_;
+    const uint32_t status = *(volatile uint32_t *)status_host_;
     if (status != 0) {
+        *(volatile uint32_t *)status_host_ = 0;
         cudaMemsetAsync(counters_, 0, (counters_len_ + 3) * sizeof(uint32_t), stream_);  // counters, status word, the chain kernel's two arrival counts
         cudaStreamSynchronize(stream_);
         if (status == 3) return fail(NU_ERR_EXECUTION, "a span of rows lies outside the key/value cache: its sequence was left out");
@@ -479,7 +481,7 @@ int Backend::matvec(const Buffer &weights, const Matrix &m, const Buffer &input,
     job.enc = m.encoding; job.layout = m.layout; job.columns = (uint32_t)m.columns; job.tokens = 1; job.in = in; job.in_stride = m.columns;
     job.count = 1; job.mode = ACT_NONE;
     job.seg[0] = {w, stride, (uint32_t)m.rows, out, m.rows};
-    job.serial = written(weights); job.partials = partials_; job.partials_floats = partials_floats_; job.counters = counters_; job.counters_len = counters_len_; job.sm_count = sm_count_;
+    job.serial = written(weights); job.partials = partials_; job.partials_floats = partials_floats_; job.counters = counters_; job.counters_len = counters_len_; job.status = status_device_; job.sm_count = sm_count_;
     if (!generic_only && fast_supported(job)) {
         if (peers_attached_ && !profiling_ && m.rows <= kPushCapacity) {
             // held back: an allreduce of this output may follow and fuse with it (allreduceSumF32)
@@ -524,7 +526,7 @@ int Backend::matvecAdd(const Buffer &weights, const Matrix &m, const Buffer &inp
     job.count = 1; job.mode = ACT_NONE;
     job.seg[0] = {w, stride, (uint32_t)m.rows, out, m.rows};
     job.add0 = res;
-    job.serial = written(weights); job.partials = partials_; job.partials_floats = partials_floats_; job.counters = counters_; job.counters_len = counters_len_; job.sm_count = sm_count_;
+    job.serial = written(weights); job.partials = partials_; job.partials_floats = partials_floats_; job.counters = counters_; job.counters_len = counters_len_; job.status = status_device_; job.sm_count = sm_count_;
     if (!generic_only && fast_supported(job)) {
         if (int rc = chainOrLaunch(job)) return rc;
     } else {
@@ -560,7 +562,7 @@ int Backend::matvecRows(const Buffer &weights, const Matrix &m, const Buffer &in
     job.enc = m.encoding; job.layout = m.layout; job.columns = (uint32_t)m.columns; job.tokens = (uint32_t)tokens; job.in = in; job.in_stride = in_stride;
     job.count = 1; job.mode = ACT_NONE;
     job.seg[0] = {w, stride, (uint32_t)m.rows, out, out_stride};
-    job.serial = written(weights); job.partials = partials_; job.partials_floats = partials_floats_; job.counters = counters_; job.counters_len = counters_len_; job.sm_count = sm_count_;
+    job.serial = written(weights); job.partials = partials_; job.partials_floats = partials_floats_; job.counters = counters_; job.counters_len = counters_len_; job.status = status_device_; job.sm_count = sm_count_;
     if (!generic_only && fast_supported(job)) launches_ += launch_fast(stream_, job);
     else launches_ += launch_matmul_generic(stream_, m.encoding, m.layout, w, stride, (uint32_t)m.rows, (uint32_t)m.columns, in, false, in_stride, out, out_stride, (uint32_t)tokens);
     wrote(output);
@@ -591,7 +593,7 @@ int Backend::matmul(const Buffer &weights, const Matrix &m, const Buffer &input,
         // Up to 8 tokens in one pass of the weights; a few more in passes of 8.
         FastJob job{};
         job.enc = m.encoding; job.layout = m.layout; job.columns = (uint32_t)m.columns; job.count = 1; job.mode = ACT_NONE; job.in_stride = in_stride;
-        job.serial = written(weights); job.partials = partials_; job.partials_floats = partials_floats_; job.counters = counters_; job.counters_len = counters_len_; job.sm_count = sm_count_;
+        job.serial = written(weights); job.partials = partials_; job.partials_floats = partials_floats_; job.counters = counters_; job.counters_len = counters_len_; job.status = status_device_; job.sm_count = sm_count_;
         job.tokens = (uint32_t)(tokens < 8 ? tokens : 8);
         job.in = (const float *)in;
         job.seg[0] = {w, stride, (uint32_t)m.rows, out, out_stride};
@@ -611,7 +613,7 @@ int Backend::matmul(const Buffer &weights, const Matrix &m, const Buffer &input,
         PrefillJob pj{};
         pj.enc = m.encoding; pj.layout = m.layout; pj.w = w; pj.stride = stride; pj.rows = (uint32_t)m.rows; pj.columns = (uint32_t)m.columns;
         pj.tokens = (uint32_t)tokens; pj.padded_tokens = (uint32_t)padded; pj.out = out; pj.out_stride = out_stride;
-        pj.status = counters_ + counters_len_; pj.sm_count = sm_count_;
+        pj.status = status_device_; pj.sm_count = sm_count_;
         if (in_dtype == NU_BF16) {
             pj.in = in; pj.in_stride = in_stride;
         } else if (padded * m.columns * 2 <= partials_floats_ * sizeof(float)) {
@@ -644,7 +646,7 @@ int Backend::segmentsJob(const Segment *segments, size_t count, const Buffer &in
     FastJob job{};
     job.enc = segments[0].matrix.encoding; job.layout = segments[0].matrix.layout; job.columns = (uint32_t)columns; job.tokens = 1; job.in = in; job.in_stride = columns;
     job.count = (uint32_t)count; job.mode = mode == NU_SEGMENTS_PLAIN ? ACT_NONE : (mode == NU_SEGMENTS_SILU_MUL_PAIR ? ACT_SILU : ACT_GELU);
-    for (size_t i = 0; i < count; ++i) job.serial = job.serial || written(segments[i].weights); job.partials = partials_; job.partials_floats = partials_floats_; job.counters = counters_; job.counters_len = counters_len_; job.sm_count = sm_count_;
+    for (size_t i = 0; i < count; ++i) job.serial = job.serial || written(segments[i].weights); job.partials = partials_; job.partials_floats = partials_floats_; job.counters = counters_; job.counters_len = counters_len_; job.status = status_device_; job.sm_count = sm_count_;
     bool same_encoding = true;
     uint64_t total_rows = 0;
     for (size_t i = 0; i < count; ++i) {
@@ -849,7 +851,7 @@ int Backend::kvJob(const char *who, const Buffer &buffer, const nu_kv_cache &c, 
     *span_ptr = resolve(spans, sequences * sizeof(nu_kv_span));
     if (!base || !*span_ptr) return fail(NU_ERR_INVALID_SHAPE, (name + ": cache or spans buffer too short").c_str());
     if (buffer.offset % 16 || spans.offset % 16) return fail(NU_ERR_INVALID_SHAPE, (name + ": cache and spans lie on 16-byte boundaries").c_str());
-    *job = {base, c.key_encoding == NU_Q8_0, c.value_encoding == NU_Q8_0, (uint32_t)c.slots, (uint32_t)c.capacity, (uint32_t)c.heads, (uint32_t)c.width, counters_ + counters_len_};
+    *job = {base, c.key_encoding == NU_Q8_0, c.value_encoding == NU_Q8_0, (uint32_t)c.slots, (uint32_t)c.capacity, (uint32_t)c.heads, (uint32_t)c.width, status_device_};
     return NU_OK;
 }
 
@@ -1079,7 +1081,7 @@ int Backend::matmulExperts(const Buffer &weights, const ExpertMatrix &t, const B
     if (!generic_only && n >= 2 * t.experts && fits_u32(n))
         launched = launch_matmul_experts_fast(stream_, t.encoding, w, stride, per_expert, (uint32_t)t.experts, (uint32_t)t.rows, (uint32_t)t.columns, l, (uint32_t)bound,
                                               (uint32_t)n, in, in_stride, (uint32_t)in_group, out, out_stride, partials_, partials_floats_ * sizeof(float),
-                                              counters_ + counters_len_);
+                                              status_device_);
     if (!launched)
         launched = launch_matmul_experts_generic(stream_, t.encoding, w, stride, per_expert, (uint32_t)t.experts, (uint32_t)t.rows, (uint32_t)t.columns, l,
                                                  (uint32_t)bound, in, in_stride, (uint32_t)in_group, out, out_stride);
@@ -1261,7 +1263,7 @@ int Backend::allreduceSumF32(const Buffer &buffer, size_t count, const Buffer *a
         pp.buf = p; pp.count = (uint32_t)count; pp.ranks = (uint32_t)peer_ranks_; pp.rank = (uint32_t)peer_rank_; pp.capacity = (uint32_t)kPushCapacity;
         for (int r = 0; r < peer_ranks_; ++r) pp.inbox[r] = (uint2 *)peer_base_[r];
         pp.seq = (uint32_t *)(inbox_ + kPushWordBytes);
-        pp.status = counters_ + counters_len_;
+        pp.status = status_device_;
         pp.wait_ns = peer_wait_ns_;
         pp.add_to = res;
         if (fuse) {

@@ -158,7 +158,7 @@ private:
     uint32_t *counters_ = nullptr;
     float *argmax_records_ = nullptr;  // 128 x (value, index, non-finite) of the argmax blocks, then their arrival counter
     size_t counters_len_ = 0;
-    uint32_t *status_host_ = nullptr;  // pinned: where the status word is read to
+    uint32_t *status_host_ = nullptr, *status_device_ = nullptr;  // the status word, in host memory, and where the kernels see it
     // per-operator profile
     bool profiling_ = false;
     uint32_t profile_max_ = 0;

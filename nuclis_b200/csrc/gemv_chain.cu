@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) chain_kernel(const __grid_co
                 there = ld_acquire_u32(link.arrivals) >= link.target;
                 if (!there) __nanosleep(64);
             }
-            if (!there) atomicExch(o.p.status, 1u);
+            if (!there) *(volatile uint32_t *)o.p.status = 1u;
         }
     }
     // the last block to leave puts the counters back to zero for the next launch

@@ -339,7 +339,7 @@ __device__ __forceinline__ void run_op(const Params &p, const Params &pm, const 
                 there = ld_acquire_u32(link.arrivals) >= link.target;
                 if (!there) __nanosleep(64);
             }
-            if (!there) atomicExch(p.status, 1u);
+            if (!there) *(volatile uint32_t *)p.status = 1u;
         }
         named_barrier(15, G::THREADS);
     } else {
@@ -684,7 +684,7 @@ __device__ __forceinline__ void run_op(const Params &p, const Params &pm, const 
         }
     }
     if (__any_sync(0xffffffffu, failed || stuck)) {
-        if (lane == 0) atomicExch(p.status, 1u);
+        if (lane == 0) *(volatile uint32_t *)p.status = 1u;
         // the slot's first warp lets the copies still in flight land before the block's shared memory is released
         if (part == 0)
             for (; consumed < issued; ++consumed) {
@@ -824,7 +824,7 @@ static bool fill_geometry(const FastJob &job, Params &p, Plan &plan) {
     plan.smem = smem_bytes<E, G, NT>(p.ksl, pair, plan.stages);
     p.partials = job.partials;
     p.counters = job.counters;
-    p.status = job.counters + job.counters_len;
+    p.status = job.status ? job.status : job.counters + job.counters_len;
     p.push = job.push;
     if (p.push.ranks && (job.mode != ACT_NONE || job.count != 1 || job.tokens != 1)) return false;  // one plain matrix, one token only
     p.norm_weight = job.norm_weight;

@@ -93,6 +93,7 @@ struct FastJob {
     size_t partials_floats;
     uint32_t *counters;
     size_t counters_len;
+    uint32_t *status;  // the word a kernel whose bounded wait ran out raises; null: counters[counters_len]
     int sm_count;
     bool serial;  // a weights buffer was written earlier in the same recording: no early start of the weight stream
     PushTarget push;

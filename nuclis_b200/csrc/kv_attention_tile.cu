@@ -3,10 +3,10 @@
 // One block a multiprocessor walks its share of all (sequence, row tile, head) units, as the kernel for few rows does
 // (kv_attention.cu), in steps of 128 keys (64 at width 256). A unit's row tile is 256 query rows, two M = 128 tiles that share every key
 // step (one tile at width 256, whose accumulator alone takes half the tensor memory).
-//   * warps 8..11 decode: a step's keys and values become f16 in shared memory, in the 128-byte-swizzled K-major layout of
+//   * warps 8..15 decode: a step's keys and values become f16 in shared memory, in the 128-byte-swizzled K-major layout of
 //     the tensor core: keys as rows of dimensions, values transposed as rows of positions. The dimensions of a key's eight
 //     stand in the order 0,4,1,5,2,6,3,7 that unpacking gives, and the queries are laid out alike.
-//   * warp 12 (one thread) issues S = Q K^T and O += P V, in an order that keeps one tile's softmax under the other's products.
+//   * warp 16 issues S = Q K^T and O += P V, in an order that keeps one tile's softmax under the other's products.
 //   * warps 0..7 are the softmax: a thread has a row; it reads S from tensor memory, writes P = 2^(S scale - m) as f16 over it, and
 //     the tensor core takes P from there. The maximum m is only moved when a score passes it by 8 (log2), so O is rarely rescaled.
 //
@@ -36,11 +36,11 @@ struct Tile {
     static constexpr int KT = W == 256 ? 64 : 128; // keys of a step
     static constexpr int NB = W / 32;
     static constexpr KvLayout L = kv_layout(W, K8, V8);
-    static constexpr int SOFT = 8, PROD = 4, THREADS = (SOFT + PROD + 4) * 32;  // + the warpgroup of the warp that issues
-    // Registers a thread, of the 128 x 512 that the block starts with: the softmax keeps its 128, the issuing warpgroup gives to the decoding one
-    static constexpr int PROD_REGS = 168, MMA_REGS = 88;
-    static_assert(SOFT * 128 + PROD * PROD_REGS + 4 * MMA_REGS <= 16 * 128, "more registers than the block has");
-    static constexpr int PARTS = 128 / KT;         // decoding threads of a key
+    static constexpr int SOFT = 8, PROD = 8, THREADS = (SOFT + PROD + 4) * 32;  // + the warpgroup of the warp that issues
+    // Registers a thread, of the 96 x 640 that the block starts with
+    static constexpr int SOFT_REGS = 136, PROD_REGS = 80, MMA_REGS = 48;
+    static_assert(SOFT * SOFT_REGS + PROD * PROD_REGS + 4 * MMA_REGS <= (SOFT + PROD + 4) * 96, "more registers than the block has");
+    static constexpr int PARTS = 128 / KT;         // of the 128 threads that rate the scales, a key's
     static constexpr int NBT = NB / PARTS;         // a key's blocks of a thread
     // shared memory
     static constexpr int Q_TILE = 128 * W * 2, Q = 0, K_BYTES = KT * W * 2, K = Q + QT * Q_TILE, V = K + 2 * K_BYTES, TABLE = V + 2 * K_BYTES;
@@ -133,6 +133,12 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t *v) {
           "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
         : "r"(addr));
 }
+__device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t (&v)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]),
+                   "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                 : "r"(addr));
+}
 __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&v)[32]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -142,9 +148,9 @@ __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&v)[
         "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
         : "memory");
 }
-__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&v)[16]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]),
-                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+__device__ __forceinline__ void tmem_store8(uint32_t addr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]),
+                 "r"(v[7])
                  : "memory");
 }
 __device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -154,7 +160,7 @@ __device__ __forceinline__ void named_barrier() { asm volatile("bar.sync %0, %1;
 // A barrier of the decoding warps that returns whether any of their threads says yes.
 __device__ __forceinline__ bool barrier_or(bool mine) {
     uint32_t any;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(any) : "r"((uint32_t)mine) : "memory");
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 2, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(any) : "r"((uint32_t)mine) : "memory");
     return any != 0;
 }
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
@@ -230,6 +236,7 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
     Segment sg;
 
     if (warp < T::SOFT) {
+        more_registers<T::SOFT_REGS>();
         // ---- softmax: thread = row `row` of M tile `q` (width 256: columns `half` of the only tile) ----
         const uint32_t group = warp / 4, q = QT == 2 ? group : 0, row = warp % 4 * 32 + lane;
         const uint32_t lanes = (warp % 4 * 32) << 16;
@@ -339,7 +346,7 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                 for (int k = 0; k < CHUNKS; ++k) {
                     uint32_t (&x)[32] = v[k % QT];
                     tmem_load_wait();
-                    if (QT == 2) tmem_load32(sfirst + (k + 1) % CHUNKS * 32, v[(k + 1) % QT]);
+                    if (QT == 2 && k + 1 < CHUNKS) tmem_load32(sfirst + (k + 1) * 32, v[(k + 1) % QT]);
                     if (edge) hide(x, k * 32);
 #pragma unroll
                     for (int c = 0; c < 32; c += 8)
@@ -382,40 +389,67 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                 const float offset = (float)shift - (m == -INFINITY ? 0.0f : m);
                 const uint64_t factor2 = two(factor, factor), offset2 = two(offset, offset);
                 uint64_t sums[4] = {0, 0, 0, 0};
+                // In pieces of 16 columns: one arrives, the next one's powers are taken, the one before is summed, packed and stored between
+                // them (the unit of the powers takes 8 cycles an instruction). P lies over S: half as wide, over columns that have been read.
+                constexpr int PIECES = COLS / 16;
+                uint32_t y[3][16], pk[8];
+                auto raise = [&](uint32_t (&x)[16], int pair) {
+                    asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+r"(x[2 * pair]));
+                    asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+r"(x[2 * pair + 1]));
+                };
+                auto gather = [&](const uint32_t (&x)[16], int pair) {
+                    sums[pair % 4] = add2(sums[pair % 4], (uint64_t)x[2 * pair] | (uint64_t)x[2 * pair + 1] << 32);
+                    pk[pair] = h2(__floats2half2_rn(__uint_as_float(x[2 * pair]), __uint_as_float(x[2 * pair + 1])));
+                };
+                const uint32_t pfirst = scol + (QT == 1 ? group * COLS : 0) / 2;
+                if (QT == 2) {
+                    tmem_load16(sfirst, y[0]);
+                    tmem_load_wait();
+                } else {
 #pragma unroll
-                for (int k = 0; k < CHUNKS; ++k) {
-                    uint32_t (&x)[32] = v[k % QT];
-                    if (QT == 2) {
-                        tmem_load_wait();
-                        if (k + 1 < CHUNKS) tmem_load32(sfirst + (k + 1) * 32, v[(k + 1) % QT]);
-                        if (edge) hide(x, k * 32);
+                    for (int c = 0; c < 16; ++c) { y[0][c] = v[0][c]; y[1][c] = v[0][16 + c]; }
+                }
+#pragma unroll
+                for (int k = 0; k < PIECES; ++k) {
+                    uint32_t (&x)[16] = y[k % 3];
+                    if (QT == 2 && k + 1 < PIECES) tmem_load16(sfirst + (k + 1) * 16, y[(k + 1) % 3]);
+                    if (QT == 2 && edge) {
+#pragma unroll
+                        for (int c = 0; c < 16; ++c)
+                            if (c > to - k * 16 || c < from - k * 16) x[c] = 0xff800000u;
                     }
-                    uint32_t pk[16];
 #pragma unroll
-                    for (int c = 0; c < 32; c += 2) {
+                    for (int c = 0; c < 16; c += 2) {
                         const uint64_t z = fma2((uint64_t)x[c] | (uint64_t)x[c + 1] << 32, factor2, offset2);
                         x[c] = (uint32_t)z;
                         x[c + 1] = (uint32_t)(z >> 32);
                     }
-                    // all of a chunk's powers ahead of their first use: the unit that makes them takes 8 cycles a warp and answers after some 20
 #pragma unroll
-                    for (int c = 0; c < 32; ++c) asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+r"(x[c]));
-#pragma unroll
-                    for (int c = 0; c < 32; c += 2) {
-                        sums[c / 2 % 4] = add2(sums[c / 2 % 4], (uint64_t)x[c] | (uint64_t)x[c + 1] << 32);
-                        pk[c / 2] = h2(__floats2half2_rn(__uint_as_float(x[c]), __uint_as_float(x[c + 1])));
+                    for (int c = 0; c < 8; ++c) {
+                        raise(x, c);
+                        if (k > 0) gather(y[(k + 2) % 3], c);
                     }
-                    // over S: half as wide, so over columns that have been read
-                    tmem_store16(scol + ((QT == 1 ? group * COLS : 0) + k * 32) / 2, pk);
-                    if (any_nan[ring]) {  // the blocks that are NaN at a position this row has weight on
+                    if (k > 0) tmem_store8(pfirst + (k - 1) * 8, pk);
+                    if (QT == 2 && k + 1 < PIECES) tmem_load_wait();
+                }
+#pragma unroll
+                for (int c = 0; c < 8; ++c) gather(y[(PIECES - 1) % 3], c);
+                tmem_store8(pfirst + (PIECES - 1) * 8, pk);
+                sums[0] = add2(add2(sums[0], sums[1]), add2(sums[2], sums[3]));
+                const float sum = low_of(sums[0]) + high_of(sums[0]);
+                if (any_nan[ring]) {  // the blocks that are NaN at a position this row has weight on: P once more
+                    tmem_store_wait();
+#pragma unroll 1
+                    for (int k = 0; k < COLS / 32; ++k) {
+                        uint32_t q16[16];
+                        tmem_load16(pfirst + k * 16, q16);
+                        tmem_load_wait();
                         const uint32_t k0 = (QT == 1 ? group * COLS : 0) + k * 32;
 #pragma unroll
                         for (int c = 0; c < 32; ++c)
-                            if (pk[c / 2] >> (c % 2 * 16) & 0xffffu) nan_blocks |= nans[ring * 256 + k0 + c] | nans[ring * 256 + 128 + k0 + c];
+                            if (q16[c / 2] >> (c % 2 * 16) & 0xffffu) nan_blocks |= nans[ring * 256 + k0 + c] | nans[ring * 256 + 128 + k0 + c];
                     }
                 }
-                sums[0] = add2(add2(sums[0], sums[1]), add2(sums[2], sums[3]));
-                const float sum = low_of(sums[0]) + high_of(sums[0]);
                 l += sum * power_of_two(-shift);
                 tmem_store_wait();
                 if (!waited) wait_or_give_up(bar(PV_DONE + q), (step - 1) & 1u, abort_flag);
@@ -526,16 +560,20 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
         }
         fence_before();
     } else if (warp < T::SOFT + T::PROD) {
-        more_registers<T::PROD_REGS>();
-        // ---- decoding: a warp has KT / 64 granules of a step. Keys: lane (g, t) its own vectors of a tile of eight; values: lane (half, words w,
-        // g) the four lanes' words of two neighbouring words, which are eight positions each of a dimension and (Q4_0) the one eight on ----
+        fewer_registers<T::PROD_REGS>();
+        // ---- decoding: a warp has one granule of a step of 128 keys, half a granule of one of 64. Keys: lane (g, t) its own vectors of a tile of
+        // eight; values: lane (half, words w, g) the four lanes' words of two neighbouring words, which are eight positions each of a dimension
+        // and (Q4_0) the one eight on. The first four warps' threads (key, part) rate the scales ----
         const uint32_t t = tid - T::SOFT * 32, key = t % KT, part = t / KT, pw = warp - T::SOFT, g8 = lane / 4, t4 = lane % 4;
-        constexpr int GRANULES = KT / 64;                                      // of a warp
-        constexpr int KVEC = L.k_vec, KWORDS = KVEC / 4;                       // words of a vector
-        constexpr int KVECS = (K8 ? 2 : 1) * NB / KWORDS, KITEMS = 2 * GRANULES * KVECS;  // vectors of a tile of eight keys; of a warp in a step
-        constexpr int VVECS = W / (V8 ? 8 : 16) / 4, VITEMS = GRANULES * VVECS / 2;       // vectors of a granule; a half warp's in a step
+        const bool rater = t < 128;
+        constexpr int TILES = KT / 64;                                          // of eight keys, of a warp
+        constexpr int KVEC = L.k_vec, KWORDS = KVEC / 4;                        // words of a vector
+        constexpr int KVECS = (K8 ? 2 : 1) * NB / KWORDS, KITEMS = TILES * KVECS;  // vectors of a tile; of a warp in a step
+        constexpr int VVECS = W / (V8 ? 8 : 16) / 4;                            // vectors of a granule
+        constexpr int VTURN = 4 / TILES, VITEMS = VVECS < VTURN ? 1 : VVECS / VTURN;  // a half warp has every VTURN-th of them
         const uint32_t half = lane / 16, vpair = lane / 8 % 2, vg = lane % 8;
-        const uint32_t vgran = GRANULES == 2 ? half : 0, vskip = GRANULES == 2 ? 0 : half, vturn = GRANULES == 2 ? 1 : 2;  // vector i * vturn + vskip of granule vgran
+        const uint32_t wgran = TILES == 2 ? pw : pw / 2, v0 = TILES == 2 ? half : pw % 2 * 2 + half;
+        const bool valued = VVECS >= VTURN || v0 < (uint32_t)VVECS;             // (one vector a granule: half a warp)
         uint32_t step = 0;
         while (walk.next(p, pl, sg)) {
             const uint32_t live_rows = sg.span.count * p.group;
@@ -546,6 +584,7 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
             const uint32_t last_granule = high / KV_GRANULE;  // what is behind it may lie past the slot's end: it is not read
             uint32_t kw[KITEMS][KWORDS], vw[VITEMS][4][2], ks[T::NBT / 2], vs[T::NBT / 2];
             auto load_scales = [&](uint32_t key0) {
+                if (!rater) return;
                 const uint32_t at = key0 + key;
                 const uint8_t *g = base + (size_t)(at / KV_GRANULE) * L.bytes + (at % KV_GRANULE * NB + part * T::NBT) * 2;
                 const bool in = at / KV_GRANULE <= last_granule;
@@ -556,30 +595,30 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                 }
             };
             auto load_keys = [&](uint32_t key0) {
-                const uint32_t gran = key0 / KV_GRANULE + pw * GRANULES;
-                const uint8_t *g = base + (size_t)gran * L.bytes + lane * KVEC;
+                const uint32_t gran = key0 / KV_GRANULE + wgran;
+                const bool in = gran <= last_granule;
+                const uint8_t *g = base + (size_t)gran * L.bytes + (TILES == 2 ? 0 : pw % 2 * (L.k_scales / 2)) + lane * KVEC;
 #pragma unroll
                 for (int i = 0; i < KITEMS; ++i) {
-                    const int tile = i / KVECS, v = i % KVECS;
-                    const uint8_t *src = g + tile / 2 * L.bytes + tile % 2 * (L.k_scales / 2) + v * 32 * KVEC;
+                    const uint8_t *src = g + i / KVECS * (L.k_scales / 2) + i % KVECS * 32 * KVEC;
                     if (KVEC == 16) {
-                        const uint4 x = gran + tile / 2 <= last_granule ? __ldg((const uint4 *)src) : make_uint4(0u, 0u, 0u, 0u);
+                        const uint4 x = in ? __ldg((const uint4 *)src) : make_uint4(0u, 0u, 0u, 0u);
                         kw[i][0] = x.x; kw[i][1] = x.y; kw[i][KWORDS - 2] = x.z; kw[i][KWORDS - 1] = x.w;
                     } else {
-                        const uint2 x = gran + tile / 2 <= last_granule ? __ldg((const uint2 *)src) : make_uint2(0u, 0u);
+                        const uint2 x = in ? __ldg((const uint2 *)src) : make_uint2(0u, 0u);
                         kw[i][0] = x.x; kw[i][1] = x.y;
                     }
                 }
             };
             auto load_values = [&](uint32_t key0) {
-                const uint32_t gran = key0 / KV_GRANULE + pw * GRANULES + vgran;
-                const bool in = gran <= last_granule;
-                const uint8_t *g = base + (size_t)gran * L.bytes + L.v_codes + vskip * 512 + vg * 64 + vpair * 8;
+                const uint32_t gran = key0 / KV_GRANULE + wgran;
+                const bool in = gran <= last_granule && valued;
+                const uint8_t *g = base + (size_t)gran * L.bytes + L.v_codes + v0 * 512 + vg * 64 + vpair * 8;
 #pragma unroll
                 for (int i = 0; i < VITEMS; ++i)
 #pragma unroll
                     for (int tt = 0; tt < 4; ++tt) {
-                        const uint2 x = in ? __ldg((const uint2 *)(g + i * vturn * 512 + tt * 16)) : make_uint2(0u, 0u);
+                        const uint2 x = in ? __ldg((const uint2 *)(g + i * VTURN * 512 + tt * 16)) : make_uint2(0u, 0u);
                         vw[i][tt][0] = x.x; vw[i][tt][1] = x.y;
                     }
             };
@@ -588,6 +627,7 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
             uint32_t nan_mask = 0;
             // the scales of the step at key0 (global step `of`): what no row of the tile sees counts as zero; the largest of all sets the step's power of two
             auto rate = [&](uint32_t key0, uint32_t of) {
+                if (!rater) return;
                 const bool seen = key0 + key >= low && key0 + key <= high;
                 float kmax = 0.0f, vmax = 0.0f;
                 nan_mask = 0;
@@ -612,6 +652,7 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
             };
             // behind the barrier that follows: the powers of two, and the scales times them
             auto publish = [&](uint32_t of, bool nan) {
+                if (!rater) return;
                 const uint32_t ring = of & 3u;
                 const int xk = (int)max(largest[ring * 2] >> 23, 64u) - 127, xv = (int)max(largest[ring * 2 + 1] >> 23, 64u) - 127;
                 const float fk = power_of_two(14 - xk), fv = power_of_two(14 - xv);  // the largest scale to [2^14, 2^15)
@@ -637,7 +678,7 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
             load_values(begin);
             rate(begin, step);
             publish(step, barrier_or(nan_mask != 0));
-            named_barrier<2, 128>();
+            named_barrier<2, 256>();
             for (uint32_t i = 0; i < sg.n; ++i, ++step) {
                 const uint32_t key0 = begin + i * KT, stage = step & 1u, parity = (step >> 1) & 1u;
                 const bool more = i + 1 < sg.n;
@@ -647,7 +688,7 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                 uint8_t *kt = smem + T::K + stage * T::K_BYTES;
 #pragma unroll
                 for (int j = 0; j < KITEMS; ++j) {
-                    const uint32_t row = pw * (KT / 4) + j / KVECS * 8 + g8, v = j % KVECS;
+                    const uint32_t row = pw * (KT / 8) + j / KVECS * 8 + g8, v = j % KVECS;
                     constexpr int BLOCKS = KWORDS / (K8 ? 2 : 1);
                     const uint32_t b0 = v * BLOCKS;
                     uint32_t pairs[BLOCKS / 2];
@@ -688,7 +729,8 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                 uint8_t *vt = smem + T::V + stage * T::K_BYTES;
 #pragma unroll
                 for (int j = 0; j < VITEMS; ++j) {
-                    const uint32_t v = j * vturn + vskip, gran = pw * GRANULES + vgran, word = v * 4 + vpair * 2, block = word / (V8 ? 4 : 2);
+                    if (!valued) break;
+                    const uint32_t v = j * VTURN + v0, gran = wgran, word = v * 4 + vpair * 2, block = word / (V8 ? 4 : 2);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {  // eight positions of the granule: 2t, 2t + 1 of every t
                         const uint4 d4 = *(const uint4 *)(value_scales + (stage * NB + block) * KT + gran * 16 + h * 8);
@@ -719,7 +761,7 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                 if (more) {
                     load_values(key0 + KT);
                     publish(step + 1, nan);
-                    named_barrier<2, 128>();  // the next step's scales are there
+                    named_barrier<2, 256>();  // the next step's scales are there
                 }
             }
         }

@@ -724,7 +724,7 @@ __global__ void __launch_bounds__(THREADS, BPS) prefill_kernel(const __grid_cons
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)BN) : "memory");
     }
-    if (tid == 0 && *abort_flag) atomicExch(p.status, 1u);
+    if (tid == 0 && *abort_flag) *(volatile uint32_t *)p.status = 1u;
 }
 
 template <int BN, int STAGES> constexpr int smem_bytes() { return STAGES * (BM * BK * 2 + BN * BK * 2) + (3 * STAGES + 1) * 8 + 16 + 1024; }
