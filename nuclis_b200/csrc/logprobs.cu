@@ -4,10 +4,10 @@
 //     m = max_i x_i,  Z = sum_i e^(x_i - m),  log p_t = (x_t - m) - ln Z,  H = ln Z - (sum_i (x_i - m) e^(x_i - m)) / Z
 //
 // Every thread keeps (m, Z, sum) of its share online, raising m once per batch of 16 values. The alternatives are kept
-// by the block: after the first round of 16 values a thread, the k-th largest of the threads' maxima bounds the k-th largest
-// value from below, so only the few values above it become candidates (64-bit keys: the value's order, then the lower
-// index), and later rounds only look at values above the k-th candidate kept. A row is cut over several blocks when there
-// are few rows; the block that arrives last joins them in block order.
+// by each warp on its own, so that no barrier stands in the loop: after its first 512 values the k-th largest of the lanes' maxima
+// bounds the k-th largest value from below, so only the few values above it become candidates (64-bit keys: the
+// value's order, then the lower index), and later only what passes the k-th candidate kept; the candidates are cut back to k when
+// eight more have come (each cut raises the bar, and what passes it costs the whole warp a look at its values). A row is cut over several blocks when there are few rows; the block that arrives last joins them in block order.
 #include "kernels.hpp"
 #include "launch.cuh"
 
@@ -15,9 +15,11 @@ namespace nu {
 
 namespace {
 
-constexpr int THREADS = 256, WARPS = THREADS / 32, EACH = 16, ROUND = THREADS * EACH;
 constexpr int MAX_K = (int)LOGPROB_ALTERNATIVES;
-constexpr int CANDIDATES = ROUND + MAX_K;
+constexpr int THREADS = 256, WARPS = THREADS / 32, EACH = 16, ROUND = THREADS * EACH;
+constexpr int RESIDENT = 4;                 // blocks a multiprocessor: 64 registers a thread, for two rounds of values
+constexpr int WARP_ROUND = 32 * EACH, CUT = 8, WARP_CANDIDATES = WARP_ROUND + MAX_K + CUT;  // a round on top of what is not yet cut back
+constexpr int CANDIDATES = WARPS * WARP_CANDIDATES;
 constexpr uint32_t SPLITS_MAX = 256;
 constexpr int FEW = 256;                    // candidates that are ranked by counting
 constexpr int RECORD = 4 + 2 * MAX_K;       // floats a block leaves: m, Z, sum, bad, then the keys
@@ -45,23 +47,13 @@ struct Stats {
         }
         m = next;
     }
-    __device__ __forceinline__ void join(const Stats &o) {
-        bad |= o.bad;
-        if (o.m > m) raise(o.m);
-        if (o.z > 0.0f) {
-            const float d = o.m - m, f = expf(d);
-            if (f > 0.0f) {
-                z += o.z * f;
-                w += (o.w + d * o.z) * f;
-            }
-        }
-    }
 };
 
 struct Shared {
     unsigned long long candidates[CANDIDATES];
     unsigned long long kept[MAX_K];
     unsigned long long best[WARPS];
+    uint32_t counts[WARPS];
     uint32_t maxima[THREADS];
     Stats stats[WARPS];
     uint32_t count, bound, last;
@@ -73,16 +65,52 @@ __device__ __forceinline__ unsigned long long warp_max(unsigned long long v) {
     return (unsigned long long)high << 32 | low;
 }
 
+// The k largest of a warp's candidates c[0..n), n >= k, to the front in falling order. One warp.
+__device__ __forceinline__ void cut_back(unsigned long long *c, uint32_t n, uint32_t k) {
+    const uint32_t lane = threadIdx.x & 31;
+    if (n <= 64) {  // by counting what is larger
+        const unsigned long long x = lane < n ? c[lane] : 0, y = lane + 32 < n ? c[lane + 32] : 0;
+        uint32_t above_x = 0, above_y = 0;
+#pragma unroll 8
+        for (uint32_t i = 0; i < n; ++i) {
+            const unsigned long long z = c[i];
+            above_x += z > x;
+            above_y += z > y;
+        }
+        __syncwarp();
+        if (x && above_x < k) c[above_x] = x;
+        if (y && above_y < k) c[above_y] = y;
+        __syncwarp();
+        return;
+    }
+    unsigned long long mine = 0, kept = 0;
+    for (uint32_t i = lane; i < n; i += 32) mine = max(mine, c[i]);
+    for (uint32_t r = 0; r < k; ++r) {
+        const unsigned long long top = warp_max(mine);
+        if (lane == r) kept = top;
+        if (mine == top) {  // keys are distinct: one lane
+            unsigned long long next = 0;
+            for (uint32_t i = lane; i < n; i += 32)
+                if (c[i] < top) next = max(next, c[i]);
+            mine = next;
+        }
+    }
+    __syncwarp();
+    if (lane < k) c[lane] = kept;
+    __syncwarp();
+}
+
 // The k largest of sh.candidates[0..n) into sh.kept, in falling order; zero where there are fewer. All threads; n is uniform.
 __device__ __forceinline__ void select(Shared &sh, uint32_t n, uint32_t k) {
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
     if (n <= FEW) {
         const unsigned long long mine = tid < n ? sh.candidates[tid] : 0;
         uint32_t above = 0;
+#pragma unroll 8
         for (uint32_t i = 0; i < n; ++i) above += sh.candidates[i] > mine;
+        if (tid < k) sh.kept[tid] = 0;
         __syncthreads();
-        if (tid < n && above < k) sh.kept[above] = mine;
-        if (tid >= n && tid < k) sh.kept[tid] = 0;
+        if (mine && above < k) sh.kept[above] = mine;
         __syncthreads();
         return;
     }
@@ -106,22 +134,25 @@ __device__ __forceinline__ void select(Shared &sh, uint32_t n, uint32_t k) {
     }
 }
 
+// The block's, in every thread: the largest m of all first, so that each part is scaled once.
 __device__ __forceinline__ Stats block_stats(Shared &sh, Stats s) {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+    auto all = [&](Stats x, float m) {  // x brought to the maximum m, summed over the warp
+        const uint32_t bad = __reduce_or_sync(0xffffffffu, x.bad);
+        const float d = x.m - m, f = x.z > 0.0f ? expf(d) : 0.0f;
+        float w = f > 0.0f ? (x.w + d * x.z) * f : 0.0f, z = f > 0.0f ? x.z * f : 0.0f;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        Stats x;
-        x.m = __shfl_xor_sync(0xffffffffu, s.m, o);
-        x.z = __shfl_xor_sync(0xffffffffu, s.z, o);
-        x.w = __shfl_xor_sync(0xffffffffu, s.w, o);
-        x.bad = __shfl_xor_sync(0xffffffffu, s.bad, o);
-        s.join(x);
-    }
+        for (int o = 16; o; o >>= 1) {
+            z += __shfl_xor_sync(0xffffffffu, z, o);
+            w += __shfl_xor_sync(0xffffffffu, w, o);
+        }
+        return Stats{m, z, w, bad};
+    };
+    s = all(s, unorder(__reduce_max_sync(0xffffffffu, order(s.m))));
     if (lane == 0) sh.stats[warp] = s;
     __syncthreads();
-    s = sh.stats[0];
-    for (int i = 1; i < WARPS; ++i) s.join(sh.stats[i]);
-    return s;
+    s = lane < WARPS ? sh.stats[lane] : Stats{-INFINITY, 0.0f, 0.0f, 0u};
+    return all(s, unorder(__reduce_max_sync(0xffffffffu, order(s.m))));
 }
 
 __device__ __forceinline__ void write_row(const LogprobJob &j, const Shared &sh, const Stats &s, uint32_t row) {
@@ -141,7 +172,7 @@ __device__ __forceinline__ void write_row(const LogprobJob &j, const Shared &sh,
     }
 }
 
-__global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(THREADS, RESIDENT) token_logprobs_kernel(const __grid_constant__ Params p) {
     extern __shared__ __align__(16) uint8_t raw[];
     Shared &sh = *(Shared *)raw;
     const LogprobJob &j = p.j;
@@ -152,27 +183,35 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const __grid_co
     const uint32_t ahead = (uint32_t)((16 - ((uintptr_t)x & 15)) & 15) / 4;
     const uint32_t begin = split == 0 ? 0 : min(j.count, ahead + split * p.piece), end = split + 1 == p.splits ? j.count : min(j.count, ahead + (split + 1) * p.piece);
     const uint32_t shift = split == 0 ? (4 - ahead) % 4 : 0;  // values of the first vector that lie before the row
-    if (tid == 0) sh.count = 0;
-    if (tid < MAX_K) sh.kept[tid] = 0;
-    __syncthreads();
+    const uint32_t lane = tid & 31, warp = tid / 32;
+    unsigned long long *own = sh.candidates + warp * WARP_CANDIDATES;
+    if (lane == 0) sh.counts[warp] = 0;
+    __syncwarp();
 
     Stats s{-INFINITY, 0.0f, 0.0f, 0u};
-    uint32_t floor = 0;      // order of the k-th value kept: later equals have higher indexes and lose
-    const long long n = (long long)end - begin + shift;  // of the piece, from the vector that holds its first value
+    uint32_t floor = 0;      // order of the k-th value this warp has kept: later equals have higher indexes and lose
+    const int n = (int)(end - begin + shift);  // of the piece, from the vector that holds its first value
     const float *v = x + begin - shift;
-    for (long long r0 = 0; r0 < n; r0 += ROUND) {
-        float a[EACH];
+    auto load = [&](float (&to)[EACH], int r0) {
 #pragma unroll
         for (int q = 0; q < EACH / 4; ++q) {
-            const long long i = r0 + (q * THREADS + tid) * 4;
-            if (i >= (long long)shift && i + 4 <= n) {
+            const int i = r0 + (q * THREADS + (int)tid) * 4;
+            if (i >= (int)shift && i + 4 <= n) {
                 const float4 f = __ldcs((const float4 *)(v + i));
-                a[q * 4] = f.x; a[q * 4 + 1] = f.y; a[q * 4 + 2] = f.z; a[q * 4 + 3] = f.w;
+                to[q * 4] = f.x; to[q * 4 + 1] = f.y; to[q * 4 + 2] = f.z; to[q * 4 + 3] = f.w;
             } else {
 #pragma unroll
-                for (int c = 0; c < 4; ++c) a[q * 4 + c] = i + c >= (long long)shift && i + c < n ? v[i + c] : -INFINITY;
+                for (int c = 0; c < 4; ++c) to[q * 4 + c] = i + c >= (int)shift && i + c < n ? v[i + c] : -INFINITY;
             }
         }
+    };
+    float next[EACH];  // the round after is on its way while one is worked on
+    load(next, 0);
+    for (int r0 = 0; r0 < n; r0 += ROUND) {
+        float a[EACH];
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) a[i] = next[i];
+        if (r0 + ROUND < n) load(next, r0 + ROUND);
         float top = a[0];
         bool nan = false;
 #pragma unroll
@@ -190,38 +229,49 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const __grid_co
         }
         if (k == 0) continue;
         const uint32_t mine = order(top);
-        const int hopeful = __syncthreads_count(mine > floor);
+        const uint32_t hopeful = __ballot_sync(0xffffffffu, mine > floor);
         if (hopeful == 0) continue;
         uint32_t bound = floor;
-        if (hopeful > 64) {  // many: only what reaches the k-th largest of the threads' maxima can be among the k largest
-            sh.maxima[tid] = mine;
-            if (tid == 0) sh.bound = 0;
-            __syncthreads();
-            uint32_t above = 0;  // threads ahead of this one, equals by number
-            for (uint32_t i = 0; i < THREADS; ++i) above += sh.maxima[i] > mine || (sh.maxima[i] == mine && i < tid);
-            if (above == k - 1) sh.bound = mine;
-            __syncthreads();
-            bound = max(floor, sh.bound - 1);  // an order is never zero, minus infinity's neither
+        if (__popc(hopeful) >= (int)k) {  // only what reaches the k-th largest of the lanes' maxima can be among the k largest
+            uint32_t above = 0;  // lanes ahead of this one, equals by number
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                const uint32_t o = __shfl_sync(0xffffffffu, mine, i);
+                above += o > mine || (o == mine && i < (int)lane);
+            }
+            bound = max(floor, __reduce_max_sync(0xffffffffu, above == k - 1 ? mine - 1 : 0u));  // (an order is never zero)
         }
         if (mine > bound) {
 #pragma unroll
             for (int i = 0; i < EACH; ++i) {
-                const long long at = r0 + ((i / 4) * THREADS + tid) * 4 + i % 4;
+                const int at = r0 + ((i / 4) * THREADS + (int)tid) * 4 + i % 4;
                 const uint32_t o = order(a[i]);
-                if (o > bound && at >= (long long)shift && at < n) sh.candidates[atomicAdd(&sh.count, 1u)] = key_of(o, (uint32_t)(begin + at - shift));
+                if (o > bound && at >= (int)shift && at < n) own[atomicAdd(&sh.counts[warp], 1u)] = key_of(o, begin + (uint32_t)at - shift);
             }
         }
+        __syncwarp();
+        const uint32_t c = sh.counts[warp];
+        if (c >= k && (floor == 0 || c > k + CUT)) {
+            cut_back(own, c, k);
+            if (lane == 0) sh.counts[warp] = k;
+            floor = (uint32_t)(own[k - 1] >> 32);
+        }
+        __syncwarp();
+    }
+    if (k) {  // the warps' candidates together: what one has at most between cuts, or its k where that is too many to rank
+        const uint32_t each = WARPS * (k + CUT) <= (uint32_t)FEW ? k + CUT : k;
+        if (sh.counts[warp] > each) {
+            cut_back(own, sh.counts[warp], k);
+            if (lane == 0) sh.counts[warp] = k;
+            __syncwarp();
+        }
+        const uint32_t c = sh.counts[warp];
+        const unsigned long long key = lane < c ? own[lane] : 0, more = lane + 32 < c ? own[lane + 32] : 0;
         __syncthreads();
-        uint32_t c = sh.count;
+        if (lane < each) sh.candidates[warp * each + lane] = key;
+        if (lane + 32 < each) sh.candidates[warp * each + lane + 32] = more;
         __syncthreads();
-        // the ones kept so far join the new ones
-        if (tid < k && sh.kept[tid]) sh.candidates[atomicAdd(&sh.count, 1u)] = sh.kept[tid];
-        __syncthreads();
-        c = sh.count;
-        select(sh, c, k);
-        if (tid == 0) sh.count = 0;
-        floor = (uint32_t)(sh.kept[k - 1] >> 32);
-        __syncthreads();
+        select(sh, WARPS * each, k);
     }
     s = block_stats(sh, s);
     if (p.splits == 1) {
@@ -278,13 +328,18 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const __grid_co
 }  // namespace
 
 int launch_token_logprobs(cudaStream_t s, const LogprobJob &j) {
-    // As many blocks as keep the multiprocessors busy (four resident each), but never less than one round a block.
+    // Cuts of a row: the ones whose blocks fill whole waves best, a block's start and join counted as five rounds; never less than a
+    // round a block.
     Params p{j, 1, j.count};
-    const uint32_t want = ((uint32_t)j.sm_count * 4 + j.rows - 1) / j.rows, most = (j.count + ROUND - 1) / ROUND;
-    uint32_t splits = want < most ? want : most;
+    const uint32_t slots = (uint32_t)j.sm_count * RESIDENT, rounds = (j.count + ROUND - 1) / ROUND;
     const uint32_t join = CANDIDATES / (j.k ? j.k : 1);  // the joining block holds every piece's candidates
-    if (splits > SPLITS_MAX) splits = SPLITS_MAX;
-    if (splits > join) splits = join;
+    uint32_t most = rounds < SPLITS_MAX ? rounds : SPLITS_MAX, splits = 1;
+    if (most > join) most = join;
+    unsigned long long best = ~0ull;
+    for (uint32_t c = 1; c <= most; ++c) {
+        const unsigned long long waves = ((unsigned long long)j.rows * c + slots - 1) / slots, cost = waves * ((rounds + c - 1) / c + 5) + (c > 1);
+        if (cost < best) { best = cost; splits = c; }
+    }
     if (splits > 1 && j.rows <= j.counters_len && (size_t)j.rows * splits * RECORD <= j.partials_floats) {
         p.piece = ((j.count + splits - 1) / splits + 3) / 4 * 4;
         p.splits = (j.count + p.piece - 1) / p.piece;
