@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
     __syncwarp();
     wait_for_previous_operator();
 
-    const Plan pl = plan<ROWS, KV_GRANULE, S::SEGMENT>(p);
+    const Plan pl = plan<ROWS, KV_GRANULE, S::SEGMENT, WARPS * SG>(p);
     Walk<ROWS, KV_GRANULE, S::SEGMENT> walk(pl);
     Segment sg;
 
@@ -518,22 +518,25 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
                 const uint32_t parts = (c1 - c0) + 1;
                 const float *first_part = p.partials + ((size_t)c0 * 2 + 1) * S::PARTIAL, *other = p.partials + ((size_t)c0 + 1) * 2 * S::PARTIAL;
                 auto part = [&](uint32_t c) { return c ? other + (size_t)(c - 1) * 2 * S::PARTIAL : first_part; };
-                float *weight = join;  // [parts][ROWS], then the sums
-                for (uint32_t i = tid; i < parts * ROWS; i += S::THREADS) {
-                    weight[i] = __ldcg(part(i / ROWS) + ROWS * W + i % ROWS);
-                    weight[(parts + i / ROWS) * ROWS + i % ROWS] = __ldcg(part(i / ROWS) + ROWS * W + ROWS + i % ROWS);
-                }
-                __syncthreads();
-                if (tid < ROWS) {
+                float *weight = join;  // [parts][ROWS]
+                for (uint32_t r = warp; r < ROWS; r += WARPS) {  // a warp a row, a lane a part
                     float top = -INFINITY, sum = 0.0f;
-                    for (uint32_t c = 0; c < parts; ++c) top = fmaxf(top, weight[c * ROWS + tid]);
-                    const float ref = top == -INFINITY ? 0.0f : top;
-                    for (uint32_t c = 0; c < parts; ++c) {
-                        const float f = exp2f(weight[c * ROWS + tid] - ref);
-                        sum += weight[(parts + c) * ROWS + tid] * f;
-                        weight[c * ROWS + tid] = f;
+                    for (uint32_t c = lane; c < parts; c += 32) {
+                        const float x = __ldcg(part(c) + ROWS * W + r);
+                        weight[c * ROWS + r] = x;
+                        top = fmaxf(top, x);
                     }
-                    row_scale[tid] = 1.0f / sum;
+#pragma unroll
+                    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    const float ref = top == -INFINITY ? 0.0f : top;
+                    for (uint32_t c = lane; c < parts; c += 32) {
+                        const float f = exp2f(weight[c * ROWS + r] - ref);
+                        sum += __ldcg(part(c) + ROWS * W + ROWS + r) * f;
+                        weight[c * ROWS + r] = f;
+                    }
+#pragma unroll
+                    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    if (lane == 0) row_scale[r] = 1.0f / sum;
                 }
                 __syncthreads();
                 for (uint32_t e = tid * 4; e < ROWS * W; e += S::THREADS * 4) {

@@ -92,7 +92,7 @@ struct Plan {
 };
 
 // One warp's finding, the same in every warp: no barrier. Lanes take entries in turn.
-template <uint32_t ROWS, uint32_t STEP, uint32_t SEGMENT>
+template <uint32_t ROWS, uint32_t STEP, uint32_t SEGMENT, uint32_t LEAST>
 __device__ __forceinline__ Plan plan(const AttentionParams &p) {
     const uint32_t lane = threadIdx.x & 31, entries = p.sequences * p.tiles, blocks = gridDim.x, heads = p.c.heads;
     uint32_t first, one = 0;  // the steps of this lane's first entry
@@ -120,10 +120,11 @@ __device__ __forceinline__ Plan plan(const AttentionParams &p) {
     r.total = total + units * SEGMENT;
     r.share = (r.total + blocks - 1) / blocks;
     if (total == 0) { r.idle = true; return r; }
-    // Even parts: 1 + count * spare / total blocks for a unit of `count` steps, at most `blocks` together. Taken if the longest part
+    // Even parts: 1 + count * spare / total blocks for a unit of `count` steps, at most `blocks` together and of LEAST steps or more (what a
+    // block's warps do at once: shorter parts would only be more to join). Taken if the longest part
     // is not much longer than an equal share, which costs most blocks a second segment.
     const unsigned long long spare = units <= blocks ? blocks - units : 0;
-    auto parts = [&](uint32_t count) { return 1 + (uint32_t)((unsigned long long)count * spare / total); };
+    auto parts = [&](uint32_t count) { return min(1 + (uint32_t)((unsigned long long)count * spare / total), (count + LEAST - 1) / LEAST); };
     if (units <= blocks) {
         uint32_t longest = 0;
         for (uint32_t e = lane; e < entries; e += 32) {

@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
     const uint32_t tmem = *tmem_slot;
     wait_for_previous_operator();
 
-    const Plan pl = plan<ROWS, KT, T::SEGMENT>(p);
+    const Plan pl = plan<ROWS, KT, T::SEGMENT, 2>(p);
     Walk<ROWS, KT, T::SEGMENT> walk(pl);
     Segment sg;
 

@@ -71,15 +71,16 @@ struct RowsParams {
     size_t stride[2];
 };
 
-__device__ __forceinline__ bool item_of(const RowsParams &p, size_t index, Item &it) {
-    it.which = (uint32_t)(index & 1);
+// (The host's limit on a call's rows keeps the count of items below 2^32.)
+__device__ __forceinline__ bool item_of(const RowsParams &p, uint32_t index, Item &it) {
+    it.which = index & 1;
     index >>= 1;
-    it.dim0 = (uint32_t)(index % p.pieces) * 128;
+    it.dim0 = index % p.pieces * 128;
     index /= p.pieces;
-    it.head = (uint32_t)(index % p.c.heads);
+    it.head = index % p.c.heads;
     index /= p.c.heads;
-    it.granule = (uint32_t)(index % p.granules);
-    it.sequence = (uint32_t)(index / p.granules);
+    it.granule = index % p.granules;
+    it.sequence = index / p.granules;
     if (it.sequence >= p.sequences) return false;
     it.dims = min(128u, p.c.l.width - it.dim0);
     it.span = kv_span(p.c, p.spans, it.sequence, p.tokens);
@@ -206,7 +207,7 @@ __global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(const RowsParams p
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     wait_for_previous_operator();
     Item it;
-    if (!item_of(p, (size_t)blockIdx.x * KV_WARPS + warp, it)) return;
+    if (!item_of(p, blockIdx.x * KV_WARPS + warp, it)) return;
     // where two spans of a call cover the same position, the row of the later span is written
     for (uint32_t later = it.sequence + 1; later < p.sequences; later += 32) {
         uint32_t covered = 0;
@@ -310,7 +311,7 @@ __global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const RowsParams p)
     const uint32_t warp = threadIdx.x / 32;
     wait_for_previous_operator();
     Item it;
-    if (!item_of(p, (size_t)blockIdx.x * KV_WARPS + warp, it)) return;
+    if (!item_of(p, blockIdx.x * KV_WARPS + warp, it)) return;
     if (it.which) {
         if (p.c.l.v8) read_item<true, true, T>(p, it, staged[warp]);
         else read_item<true, false, T>(p, it, staged[warp]);
