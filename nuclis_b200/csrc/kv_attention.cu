@@ -9,12 +9,13 @@
 //     to the codes. What is not exact in f16, the query and the probabilities, is split: x = hi + lo with both in
 //     f16 (22 bits). The 16 rows of the A operand are the hi parts of eight query rows and their lo parts, so the split
 //     costs no second instruction, and the two sums of a row come out in the same thread.
-//   * q . k = sum_b d_b (q_b . c_b): one accumulator pair of instructions per block of 32, then F32 FMAs with d_b. The key's code
-//     without sign is left where it lies in its word: as f16 that is code * 2^-24, a subnormal number (16 times that
-//     from a high nibble, which the query's fragment makes up for), so a pair of codes costs one logical operation. The
-//     offset (8 or 128) comes off the sum instead, sum_b d_b * sum(q_b): one more product with the scales as they lie. It is as
-//     large as the sums themselves, so nothing is lost; the values' sums run over the positions, where it would grow
-//     with their number, so their codes get their sign first.
+//   * q . k = sum_b d_b (q_b . c_b): one accumulator pair of instructions per block of 32, then F32 FMAs with d_b. Four-bit codes
+//     get their sign on the way (two operations a pair). Eight-bit key codes are left without sign where they lie in their word: as
+//     f16 that is code * 2^-24, a subnormal number, so a pair costs one permute; the offset of 128 comes off the
+//     sum instead, sum_b d_b * sum(q_b): one more product with the scales as they lie. It is as large as the sums themselves, so
+//     nothing is lost. (Four-bit codes left like that lose the product's low bits: it is aligned by the subnormal's exponent,
+//     under which they have six leading zeros more; the result was off by 1.9e-6 instead of 3e-7. And the values' sums
+//     run over the positions, where the offset's share would grow with their number.)
 //   * p v = sum_j (p_j d_jb) c_j: the scale goes into the probability, once per block, before it is split. The products
 //     p d are kept near 2^11 by a power of two per warp (`bias`), lowered when a larger scale comes by: f16's range is no limit,
 //     and what is lost of a position is below 2^-36 of the largest value seen.
@@ -258,8 +259,8 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
             top = __reduce_max_sync(0xffffffffu, top);
             // 2^e: from the exponent's bits; rows of zeros and of subnormal values count as 2^-126
             const int e = (int)max(top >> 23, 1u) - 127;
-            const float down = top >= 0x7f800000u ? NAN : scalbnf(1.0f, -e), up = K8 ? 1.0f : 0.0625f;
-            if (lane == 0) row_scale[r] = scalbnf(p.scale, e - 13 + 24);  // the query's power of two, and the codes'
+            const float down = top >= 0x7f800000u ? NAN : scalbnf(1.0f, -e);
+            if (lane == 0) row_scale[r] = scalbnf(p.scale, e - 13 + (K8 ? 24 : 0));  // the query's power of two, and the codes'
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -278,10 +279,7 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
                 const uint32_t b = lane / 4, tt = lane % 4;
                 uint32_t hi[4], lo[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float f = i % 2 ? up : 1.0f;  // Q4_0: dimensions 1, 5, 3, 7 meet high nibbles
-                    hi[i] = pack_hi_lo(x[i] * f, x[i + 4] * f, lo[i]);
-                }
+                for (int i = 0; i < 4; ++i) hi[i] = pack_hi_lo(x[i], x[i + 4], lo[i]);
                 // the pair of dimensions i, i + 4 of the eight is the k pair of step i / 2, half i % 2
                 fragments[(2 * b) * 32 + r * 4 + tt] = make_uint4(hi[0], lo[0], hi[1], lo[1]);
                 fragments[(2 * b + 1) * 32 + r * 4 + tt] = make_uint4(hi[2], lo[2], hi[3], lo[3]);
@@ -330,13 +328,15 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
                     const uint8_t *gran = stage + j / 2 * L.bytes;
                     load_words<K8 ? 2 * NB : NB, L.k_vec>(gran + j % 2 * (L.k_scales / 2), lane, codes[j]);
                     load_scales<NB>(gran + L.k_scales, j % 2 * 8 + 2 * t, scales[j]);
-                    // what the codes' offset adds: sum_b d_b * offset * sum(q_b), in units of 2^-24; the sums carry 2^-5
-                    float c[4];
-                    const uint32_t pair = 2 * t < NB ? *(const uint32_t *)(gran + L.k_scales + ((j % 2 * 8 + g) * NB + 2 * t) * 2) : 0u;
-                    mma_zero(c, sums, pair, 0u);
-                    constexpr float OFFSET = -(K8 ? 128.0f : 8.0f) * 32.0f / 16777216.0f;
-                    s[j][0] = (c[0] + c[2]) * OFFSET;
-                    s[j][1] = (c[1] + c[3]) * OFFSET;
+                    s[j][0] = s[j][1] = 0.0f;
+                    if (K8) {  // what the codes' offset takes off: sum_b d_b * 128 * sum(q_b), in units of 2^-24; the sums carry 2^-5
+                        float c[4];
+                        const uint32_t pair = 2 * t < NB ? *(const uint32_t *)(gran + L.k_scales + ((j % 2 * 8 + g) * NB + 2 * t) * 2) : 0u;
+                        mma_zero(c, sums, pair, 0u);
+                        constexpr float OFFSET = -128.0f * 32.0f / 16777216.0f;
+                        s[j][0] = (c[0] + c[2]) * OFFSET;
+                        s[j][1] = (c[1] + c[3]) * OFFSET;
+                    }
                 }
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
@@ -349,8 +349,8 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
                             mma(c, q1, __byte_perm(codes[j][2 * b + 1], 0u, 0x4140), __byte_perm(codes[j][2 * b + 1], 0u, 0x4342));
                         } else {
                             const uint32_t w = codes[j][b], w8 = w >> 8;
-                            mma_zero(c, q0, w & 0x000f000fu, w & 0x00f000f0u);
-                            mma(c, q1, w8 & 0x000f000fu, w8 & 0x00f000f0u);
+                            mma_zero(c, q0, low_codes(w, k1024), high_codes(w, k1024));
+                            mma(c, q1, low_codes(w8, k1024), high_codes(w8, k1024));
                         }
                         s[j][0] = fmaf(scale_of<NB>(scales[j], 0, b), c[0] + c[2], s[j][0]);
                         s[j][1] = fmaf(scale_of<NB>(scales[j], 1, b), c[1] + c[3], s[j][1]);
