@@ -1,7 +1,6 @@
 """The synthetic dense decode layer stack: 64 layers of QKV -> O -> SwiGLU gate/up -> down.
 
-Only the matmul chain of a decoder layer is here (attention, norms and
-residuals are other operators' business): per layer
+The matmul chain of a decoder layer: per layer
 
     qkv = Wqkv . h                      Q4_K  [hidden + 2 kv][hidden]
     o   = Wo . qkv[:hidden]             Q4_K  [hidden][hidden]         (+ allreduce)
@@ -16,6 +15,10 @@ random weights overflow F32 within a dozen products, and the norms that keep a
 real model bounded are not part of this path. Stream order keeps the layers
 serial all the same, and every weight byte of every layer is read each step.
 
+Norms and residuals come in with ``enable_norms``, attention over a quantized
+key/value cache between QKV and O with ``enable_attention``; without the latter O
+reads the Q slice as it is, which is what the matmul benchmark times.
+
 With ``ranks`` > 1 the layer is row-split (see ``shard``): each rank holds its
 rows of QKV/gate/up and its K slice of O/down, and the partial O and down
 outputs are summed over the ranks.
@@ -27,7 +30,7 @@ from dataclasses import dataclass, field
 import numpy as np
 
 from . import encoding as enc
-from .backend import Backend, Buffer, Matrix, Segment, SegmentMode
+from .backend import Backend, Buffer, KvCache, Matrix, Segment, SegmentMode, kv_spans
 from .errors import NuclisError
 from .shard import LayerShapes, RankShapes, rank_shapes
 
@@ -93,6 +96,40 @@ class Stack:
         w.down = prepared
         self.m_down = m
 
+    # ---- attention ----
+    def enable_attention(self, capacity: int, width: int = 128, key_encoding: int = enc.Q8_0, value_encoding: int = enc.Q8_0, window: int = 0) -> None:
+        """Adds what a decoder layer has between its QKV and its O projection: the step's keys and values into the layer's quantized
+        cache, and causal grouped-query attention over it (heads of ``width``; this rank's where the layer is split). The step's
+        position is read on the device: ``seek`` moves a recorded step on."""
+        b, l, m = self.backend, self.local, self.tokens
+        if l.q_rows % width or l.kv_rows % width or l.q_rows % l.kv_rows:
+            raise ValueError("the rows of Q and of K are whole heads, and a key/value head serves as many query heads as another")
+        self.kv_shape = KvCache(1, (capacity + 15) // 16 * 16, l.kv_rows // width, width, key_encoding, value_encoding)
+        self.kv_window = window
+        self.caches = [b.create(self.kv_shape.bytes) for _ in self.layers]
+        self.spans = b.create(16)
+        # a prompt's rows go into O's prefill product as BF16, which rounds them anyway
+        self.att_dtype = enc.BF16 if m > Backend.matvec_rows_max else enc.F32
+        self.att = b.create((Backend.matmul_padded(m) if m > 1 else 1) * l.q_rows * (2 if self.att_dtype == enc.BF16 else 4))
+        self.seek(0)
+
+    def seek(self, position: int) -> None:
+        """The next step's rows stand at ``position`` and behind it (between recordings: the spans are uploaded)."""
+        self.spans.write(kv_spans([(0, position, self.tokens)]))
+
+    def record_attention(self, layer: int) -> tuple[Buffer, int, int]:
+        """O's input for the layer: buffer, row stride and dtype."""
+        b, l, m = self.backend, self.local, self.tokens
+        if getattr(self, "caches", None) is None:
+            return self.qkv.slice(0, self.qkv.len), l.qkv_rows, enc.F32
+        cache, shape = self.caches[layer], self.kv_shape
+        keys = self.qkv.slice(l.q_rows * 4, self.qkv.len - l.q_rows * 4)
+        values = self.qkv.slice((l.q_rows + l.kv_rows) * 4, self.qkv.len - (l.q_rows + l.kv_rows) * 4)
+        b.kv_write(cache, shape, self.spans, 1, m, keys, l.qkv_rows, values, l.qkv_rows)
+        b.attention(cache, shape, self.spans, 1, m, self.qkv, l.qkv_rows, l.q_rows // shape.width, self.att, l.q_rows, window=self.kv_window,
+                    out_dtype=self.att_dtype)
+        return self.att, l.q_rows, self.att_dtype
+
     # ---- the recording of one step ----
     def enable_norms(self, seed: int = 0) -> None:
         """Adds what a pre-norm decoder layer has around its projections (inference/src/models/qwen35_metal.zig:635-640):
@@ -115,9 +152,10 @@ class Stack:
         staging passes of QKV and of the gate/up pair, the adds into the writes of O and down; with the layer split over
         ranks (``reduce``) the adds are folded into the gathers of the two sums instead."""
         b, hidden = self.backend, self.shapes.hidden
-        a_in = self.qkv.slice(0, self.qkv.len)
-        for w in self.layers:
+        attention = 2 if getattr(self, "caches", None) is not None else 0
+        for i, w in enumerate(self.layers):
             b.matvec_segments_normed([Segment(w.qkv, self.m_qkv, self.qkv)], self.residual, self.norm_attn)
+            a_in, _, _ = self.record_attention(i)
             if reduce:
                 b.matvec(w.o, self.m_o, a_in, self.o)
                 b.allreduce_sum_add_f32(self.o, self.residual, hidden)
@@ -130,19 +168,21 @@ class Stack:
                 b.allreduce_sum_add_f32(self.d, self.residual, hidden)
             else:
                 b.matvec_add(w.down, self.m_down, self.g, self.residual, self.residual)
-        return (6 if reduce else 4) * len(self.layers)
+        return ((6 if reduce else 4) + attention) * len(self.layers)
 
     def record(self, allreduce: bool | None = None) -> int:
         """Records every layer's chain into the open recording; returns how many operators it recorded."""
         b, s, l, m = self.backend, self.shapes, self.local, self.tokens
         reduce = l.ranks > 1 if allreduce is None else allreduce
         ops = 0
-        a_in = self.qkv.slice(0, self.qkv.len)  # the Q slice: the first q_rows floats of each token row
+        attention = 2 if getattr(self, "caches", None) is not None else 0
         if getattr(self, "residual", None) is not None and m == 1:
             return self.record_with_norms(reduce)
-        for w in self.layers:
+        for i, w in enumerate(self.layers):
+            ops += attention
             if m == 1:
                 b.matvec(w.qkv, self.m_qkv, self.h, self.qkv)
+                a_in, a_stride, a_dtype = self.record_attention(i)  # without attention the Q slice: the first q_rows floats of each token row
                 b.matvec(w.o, self.m_o, a_in, self.o)
                 ops += 2
                 if reduce:
@@ -166,7 +206,8 @@ class Stack:
                     ops += 1
             else:
                 b.matmul(w.qkv, self.m_qkv, self.h, s.hidden, self.qkv, l.qkv_rows, m)
-                b.matmul(w.o, self.m_o, a_in, l.qkv_rows, self.o, s.hidden, m)
+                a_in, a_stride, a_dtype = self.record_attention(i)
+                b.matmul(w.o, self.m_o, a_in, a_stride, self.o, s.hidden, m, in_dtype=a_dtype)
                 ops += 2
                 if reduce:
                     b.allreduce_sum_f32(self.o, m * s.hidden)
