@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
     Walk<ROWS, KV_GRANULE, S::SEGMENT> walk(pl);
     Segment sg;
 
-    uint32_t turn = 0;  // stages this warp has taken, over all segments: position and phase in the ring
+    uint32_t turn = 0, phase = 0;  // the warp's place in its ring, over all segments
     bool alive = true;
     while (walk.next(p, pl, sg)) {
         // ---- the segment: granules [g0, g0 + n) of one unit, which the blocks c0 .. c1 share ----
@@ -229,13 +229,18 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
         const uint32_t g0 = sg.first + skip;
         const uint8_t *base = kv_head(p.c, span.slot, head) + (size_t)g0 * L.bytes;
         const uint32_t stages = (n + SG - 1) / SG, mystages = stages > warp ? (stages - warp + WARPS - 1) / WARPS : 0;
-        auto request = [&](uint32_t i) {  // the warp's stage i of this segment
-            const uint32_t st = warp + i * WARPS, pos = (turn + i) % STAGES;
-            const uint32_t bytes = min((uint32_t)SG, n - st * SG) * L.bytes;
-            bulk_load(smem_u32(ring + (warp * STAGES + pos) * S::STAGE), base + (size_t)st * S::STAGE, bytes, smem_u32(bars + warp * STAGES + pos));
+        // the ring: `turn` is the place of the warp's next stage, `phase` its barrier's parity; a place is filled again as soon as it is read
+        const uint8_t *source = base + (size_t)warp * S::STAGE;
+        uint32_t left = mystages, place = turn;
+        auto request = [&]() {
+            const uint32_t bytes = SG == 1 || left > 1 ? S::STAGE : min((uint32_t)SG, n - (warp + (mystages - 1) * WARPS) * SG) * L.bytes;
+            bulk_load(smem_u32(ring + (warp * STAGES + place) * S::STAGE), source, bytes, smem_u32(bars + warp * STAGES + place));
+            source += (size_t)WARPS * S::STAGE;
+            --left;
+            place = place + 1 == STAGES ? 0 : place + 1;
         };
         if (lane == 0)
-            for (uint32_t i = 0; i < min(mystages, (uint32_t)STAGES); ++i) request(i);
+            for (uint32_t i = 0; i < min(mystages, (uint32_t)STAGES); ++i) request();
 
         // ---- the rows, split into f16 halves after a power of two that brings each row's largest value to [2^13, 2^14) ----
         const size_t rows0 = (size_t)sequence * p.tokens;  // the sequence's first row in the call
@@ -305,17 +310,21 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
         for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
 
         for (uint32_t i = 0; i < mystages && alive; ++i) {
-            const uint32_t slot = (turn + i) % STAGES;
-            alive = mbar_wait(smem_u32(bars + warp * STAGES + slot), (turn + i) / STAGES & 1u);
+            const uint32_t slot = turn;
+            alive = mbar_wait(smem_u32(bars + warp * STAGES + slot), phase);
             if (!__all_sync(0xffffffffu, alive)) {  // a copy never came: report, let the others in flight land, give up the block's results
                 *(volatile uint32_t *)p.c.status = 1u;
-                for (uint32_t k = i + 1; k < min(i + STAGES, mystages); ++k) mbar_wait(smem_u32(bars + warp * STAGES + (turn + k) % STAGES), (turn + k) / STAGES & 1u);
+                for (uint32_t k = i + 1; k < min(i + STAGES, mystages); ++k) {
+                    if (++turn == STAGES) { turn = 0; phase ^= 1u; }
+                    mbar_wait(smem_u32(bars + warp * STAGES + turn), phase);
+                }
                 alive = false;
                 break;
             }
+            if (++turn == STAGES) { turn = 0; phase ^= 1u; }
             const uint8_t *stage = ring + (warp * STAGES + slot) * S::STAGE;
             const uint32_t st = warp + i * WARPS, key0 = (g0 + st * SG) * KV_GRANULE;
-            const uint32_t here = min((uint32_t)SG, n - st * SG) * KV_GRANULE;  // positions that were copied
+            const uint32_t here = SG == 1 ? KV_GRANULE : min((uint32_t)SG, n - st * SG) * KV_GRANULE;  // positions that were copied
             const bool at_edge = key0 < all_low || key0 + SG * KV_GRANULE - 1 > first_pos || here < SG * KV_GRANULE;
             auto take = [&](auto edge_tag) {
             constexpr bool edge = decltype(edge_tag)::value;
@@ -452,9 +461,8 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
             if (at_edge) take(std::true_type{});
             else take(std::false_type{});
             __syncwarp();
-            if (lane == 0 && i + STAGES < mystages) request(i + STAGES);
+            if (lane == 0 && left) request();
         }
-        turn += mystages;
 
         // ---- join the warps ----
         l += __shfl_xor_sync(0xffffffffu, l, 1);

@@ -85,9 +85,10 @@ __device__ __forceinline__ void unit_range(const AttentionParams &p, const KvSpa
 //
 // Where a block starts: which entry ((sequence, row tile), all of whose heads have the same steps) and how far into it.
 struct Plan {
-    bool even;                      // every block has one part of one unit; else an equal share of all steps (and segments)
+    bool even;                      // every block has one part of one unit
+    bool whole;                     // every block has whole units, longest first; else an equal share of all steps (and segments)
     unsigned long long share, total;
-    uint32_t entry, in;             // in: blocks (even) or steps into the entry
+    uint32_t entry, in;             // in: blocks (even) or steps into the entry; whole: the units
     bool idle;
 };
 
@@ -133,6 +134,27 @@ __device__ __forceinline__ Plan plan(const AttentionParams &p) {
         }
         r.even = __reduce_max_sync(0xffffffffu, longest) <= r.share + SEGMENT;
     }
+    // Whole units: a prompt has its units in order of length, so the blocks take them from the longest down, forwards and backwards in turn.
+    // Nothing is joined then; taken where no block gets much more than an equal share (with many rounds none does).
+    if (p.sequences == 1 && units > blocks) {
+        const uint32_t n = (uint32_t)units, rounds = (n + blocks - 1) / blocks;
+        uint32_t longest = 0;
+        if (rounds <= 8)
+            for (uint32_t b = lane; b < blocks; b += 32) {
+                uint32_t load = 0;
+                for (uint32_t j = 0; j < rounds; ++j) {
+                    const uint32_t u = j * blocks + (j & 1u ? blocks - 1 - b : b);
+                    if (u < n) load += steps((n - 1 - u) / heads) + SEGMENT;
+                }
+                longest = max(longest, load);
+            }
+        r.whole = __reduce_max_sync(0xffffffffu, longest) <= r.share + SEGMENT;
+        if (r.whole) {
+            r.in = n;
+            r.share = rounds;
+            return r;
+        }
+    }
     const unsigned long long at = r.even ? blockIdx.x : blockIdx.x * r.share;
     unsigned long long before = 0;
     r.idle = true;
@@ -175,13 +197,26 @@ struct Walk {
     unsigned long long at, end, entry_begin;
     uint32_t entry;
     __device__ __forceinline__ explicit Walk(const Plan &pl) {
-        at = pl.even ? 0 : blockIdx.x * pl.share;
-        end = pl.idle ? 0 : pl.even ? 1 : min(pl.total, at + pl.share);  // even parts: one turn
+        at = pl.even || pl.whole ? 0 : blockIdx.x * pl.share;
+        end = pl.idle ? 0 : pl.even ? 1 : pl.whole ? pl.share : min(pl.total, at + pl.share);  // even parts: one turn; whole units: one a round
         entry_begin = at - pl.in;
         entry = pl.entry;
     }
     __device__ __forceinline__ bool next(const AttentionParams &p, const Plan &pl, Segment &s) {
         while (at < end) {
+            if (pl.whole) {
+                const uint32_t j = (uint32_t)at++, u = j * gridDim.x + (j & 1u ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+                if (u >= pl.in) continue;
+                s.sequence = 0;
+                s.tile = (pl.in - 1 - u) / p.c.heads;
+                s.head = (pl.in - 1 - u) % p.c.heads;
+                s.span = kv_span(p.c, p.spans, 0, p.tokens);
+                unit_range<ROWS, STEP>(p, s.span, s.tile, s.first, s.count);
+                s.skip = 0;
+                s.n = s.count;
+                s.c0 = s.c1 = blockIdx.x;
+                return true;
+            }
             s.sequence = entry / p.tiles;
             s.tile = entry % p.tiles;
             s.span = kv_span(p.c, p.spans, s.sequence, p.tokens);

@@ -527,33 +527,63 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                 named_barrier<1, 256>();
                 if (tid == 0) *last = atomicAdd(p.counters + sg.c0, 1u) == sg.c1 - sg.c0;
                 named_barrier<1, 256>();
-                if (*last) {  // this block arrived last: the parts of all blocks, in their order; a warp takes a row at a time
+                if (*last) {  // this block arrived last: the parts of all blocks, in their order
                     __threadfence();
                     const uint32_t parts = sg.c1 - sg.c0 + 1;
                     auto part = [&](uint32_t c) { return p.partials + ((size_t)(sg.c0 + c) * 2 + (c == 0)) * T::PARTIAL; };
-                    for (uint32_t r = warp; r < (uint32_t)ROWS; r += T::SOFT) {
-                        const uint32_t to = tile_row0 + r;
-                        if (to >= live_rows) break;
+                    // a thread a row finds the parts' weights, 2^(their maximum - the row's) over the row's sum (KEPT parts' into the queries' place);
+                    // then a warp adds up ROWS_AT rows at a time, so that many loads are on their way
+                    constexpr uint32_t KEPT = 32, ROWS_AT = 4, EACH = W / 32;
+                    static_assert(KEPT * ROWS * 4 <= QT * T::Q_TILE, "the weights take the queries' place");
+                    float *weight = (float *)(smem + T::Q);  // [KEPT][ROWS]
+                    // a part that the row does not see (its maximum is minus infinity) has weight 0 and stays out, whatever it holds
+                    auto weigh = [](float m, float mm, float inv) {
+                        const float f = exp2_approx(m - mm);
+                        return f == 0.0f ? 0.0f : f * inv;
+                    };
+                    if (tid < (uint32_t)ROWS) {
                         float mm = -INFINITY, ll = 0.0f;
-                        for (uint32_t c = 0; c < parts; ++c) mm = fmaxf(mm, __ldcg(part(c) + ROWS * W + r));
-                        const float ref = mm == -INFINITY ? 0.0f : mm;
-                        constexpr int EACH = W / 32;
-                        float acc[EACH] = {};
-#pragma unroll 4
-                        for (uint32_t c = 0; c < parts; ++c) {
-                            const float f = exp2_approx(__ldcg(part(c) + ROWS * W + r) - ref);
-                            ll += __ldcg(part(c) + ROWS * W + ROWS + r) * f;
-#pragma unroll
-                            for (int k = 0; k < EACH; ++k) {
-                                const float x = __ldcg(part(c) + (size_t)r * W + k * 32 + lane);
-                                acc[k] = f > 0.0f ? fmaf(x, f, acc[k]) : acc[k];  // a part that the row does not see may hold anything
-                            }
-                        }
-                        __nv_bfloat16 *dst = (__nv_bfloat16 *)p.out + (rows0 + to / p.group) * p.out_stride + (size_t)(sg.head * p.group + to % p.group) * W;
-                        const float inv = 1.0f / ll;
-#pragma unroll
-                        for (int k = 0; k < EACH; ++k) dst[k * 32 + lane] = __float2bfloat16_rn(acc[k] * inv);
+                        for (uint32_t c = 0; c < parts; ++c) mm = fmaxf(mm, __ldcg(part(c) + ROWS * W + tid));
+                        mm = mm == -INFINITY ? 0.0f : mm;
+                        for (uint32_t c = 0; c < parts; ++c) ll += __ldcg(part(c) + ROWS * W + ROWS + tid) * exp2_approx(__ldcg(part(c) + ROWS * W + tid) - mm);
+                        ll = 1.0f / ll;
+                        for (uint32_t c = 0; c < min(parts, KEPT); ++c) weight[c * ROWS + tid] = weigh(__ldcg(part(c) + ROWS * W + tid), mm, ll);
+                        exchange[tid] = mm;
+                        exchange[256 + tid] = ll;
                     }
+                    named_barrier<1, 256>();
+                    for (uint32_t r0 = warp * ROWS_AT; r0 < (uint32_t)ROWS; r0 += T::SOFT * ROWS_AT) {
+                        float acc[ROWS_AT][EACH] = {};
+#pragma unroll 2
+                        for (uint32_t c = 0; c < parts; ++c)
+#pragma unroll
+                            for (uint32_t i = 0; i < ROWS_AT; ++i) {
+                                const float f = c < KEPT ? weight[c * ROWS + r0 + i] : weigh(__ldcg(part(c) + ROWS * W + r0 + i), exchange[r0 + i], exchange[256 + r0 + i]);
+                                float x[EACH];
+                                const float *src = part(c) + (size_t)(r0 + i) * W + lane * EACH;
+                                if (EACH == 2) {
+                                    const float2 y = __ldcg((const float2 *)src);
+                                    x[0] = y.x; x[EACH - 1] = y.y;
+                                } else {
+#pragma unroll
+                                    for (uint32_t k = 0; k < EACH; k += 4) {
+                                        const float4 y = __ldcg((const float4 *)(src + k));
+                                        x[k] = y.x; x[(k + 1) % EACH] = y.y; x[(k + 2) % EACH] = y.z; x[(k + 3) % EACH] = y.w;
+                                    }
+                                }
+#pragma unroll
+                                for (uint32_t k = 0; k < EACH; ++k) acc[i][k] = f != 0.0f ? fmaf(x[k], f, acc[i][k]) : acc[i][k];
+                            }
+#pragma unroll
+                        for (uint32_t i = 0; i < ROWS_AT; ++i) {
+                            const uint32_t to = tile_row0 + r0 + i;
+                            if (to >= live_rows) continue;
+                            __nv_bfloat16 *dst = (__nv_bfloat16 *)p.out + (rows0 + to / p.group) * p.out_stride + (size_t)(sg.head * p.group + to % p.group) * W + lane * EACH;
+#pragma unroll
+                            for (uint32_t k = 0; k < EACH; ++k) dst[k] = __float2bfloat16_rn(acc[i][k]);
+                        }
+                    }
+                    named_barrier<1, 256>();
                     if (tid == 0) p.counters[sg.c0] = 0;
                 }
             }

@@ -227,6 +227,11 @@ __global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(const RowsParams p
     }
 }
 
+// A code without sign, placed in the low bits of 2^23, less 2^23 and its offset: exact, and the two operations run at four times a
+// conversion's rate.
+template <bool Q8>
+__device__ __forceinline__ float code_value(uint32_t code) { return __uint_as_float(code | 0x4b000000u) - (Q8 ? 8388736.0f : 8388616.0f); }
+
 template <typename T>
 __device__ __forceinline__ T out_value(float x);
 template <>
@@ -259,11 +264,11 @@ __device__ __forceinline__ void read_item(const RowsParams &p, const Item &it, S
                 for (int i = 0; i < 4; ++i) {
                     const uint32_t at = 2 * t + (i & 1) + (i >> 1) * 8;
                     if (Q8) {
-                        st.x[at][b * 32 + w * 8 + slot] = out_value<T>(__fmul_rn(d[i], (float)((int)(word >> (8 * i) & 255u) - 128)));
+                        st.x[at][b * 32 + w * 8 + slot] = out_value<T>(__fmul_rn(d[i], code_value<true>(word >> (8 * i) & 255u)));
                     } else {
                         const uint32_t byte = word >> (8 * ((i & 1) * 2 + (i >> 1)));
-                        st.x[at][b * 32 + w * 16 + slot] = out_value<T>(__fmul_rn(d[i], (float)((int)(byte & 15u) - 8)));
-                        st.x[at][b * 32 + w * 16 + 8 + slot] = out_value<T>(__fmul_rn(d[i], (float)((int)(byte >> 4 & 15u) - 8)));
+                        st.x[at][b * 32 + w * 16 + slot] = out_value<T>(__fmul_rn(d[i], code_value<false>(byte & 15u)));
+                        st.x[at][b * 32 + w * 16 + 8 + slot] = out_value<T>(__fmul_rn(d[i], code_value<false>(byte >> 4 & 15u)));
                     }
                 }
             }
@@ -278,8 +283,8 @@ __device__ __forceinline__ void read_item(const RowsParams &p, const Item &it, S
                 alignas(16) T x[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const int code = Q8 ? (int)((i % 4 < 2 ? w0 : w1) >> (8 * (i % 2 * 2 + i / 4)) & 255u) - 128 : (int)(w0 >> (4 * i) & 15u) - 8;
-                    x[i] = out_value<T>(__fmul_rn(d, (float)code));
+                    const uint32_t code = Q8 ? (i % 4 < 2 ? w0 : w1) >> (8 * (i % 2 * 2 + i / 4)) & 255u : w0 >> (4 * i) & 15u;
+                    x[i] = out_value<T>(__fmul_rn(d, code_value<Q8>(code)));
                 }
 #pragma unroll
                 for (int v = 0; v < (int)sizeof(x) / 16; ++v) *(uint4 *)((uint8_t *)&st.x[at][b * 32 + t * 8] + v * 16) = ((const uint4 *)x)[v];
