@@ -21,21 +21,25 @@ constexpr int KV_THREADS = 128;
 // Eight lanes hold a block, four values each. Returns this lane's four codes without sign (one a byte), and the scale.
 template <bool Q8>
 __device__ __forceinline__ uint32_t quantize4(const float x[4], float &scale) {
-    float top = 0.0f;  // the value of the largest magnitude, the first of equals
-    bool bad = false;
+    // magnitudes as integers: their order is the floats', and NaN and infinity come out on top
+    uint32_t a[4], own = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        bad |= !isfinite(x[i]);
-        if (fabsf(x[i]) > fabsf(top)) top = x[i];
+        a[i] = __float_as_uint(x[i]) & 0x7fffffffu;
+        own = max(own, a[i]);
     }
+    uint32_t top = own;
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
-        const float other = __shfl_xor_sync(0xffffffffu, top, o);
-        const bool lower = (threadIdx.x & o) != 0;  // the other lane holds earlier values
-        bad |= __shfl_xor_sync(0xffffffffu, (int)bad, o) != 0;
-        if (lower ? fabsf(other) >= fabsf(top) : fabsf(other) > fabsf(top)) top = other;
+    for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const bool bad = top >= 0x7f800000u;
+    float d;
+    if (Q8) {
+        d = __fmul_rn(__uint_as_float(top), 1.0f / 127.0f);
+    } else {  // with the sign of the first value of that magnitude
+        const float first = a[0] == top ? x[0] : a[1] == top ? x[1] : a[2] == top ? x[2] : x[3];
+        const uint32_t group = threadIdx.x & 24u, have = __ballot_sync(0xffffffffu, own == top) >> group & 0xffu;
+        d = __shfl_sync(0xffffffffu, first, group + __ffs(have) - 1) * -0.125f;
     }
-    float d = Q8 ? __fmul_rn(fabsf(top), 1.0f / 127.0f) : top * -0.125f;
     d = fminf(fmaxf(d, -65504.0f), 65504.0f);
     scale = bad ? NAN : d;
     const float inverse = bad || __half2float(__float2half_rn(d)) == 0.0f ? 0.0f : __fdiv_rn(1.0f, d);
@@ -104,27 +108,79 @@ __device__ __forceinline__ void transpose_bytes(uint32_t a, uint32_t b, uint32_t
 
 constexpr int KV_WARPS = KV_THREADS / 32;
 
-template <bool VALUES, bool Q8>
+// FULL: the piece has 128 dimensions and the codes lie in vectors of 16 bytes (widths of whole 128s), so that every place is a
+// matter of shifts.
+// The second half of writing values: the rows' codes in `words` ([position][lane], four a word) become the cache's words.
+template <bool Q8, bool FULL>
+__device__ __forceinline__ void transpose_item(const KvLayout &l, const Item &it, uint8_t *g, uint32_t (&words)[512]) {
+    const uint32_t lane = threadIdx.x & 31, mine = lane * 4, dims = FULL ? 128 : it.dims;
+    const bool live = FULL || mine < dims;
+    // this lane's words: four dimensions (four codes a byte of theirs, or with the partner's as nibbles), four groups of positions
+    uint32_t codes[KV_GRANULE];
+#pragma unroll
+    for (uint32_t at = 0; at < KV_GRANULE; ++at) codes[at] = words[at * 32 + lane];
+    __syncwarp();
+    const uint32_t per = Q8 ? dims / 8 : dims / 16;  // words of a lane slot
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt) {
+        uint32_t c[4];
+        transpose_bytes(codes[2 * tt], codes[2 * tt + 1], codes[8 + 2 * tt], codes[9 + 2 * tt], c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t w = c[i];
+            if (!Q8) {
+                w = __byte_perm(w, 0, 0x3120) & 0x0f0f0f0fu;  // 2t, 8 + 2t, 2t + 1, 9 + 2t
+                w |= __shfl_xor_sync(0xffffffffu, w, 2) << 4;
+            }
+            const uint32_t word = mine / (Q8 ? 8 : 16), slot = ((mine + i) % 8) * 4 + tt;
+            // vectors of four words a slot, as the cache keeps them
+            if (live && (Q8 || !(mine & 8))) words[word / 4 * 128 + slot * 4 + word % 4] = w;
+        }
+    }
+    __syncwarp();
+    const uint32_t word0 = Q8 ? it.dim0 / 8 : it.dim0 / 16;
+    if (it.live == 0xffffu && (FULL || (l.v_vec == 16 && per % 4 == 0))) {
+#pragma unroll
+        for (uint32_t v = 0; v < (Q8 ? 4 : 2); ++v)
+            if (FULL || v < per / 4) *(uint4 *)(g + l.v_codes + (word0 / 4 + v) * 512 + lane * 16) = *(const uint4 *)&words[v * 128 + lane * 4];
+    } else {
+        const uint32_t tt = lane % 4;
+#pragma unroll 1
+        for (uint32_t w = 0; w < per; ++w) {
+            const uint32_t x = words[w / 4 * 128 + lane * 4 + w % 4];
+            uint8_t *dst = g + l.v_codes + kv_word(FULL ? 16 : l.v_vec, lane, word0 + w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t at = Q8 ? 2 * tt + (i & 1) + (i >> 1) * 8 : 2 * tt + (i >> 1) + (i & 1) * 8;
+                if (it.live >> at & 1u) dst[i] = (uint8_t)(x >> (8 * i));
+            }
+        }
+    }
+}
+
+template <bool VALUES, bool Q8, bool FULL>
 __device__ __forceinline__ void write_item(const RowsParams &p, const Item &it, uint32_t (&words)[512], __half (&scales)[64]) {
     const KvLayout &l = p.c.l;
-    const uint32_t lane = threadIdx.x & 31, mine = lane * 4;
-    const bool live = mine < it.dims;  // blocks are whole: the eight lanes of one are live together
+    const uint32_t lane = threadIdx.x & 31, mine = lane * 4, dims = FULL ? 128 : it.dims;
+    const bool live = FULL || mine < dims;  // blocks are whole: the eight lanes of one are live together
     const uint32_t dim = it.dim0 + mine, b = dim / 32;
     // row of position 0 of the granule, before the rows' start where the span begins inside it; only live positions are read
     const float *row0 = (const float *)p.rows[VALUES] + ((ptrdiff_t)it.sequence * p.tokens + (ptrdiff_t)it.granule * KV_GRANULE - it.span.first) * (ptrdiff_t)p.stride[VALUES] +
                         (size_t)it.head * l.width + dim;
     uint8_t *g = kv_head(p.c, it.span.slot, it.head) + (size_t)it.granule * l.bytes;
     const bool aligned = ((uintptr_t)row0 | p.stride[VALUES] * 4) % 16 == 0;
-    uint32_t codes[KV_GRANULE];
+    const uint32_t t = dim % 32 / 8, second = dim / 4 % 2;
+    // Four positions at a time, their loads together; not unrolled further: a warp runs this once, and fetching the code was
+    // what it waited for when it was 16 positions long.
+#pragma unroll 1
+    for (uint32_t at0 = 0; at0 < KV_GRANULE; at0 += 4) {
+        if (!(it.live >> at0 & 15u)) continue;
+        float x[4][4];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        float x[8][4];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int at = half * 8 + i;
+        for (uint32_t i = 0; i < 4; ++i) {
             x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.0f;
-            if ((it.live >> at & 1u) && live) {
-                const float *row = row0 + (ptrdiff_t)at * (ptrdiff_t)p.stride[VALUES];
+            if ((it.live >> (at0 + i) & 1u) && live) {
+                const float *row = row0 + (ptrdiff_t)(at0 + i) * (ptrdiff_t)p.stride[VALUES];
                 if (aligned) {
                     const float4 v = __ldcs((const float4 *)row);
                     x[i][0] = v.x; x[i][1] = v.y; x[i][2] = v.z; x[i][3] = v.w;
@@ -135,70 +191,36 @@ __device__ __forceinline__ void write_item(const RowsParams &p, const Item &it, 
             }
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int at = half * 8 + i;
-            codes[at] = 0;
+        for (uint32_t i = 0; i < 4; ++i) {
+            const uint32_t at = at0 + i;
             if (!(it.live >> at & 1u)) continue;  // the same for the whole warp
             float scale;
-            codes[at] = quantize4<Q8>(x[i], scale);
+            const uint32_t codes = quantize4<Q8>(x[i], scale);
             if (lane % 8 == 0 && live) scales[at * 4 + lane / 8] = __float2half_rn(scale);
-            if (!VALUES) {
-                const uint32_t near = __shfl_xor_sync(0xffffffffu, codes[at], 1);  // the other half of eight dimensions
-                const uint32_t t = dim % 32 / 8, second = dim / 4 % 2;
+            if (VALUES) {
+                words[at * 32 + lane] = codes;
+            } else {
+                const uint32_t near = __shfl_xor_sync(0xffffffffu, codes, 1);  // the other half of eight dimensions
+                uint32_t *dst = (uint32_t *)(g + kv_key_word(l, FULL ? 16 : l.k_vec, at, b, t, Q8 ? second : 0));
                 if (live && Q8) {  // bytes 0,4,1,5 by the lane of dimensions 0..3, bytes 2,6,3,7 by the other
-                    const uint32_t low = second ? near : codes[at], high = second ? codes[at] : near;
-                    *(uint32_t *)(g + kv_key_word(l, at, b, t, second)) = __byte_perm(low, high, second ? 0x7362 : 0x5140);
+                    const uint32_t low = second ? near : codes, high = second ? codes : near;
+                    *dst = __byte_perm(low, high, second ? 0x7362 : 0x5140);
                 } else if (live && !second) {
-                    *(uint32_t *)(g + kv_key_word(l, at, b, t, 0)) = nibbles(codes[at]) | nibbles(near) << 16;
+                    *dst = nibbles(codes) | nibbles(near) << 16;
                 }
             }
         }
     }
     __syncwarp();
     uint8_t *gs = g + (VALUES ? l.v_scales : l.k_scales);
-    const uint32_t blocks = it.dims / 32;
-    if (it.live == 0xffffu && l.blocks == 4) {
-        ((uint32_t *)gs)[lane] = ((const uint32_t *)scales)[lane];
+    if (it.live == 0xffffu && FULL) {  // two blocks a word, two words a position
+        *(uint32_t *)(gs + lane / 2 * l.blocks * 2 + it.dim0 / 16 + lane % 2 * 4) = ((const uint32_t *)scales)[lane];
     } else {
+        const uint32_t blocks = dims / 32;
         for (uint32_t i = lane; i < KV_GRANULE * blocks; i += 32)
             if (it.live >> (i / blocks) & 1u) ((__half *)gs)[i / blocks * l.blocks + it.dim0 / 32 + i % blocks] = scales[i / blocks * 4 + i % blocks];
     }
-    if (!VALUES) return;
-
-    // this lane's words: four dimensions (four codes a byte of theirs, or with the partner's as nibbles), four groups of positions
-    const uint32_t per = Q8 ? it.dims / 8 : it.dims / 16;  // words of a lane slot
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        uint32_t c[4];
-        transpose_bytes(codes[2 * t], codes[2 * t + 1], codes[8 + 2 * t], codes[9 + 2 * t], c);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t w = c[i];
-            if (!Q8) {
-                w = __byte_perm(w, 0, 0x3120);  // 2t, 8 + 2t, 2t + 1, 9 + 2t
-                w |= __shfl_xor_sync(0xffffffffu, w, 2) << 4;
-            }
-            const uint32_t word = mine / (Q8 ? 8 : 16), slot = ((mine + i) % 8) * 4 + t;
-            // vectors of four words a slot, as the cache keeps them
-            if (live && (Q8 || !(mine & 8))) words[word / 4 * 128 + slot * 4 + word % 4] = w;
-        }
-    }
-    __syncwarp();
-    const uint32_t word0 = Q8 ? it.dim0 / 8 : it.dim0 / 16;
-    if (it.live == 0xffffu && l.v_vec == 16 && per % 4 == 0) {
-        for (uint32_t v = 0; v < per / 4; ++v) *(uint4 *)(g + l.v_codes + (word0 / 4 + v) * 512 + lane * 16) = *(const uint4 *)&words[v * 128 + lane * 4];
-    } else {
-        const uint32_t t = lane % 4;
-        for (uint32_t w = 0; w < per; ++w) {
-            const uint32_t x = words[w / 4 * 128 + lane * 4 + w % 4];
-            uint8_t *dst = g + l.v_codes + kv_word(l.v_vec, lane, word0 + w);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t at = Q8 ? 2 * t + (i & 1) + (i >> 1) * 8 : 2 * t + (i >> 1) + (i & 1) * 8;
-                if (it.live >> at & 1u) dst[i] = (uint8_t)(x >> (8 * i));
-            }
-        }
-    }
+    if (VALUES) transpose_item<Q8, FULL>(l, it, g, words);
 }
 
 __global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(const RowsParams p) {
@@ -218,12 +240,13 @@ __global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(const RowsParams p
         }
         it.live &= ~__reduce_or_sync(0xffffffffu, covered);
     }
+    const bool full = p.c.l.width % 128 == 0;
     if (it.which) {
-        if (p.c.l.v8) write_item<true, true>(p, it, words[warp], scales[warp]);
-        else write_item<true, false>(p, it, words[warp], scales[warp]);
+        if (p.c.l.v8) full ? write_item<true, true, true>(p, it, words[warp], scales[warp]) : write_item<true, true, false>(p, it, words[warp], scales[warp]);
+        else full ? write_item<true, false, true>(p, it, words[warp], scales[warp]) : write_item<true, false, false>(p, it, words[warp], scales[warp]);
     } else {
-        if (p.c.l.k8) write_item<false, true>(p, it, words[warp], scales[warp]);
-        else write_item<false, false>(p, it, words[warp], scales[warp]);
+        if (p.c.l.k8) full ? write_item<false, true, true>(p, it, words[warp], scales[warp]) : write_item<false, true, false>(p, it, words[warp], scales[warp]);
+        else full ? write_item<false, false, true>(p, it, words[warp], scales[warp]) : write_item<false, false, false>(p, it, words[warp], scales[warp]);
     }
 }
 
@@ -246,25 +269,29 @@ struct Staged {
     T x[KV_GRANULE][ROW];
 };
 
-template <bool VALUES, bool Q8, typename T>
+template <bool VALUES, bool Q8, bool FULL, typename T>
 __device__ __forceinline__ void read_item(const RowsParams &p, const Item &it, Staged<T> &st) {
     const KvLayout &l = p.c.l;
-    const uint32_t lane = threadIdx.x & 31, slot = lane / 4, t = lane % 4, b0 = it.dim0 / 32;
+    const uint32_t lane = threadIdx.x & 31, slot = lane / 4, t = lane % 4, b0 = it.dim0 / 32, dims = FULL ? 128 : it.dims;
     const uint8_t *g = kv_head(p.c, it.span.slot, it.head) + (size_t)it.granule * l.bytes;
     const __half *scales = (const __half *)(g + (VALUES ? l.v_scales : l.k_scales)) + b0;
     if (VALUES) {
-        for (uint32_t b = 0; b < it.dims / 32; ++b) {
+        constexpr int PER = Q8 ? 4 : 2;  // words of a block
+        const uint8_t *codes = g + l.v_codes;
+#pragma unroll
+        for (uint32_t b = 0; b < 4; ++b) {
+            if (!FULL && b >= dims / 32) break;
             float d[4];  // of positions 2t, 2t + 1, 8 + 2t, 9 + 2t
 #pragma unroll
             for (int i = 0; i < 4; ++i) d[i] = __half2float(scales[(2 * t + (i & 1) + (i >> 1) * 8) * l.blocks + b]);
 #pragma unroll
-            for (int w = 0; w < (Q8 ? 4 : 2); ++w) {
-                const uint32_t word = *(const uint32_t *)(g + l.v_codes + kv_word(l.v_vec, lane, (b0 + b) * (Q8 ? 4 : 2) + w));
+            for (int w = 0; w < PER; ++w) {
+                const uint32_t word = *(const uint32_t *)(codes + kv_word(FULL ? 16 : l.v_vec, lane, (b0 + b) * PER + w));
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const uint32_t at = 2 * t + (i & 1) + (i >> 1) * 8;
                     if (Q8) {
-                        st.x[at][b * 32 + w * 8 + slot] = out_value<T>(__fmul_rn(d[i], code_value<true>(word >> (8 * i) & 255u)));
+                        st.x[at][b * 32 + w * 8 + slot] = out_value<T>(__fmul_rn(d[i], code_value<true>(__byte_perm(word, 0u, 0x4440 + i))));
                     } else {
                         const uint32_t byte = word >> (8 * ((i & 1) * 2 + (i >> 1)));
                         st.x[at][b * 32 + w * 16 + slot] = out_value<T>(__fmul_rn(d[i], code_value<false>(byte & 15u)));
@@ -275,15 +302,18 @@ __device__ __forceinline__ void read_item(const RowsParams &p, const Item &it, S
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (uint32_t j = 0; j < 2; ++j) {
             const uint32_t at = j * 8 + slot;
-            for (uint32_t b = 0; b < it.dims / 32; ++b) {
+#pragma unroll
+            for (uint32_t b = 0; b < 4; ++b) {
+                if (!FULL && b >= dims / 32) break;
                 const float d = __half2float(scales[at * l.blocks + b]);
-                const uint32_t w0 = *(const uint32_t *)(g + kv_key_word(l, at, b0 + b, t, 0)), w1 = Q8 ? *(const uint32_t *)(g + kv_key_word(l, at, b0 + b, t, 1)) : 0u;
+                const uint32_t w0 = *(const uint32_t *)(g + kv_key_word(l, FULL ? 16 : l.k_vec, at, b0 + b, t, 0));
+                const uint32_t w1 = Q8 ? *(const uint32_t *)(g + kv_key_word(l, FULL ? 16 : l.k_vec, at, b0 + b, t, 1)) : 0u;
                 alignas(16) T x[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const uint32_t code = Q8 ? (i % 4 < 2 ? w0 : w1) >> (8 * (i % 2 * 2 + i / 4)) & 255u : w0 >> (4 * i) & 15u;
+                    const uint32_t code = Q8 ? __byte_perm(i % 4 < 2 ? w0 : w1, 0u, 0x4440 + i % 2 * 2 + i / 4) : w0 >> (4 * i) & 15u;
                     x[i] = out_value<T>(__fmul_rn(d, code_value<Q8>(code)));
                 }
 #pragma unroll
@@ -296,15 +326,26 @@ __device__ __forceinline__ void read_item(const RowsParams &p, const Item &it, S
     T *row0 = (T *)p.rows[VALUES] + ((ptrdiff_t)it.sequence * p.tokens + (ptrdiff_t)it.granule * KV_GRANULE - it.span.first) * (ptrdiff_t)p.stride[VALUES] +
               (size_t)it.head * l.width + it.dim0;
     constexpr uint32_t V = 16 / sizeof(T);
-    const uint32_t lanes = it.dims / V;  // vectors of a row
+    const uint32_t lanes = dims / V;  // vectors of a row
     if (((uintptr_t)row0 | p.stride[VALUES] * sizeof(T)) % 16 == 0) {
-        for (uint32_t i = lane; i < KV_GRANULE * lanes; i += 32) {
-            const uint32_t at = i / lanes, v = i % lanes;
-            if (it.live >> at & 1u) *(uint4 *)(row0 + (ptrdiff_t)at * (ptrdiff_t)p.stride[VALUES] + v * V) = *(const uint4 *)&st.x[at][v * V];
+        if (FULL) {
+            constexpr uint32_t LANES = 128 / V, TURN = 32 / LANES;  // rows a turn
+            T *dst = row0 + (ptrdiff_t)(lane / LANES) * (ptrdiff_t)p.stride[VALUES] + lane % LANES * V;
+#pragma unroll
+            for (uint32_t at = 0; at < KV_GRANULE; at += TURN) {
+                const uint32_t r = at + lane / LANES;
+                if (it.live >> r & 1u) __stcs((uint4 *)dst, *(const uint4 *)&st.x[r][lane % LANES * V]);
+                dst += (ptrdiff_t)TURN * (ptrdiff_t)p.stride[VALUES];
+            }
+        } else {
+            for (uint32_t i = lane; i < KV_GRANULE * lanes; i += 32) {
+                const uint32_t at = i / lanes, v = i % lanes;
+                if (it.live >> at & 1u) *(uint4 *)(row0 + (ptrdiff_t)at * (ptrdiff_t)p.stride[VALUES] + v * V) = *(const uint4 *)&st.x[at][v * V];
+            }
         }
     } else {
-        for (uint32_t i = lane; i < KV_GRANULE * it.dims; i += 32) {
-            const uint32_t at = i / it.dims, d = i % it.dims;
+        for (uint32_t i = lane; i < KV_GRANULE * dims; i += 32) {
+            const uint32_t at = i / dims, d = i % dims;
             if (it.live >> at & 1u) row0[(ptrdiff_t)at * (ptrdiff_t)p.stride[VALUES] + d] = st.x[at][d];
         }
     }
@@ -317,12 +358,13 @@ __global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const RowsParams p)
     wait_for_previous_operator();
     Item it;
     if (!item_of(p, blockIdx.x * KV_WARPS + warp, it)) return;
+    const bool full = p.c.l.width % 128 == 0;
     if (it.which) {
-        if (p.c.l.v8) read_item<true, true, T>(p, it, staged[warp]);
-        else read_item<true, false, T>(p, it, staged[warp]);
+        if (p.c.l.v8) full ? read_item<true, true, true, T>(p, it, staged[warp]) : read_item<true, true, false, T>(p, it, staged[warp]);
+        else full ? read_item<true, false, true, T>(p, it, staged[warp]) : read_item<true, false, false, T>(p, it, staged[warp]);
     } else {
-        if (p.c.l.k8) read_item<false, true, T>(p, it, staged[warp]);
-        else read_item<false, false, T>(p, it, staged[warp]);
+        if (p.c.l.k8) full ? read_item<false, true, true, T>(p, it, staged[warp]) : read_item<false, true, false, T>(p, it, staged[warp]);
+        else full ? read_item<false, false, true, T>(p, it, staged[warp]) : read_item<false, false, false, T>(p, it, staged[warp]);
     }
 }
 

@@ -87,10 +87,11 @@ __host__ __device__ constexpr uint32_t kv_word(uint32_t vec, uint32_t lane, uint
     return word * 4 / vec * 32 * vec + lane * vec + word * 4 % vec;
 }
 // Key codes: offset in the granule of the word(s) that hold dimensions 32 b + 8 t .. + 7 of position `at`.
-__host__ __device__ inline uint32_t kv_key_word(const KvLayout &l, uint32_t at, uint32_t b, uint32_t t, uint32_t second) {
-    const uint32_t tile = at / 8, lane = at % 8 * 4 + t;
-    return tile * (kv_code_bytes(l.width, l.k8) / 2) + kv_word(l.k_vec, lane, l.k8 ? 2 * b + second : b);
+// (`vec`: the layout's, which a caller that knows it to be 16 passes as that constant.)
+__host__ __device__ inline uint32_t kv_key_word(const KvLayout &l, uint32_t vec, uint32_t at, uint32_t b, uint32_t t, uint32_t second) {
+    return at / 8 * (l.k_scales / 2) + kv_word(vec, at % 8 * 4 + t, l.k8 ? 2 * b + second : b);
 }
+__host__ __device__ inline uint32_t kv_key_word(const KvLayout &l, uint32_t at, uint32_t b, uint32_t t, uint32_t second) { return kv_key_word(l, l.k_vec, at, b, t, second); }
 // Value codes: offset of the byte that holds dimension `dim` of position `at`; Q4_0: the high nibble if dim & 8.
 __host__ __device__ inline uint32_t kv_value_byte(const KvLayout &l, uint32_t at, uint32_t dim) {
     const uint32_t half = at / 8, t = at % 8 / 2, e = at % 2, lane = dim % 8 * 4 + t;
