@@ -796,7 +796,7 @@ int Backend::argmax(const Buffer &logits, size_t count, const Buffer &result) {
 // No reference analogue: see nu_cuda_token_logprobs in the header and logprobs.cu.
 int Backend::tokenLogprobs(const Buffer &logits, size_t rows, size_t count, size_t in_stride, const Buffer &tokens, const Buffer &logprobs, const Buffer &entropies, size_t k,
                            const Buffer *top, const Buffer *top_logprobs) {
-    if (rows == 0 || count == 0 || count > 0x7fffffffull || rows > (1u << 22) || in_stride < count || in_stride > (1ull << 40) || k > LOGPROB_ALTERNATIVES || k > count)
+    if (rows == 0 || count == 0 || count > (1u << 30) || rows > (1u << 22) || in_stride < count || in_stride > (1ull << 40) || k > LOGPROB_ALTERNATIVES || k > count)
         return fail(NU_ERR_INVALID_SHAPE, "token_logprobs: shape");
     if (k && (!top || !top_logprobs)) return fail(NU_ERR_INVALID_SHAPE, "token_logprobs: alternatives without a buffer for them");
     LogprobJob j{};

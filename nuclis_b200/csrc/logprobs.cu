@@ -7,7 +7,10 @@
 // by each warp on its own, so that no barrier stands in the loop: after its first 512 values the k-th largest of the lanes' maxima
 // bounds the k-th largest value from below, so only the few values above it become candidates (64-bit keys: the
 // value's order, then the lower index), and later only what passes the k-th candidate kept; the candidates are cut back to k when
-// eight more have come (each cut raises the bar, and what passes it costs the whole warp a look at its values). A row is cut over several blocks when there are few rows; the block that arrives last joins them in block order.
+// eight more have come (each cut raises the bar, and what passes it costs the whole warp a look at its values).
+//
+// The rounds of 4096 values of all rows are laid end to end and every block takes the same number of them, so that all end
+// together; a row that several blocks share is joined by the one that arrives last, in block order.
 #include "kernels.hpp"
 #include "launch.cuh"
 
@@ -17,22 +20,24 @@ namespace {
 
 constexpr int MAX_K = (int)LOGPROB_ALTERNATIVES;
 constexpr int THREADS = 256, WARPS = THREADS / 32, EACH = 16, ROUND = THREADS * EACH;
-constexpr int RESIDENT = 4;                 // blocks a multiprocessor: 64 registers a thread, for two rounds of values
+constexpr int RESIDENT = 3;                 // blocks a multiprocessor: 85 registers a thread, for two rounds of values
 constexpr int WARP_ROUND = 32 * EACH, CUT = 8, WARP_CANDIDATES = WARP_ROUND + MAX_K + CUT;  // a round on top of what is not yet cut back
 constexpr int CANDIDATES = WARPS * WARP_CANDIDATES;
-constexpr uint32_t SPLITS_MAX = 256;
+constexpr uint32_t PARTS_MAX = 128;         // blocks that share a row: what the joining block ranks
+static_assert(PARTS_MAX * MAX_K <= (uint32_t)CANDIDATES && PARTS_MAX <= (uint32_t)THREADS, "the joining block holds every part's candidates");
 constexpr int FEW = 256;                    // candidates that are ranked by counting
 constexpr int RECORD = 4 + 2 * MAX_K;       // floats a block leaves: m, Z, sum, bad, then the keys
 
 struct Params {
     LogprobJob j;
-    uint32_t splits, piece;  // blocks a row, logits a block
+    uint32_t rounds, share;  // rounds a row, rounds a block
 };
 
 __device__ __forceinline__ uint32_t order(float x) {  // larger floats have larger keys; both zeros the same
     const uint32_t b = __float_as_uint(x + 0.0f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+constexpr uint32_t LOWEST = 0x00800000u;  // the order of the lowest finite value (minus infinity's is one less)
 __device__ __forceinline__ float unorder(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 __device__ __forceinline__ unsigned long long key_of(uint32_t ord, uint32_t index) { return (unsigned long long)ord << 32 | (0xffffffffu - index); }
 
@@ -176,15 +181,21 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) token_logprobs_kernel(const
     extern __shared__ __align__(16) uint8_t raw[];
     Shared &sh = *(Shared *)raw;
     const LogprobJob &j = p.j;
-    const uint32_t tid = threadIdx.x, row = blockIdx.x / p.splits, split = blockIdx.x % p.splits, k = j.k;
-    wait_for_previous_operator();
-    const float *x = j.logits + (size_t)row * j.stride;
-    // a block's piece starts on a 16-byte boundary: the first also has the values ahead of it
-    const uint32_t ahead = (uint32_t)((16 - ((uintptr_t)x & 15)) & 15) / 4;
-    const uint32_t begin = split == 0 ? 0 : min(j.count, ahead + split * p.piece), end = split + 1 == p.splits ? j.count : min(j.count, ahead + (split + 1) * p.piece);
-    const uint32_t shift = split == 0 ? (4 - ahead) % 4 : 0;  // values of the first vector that lie before the row
-    const uint32_t lane = tid & 31, warp = tid / 32;
+    const uint32_t tid = threadIdx.x, k = j.k, lane = tid & 31, warp = tid / 32;
     unsigned long long *own = sh.candidates + warp * WARP_CANDIDATES;
+    wait_for_previous_operator();
+    const unsigned long long total = (unsigned long long)j.rows * p.rounds, last_round = min(total, (blockIdx.x + 1ull) * p.share);
+    for (unsigned long long at_round = (unsigned long long)blockIdx.x * p.share; at_round < last_round;) {
+    // this block's part of the row: rounds [r_begin, r_end); the row is that of blocks c0 .. c1
+    const uint32_t row = (uint32_t)(at_round / p.rounds), r_begin = (uint32_t)(at_round % p.rounds);
+    const uint32_t r_end = (uint32_t)min((unsigned long long)p.rounds, r_begin + (last_round - at_round));
+    const uint32_t c0 = (uint32_t)((unsigned long long)row * p.rounds / p.share), c1 = (uint32_t)(((unsigned long long)(row + 1) * p.rounds - 1) / p.share);
+    at_round += r_end - r_begin;
+    const float *x = j.logits + (size_t)row * j.stride;
+    // a part starts on a 16-byte boundary: the first also has the values ahead of it
+    const uint32_t ahead = (uint32_t)((16 - ((uintptr_t)x & 15)) & 15) / 4;
+    const uint32_t begin = r_begin == 0 ? 0 : min(j.count, ahead + r_begin * ROUND), end = r_end == p.rounds ? j.count : min(j.count, ahead + r_end * ROUND);
+    const uint32_t shift = r_begin == 0 ? (4 - ahead) % 4 : 0;  // values of the first vector that lie before the row
     if (lane == 0) sh.counts[warp] = 0;
     __syncwarp();
 
@@ -193,30 +204,27 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) token_logprobs_kernel(const
     const int n = (int)(end - begin + shift);  // of the piece, from the vector that holds its first value
     const float *v = x + begin - shift;
     auto load = [&](float (&to)[EACH], int r0) {
+        if (r0 >= n) return;
+        const float *src = v + r0 + (int)tid * 4;
+        if (r0 >= (int)shift && r0 + ROUND <= n) {
 #pragma unroll
-        for (int q = 0; q < EACH / 4; ++q) {
-            const int i = r0 + (q * THREADS + (int)tid) * 4;
-            if (i >= (int)shift && i + 4 <= n) {
-                const float4 f = __ldcs((const float4 *)(v + i));
+            for (int q = 0; q < EACH / 4; ++q) {
+                const float4 f = __ldcs((const float4 *)(src + q * THREADS * 4));
                 to[q * 4] = f.x; to[q * 4 + 1] = f.y; to[q * 4 + 2] = f.z; to[q * 4 + 3] = f.w;
-            } else {
+            }
+        } else {  // a part's first or last round
 #pragma unroll
-                for (int c = 0; c < 4; ++c) to[q * 4 + c] = i + c >= (int)shift && i + c < n ? v[i + c] : -INFINITY;
+            for (int i = 0; i < EACH; ++i) {
+                const int at = r0 + (i / 4 * THREADS + (int)tid) * 4 + i % 4;
+                to[i] = at >= (int)shift && at < n ? v[at] : -INFINITY;
             }
         }
     };
-    float next[EACH];  // the round after is on its way while one is worked on
-    load(next, 0);
-    for (int r0 = 0; r0 < n; r0 += ROUND) {
-        float a[EACH];
-#pragma unroll
-        for (int i = 0; i < EACH; ++i) a[i] = next[i];
-        if (r0 + ROUND < n) load(next, r0 + ROUND);
+    auto work = [&](const float (&a)[EACH], int r0) {
         float top = a[0];
-        bool nan = false;
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) { top = fmaxf(top, a[i]); nan |= a[i] != a[i]; }
-        if (nan || top == INFINITY) s.bad = 1;
+        for (int i = 1; i < EACH; ++i) top = fmaxf(top, a[i]);  // (a NaN shows in the sum)
+        if (top == INFINITY) s.bad = 1;
         if (top > s.m) s.raise(top);
         const float m = s.m == -INFINITY ? 0.0f : s.m;
 #pragma unroll
@@ -227,10 +235,10 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) token_logprobs_kernel(const
             s.z += e;
             s.w = fmaf(fmaxf(d, -1000.0f), e, s.w);  // the bound only meets terms whose e is zero
         }
-        if (k == 0) continue;
+        if (k == 0) return;
         const uint32_t mine = order(top);
         const uint32_t hopeful = __ballot_sync(0xffffffffu, mine > floor);
-        if (hopeful == 0) continue;
+        if (hopeful == 0) return;
         uint32_t bound = floor;
         if (__popc(hopeful) >= (int)k) {  // only what reaches the k-th largest of the lanes' maxima can be among the k largest
             uint32_t above = 0;  // lanes ahead of this one, equals by number
@@ -241,13 +249,27 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) token_logprobs_kernel(const
             }
             bound = max(floor, __reduce_max_sync(0xffffffffu, above == k - 1 ? mine - 1 : 0u));  // (an order is never zero)
         }
-        if (mine > bound) {
+        // which of the lane's values pass: compared as floats, unless minus infinities count too (the row has had fewer than k others)
+        uint32_t passed = 0;
+        if (bound >= LOWEST) {
+            const float limit = unorder(bound == 0x7fffffffu ? bound - 1 : bound);  // (just below zero is not minus zero, which equals it)
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) passed |= (uint32_t)(a[i] > limit) << i;
+        } else {
 #pragma unroll
             for (int i = 0; i < EACH; ++i) {
-                const int at = r0 + ((i / 4) * THREADS + (int)tid) * 4 + i % 4;
-                const uint32_t o = order(a[i]);
-                if (o > bound && at >= (int)shift && at < n) own[atomicAdd(&sh.counts[warp], 1u)] = key_of(o, begin + (uint32_t)at - shift);
+                const int at = r0 + (i / 4 * THREADS + (int)tid) * 4 + i % 4;
+                passed |= (uint32_t)(order(a[i]) > bound && at >= (int)shift && at < n) << i;
             }
+        }
+        while (passed) {  // few
+            const int i = __ffs(passed) - 1;
+            passed &= passed - 1;
+            const int at = r0 + (i / 4 * THREADS + (int)tid) * 4 + i % 4;
+            float x_i = a[0];
+#pragma unroll
+            for (int j = 1; j < EACH; ++j) x_i = j == i ? a[j] : x_i;
+            own[atomicAdd(&sh.counts[warp], 1u)] = key_of(order(x_i), begin + (uint32_t)at - shift);
         }
         __syncwarp();
         const uint32_t c = sh.counts[warp];
@@ -257,7 +279,18 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) token_logprobs_kernel(const
             floor = (uint32_t)(own[k - 1] >> 32);
         }
         __syncwarp();
+    };
+    float next[EACH];  // the round after is on its way while one is worked on
+    load(next, 0);
+#pragma unroll 1
+    for (int r0 = 0; r0 < n; r0 += ROUND) {
+        float a[EACH];
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) a[i] = next[i];
+        load(next, r0 + ROUND);
+        work(a, r0);
     }
+    if (s.z != s.z) s.bad = 1;
     if (k) {  // the warps' candidates together: what one has at most between cuts, or its k where that is too many to rank
         const uint32_t each = WARPS * (k + CUT) <= (uint32_t)FEW ? k + CUT : k;
         if (sh.counts[warp] > each) {
@@ -274,25 +307,27 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) token_logprobs_kernel(const
         select(sh, WARPS * each, k);
     }
     s = block_stats(sh, s);
-    if (p.splits == 1) {
+    if (c0 == c1) {
         write_row(j, sh, s, row);
-        return;
+        __syncthreads();
+        continue;
     }
 
     // ---- several blocks a row: the last one joins ----
-    float *records = j.partials + (size_t)row * p.splits * RECORD;
-    float *mine = records + (size_t)split * RECORD;
+    const uint32_t parts = c1 - c0 + 1;
+    auto record = [&](uint32_t c) { return j.partials + ((size_t)(c0 + c) * 2 + (c == 0)) * RECORD; };  // a block's second place: the row that starts in it
+    float *mine = record(blockIdx.x - c0);
     if (tid == 0) { mine[0] = s.m; mine[1] = s.z; mine[2] = s.w; mine[3] = __uint_as_float(s.bad); }
     if (tid < k) ((unsigned long long *)(mine + 4))[tid] = sh.kept[tid];
     __threadfence();
     __syncthreads();
-    if (tid == 0) sh.last = atomicAdd(j.counters + row, 1u) == p.splits - 1;
+    if (tid == 0) sh.last = atomicAdd(j.counters + c0, 1u) == parts - 1;
     __syncthreads();
-    if (!sh.last) return;
+    if (!sh.last) continue;  // (uniform; the next part's first barrier is behind this read)
     __threadfence();
     Stats all{-INFINITY, 0.0f, 0.0f, 0u};
-    if (tid < p.splits) {
-        const float *r = records + (size_t)tid * RECORD;
+    if (tid < parts) {
+        const float *r = record(tid);
         all = {__ldcg(r), __ldcg(r + 1), __ldcg(r + 2), __float_as_uint(__ldcg(r + 3))};
     }
     __syncthreads();
@@ -300,18 +335,18 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) token_logprobs_kernel(const
     if (k) {
         // the k-th largest of the pieces' first candidates bounds what can be among the k largest, as above
         uint32_t bound = 0;
-        sh.maxima[tid] = tid < p.splits ? (uint32_t)(__ldcg((const unsigned long long *)(records + (size_t)tid * RECORD + 4)) >> 32) : 0u;
+        sh.maxima[tid] = tid < parts ? (uint32_t)(__ldcg((const unsigned long long *)(record(tid) + 4)) >> 32) : 0u;
         if (tid == 0) { sh.bound = 0; sh.count = 0; }
         __syncthreads();
-        if (p.splits > k) {
+        if (parts > k) {
             uint32_t above = 0;
             for (uint32_t i = 0; i < THREADS; ++i) above += sh.maxima[i] > sh.maxima[tid] || (sh.maxima[i] == sh.maxima[tid] && i < tid);
             if (above == k - 1) sh.bound = sh.maxima[tid];
             __syncthreads();
             bound = sh.bound;
         }
-        for (uint32_t i = tid; i < p.splits * k; i += THREADS) {
-            const unsigned long long key = __ldcg((const unsigned long long *)(records + (size_t)(i / k) * RECORD + 4) + i % k);
+        for (uint32_t i = tid; i < parts * k; i += THREADS) {
+            const unsigned long long key = __ldcg((const unsigned long long *)(record(i / k) + 4) + i % k);
             if (key && (uint32_t)(key >> 32) >= bound) {
                 const uint32_t at = atomicAdd(&sh.count, 1u);
                 if (at < (uint32_t)CANDIDATES) sh.candidates[at] = key;
@@ -322,29 +357,20 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) token_logprobs_kernel(const
         select(sh, c, k);
     }
     write_row(j, sh, all, row);
-    if (tid == 0) j.counters[row] = 0;
+    if (tid == 0) j.counters[c0] = 0;
+    __syncthreads();
+    }
 }
 
 }  // namespace
 
 int launch_token_logprobs(cudaStream_t s, const LogprobJob &j) {
-    // Cuts of a row: the ones whose blocks fill whole waves best, a block's start and join counted as five rounds; never less than a
-    // round a block.
-    Params p{j, 1, j.count};
-    const uint32_t slots = (uint32_t)j.sm_count * RESIDENT, rounds = (j.count + ROUND - 1) / ROUND;
-    const uint32_t join = CANDIDATES / (j.k ? j.k : 1);  // the joining block holds every piece's candidates
-    uint32_t most = rounds < SPLITS_MAX ? rounds : SPLITS_MAX, splits = 1;
-    if (most > join) most = join;
-    unsigned long long best = ~0ull;
-    for (uint32_t c = 1; c <= most; ++c) {
-        const unsigned long long waves = ((unsigned long long)j.rows * c + slots - 1) / slots, cost = waves * ((rounds + c - 1) / c + 5) + (c > 1);
-        if (cost < best) { best = cost; splits = c; }
-    }
-    if (splits > 1 && j.rows <= j.counters_len && (size_t)j.rows * splits * RECORD <= j.partials_floats) {
-        p.piece = ((j.count + splits - 1) / splits + 3) / 4 * 4;
-        p.splits = (j.count + p.piece - 1) / p.piece;
-    }
-    launch_after_previous_smem(token_logprobs_kernel, dim3(j.rows * p.splits), dim3(THREADS), sizeof(Shared), s, p);
+    // A block for every place on the multiprocessors, less when there are fewer rounds; no row over more than PARTS_MAX blocks.
+    Params p{j, (j.count + ROUND - 1) / ROUND, 0};
+    const unsigned long long total = (unsigned long long)j.rows * p.rounds, slots = (unsigned long long)j.sm_count * RESIDENT;
+    const unsigned long long least = (p.rounds + PARTS_MAX - 2) / (PARTS_MAX - 1), even = (total + slots - 1) / slots;
+    p.share = (uint32_t)(even > least ? even : least);
+    launch_after_previous_smem(token_logprobs_kernel, dim3((unsigned)((total + p.share - 1) / p.share)), dim3(THREADS), sizeof(Shared), s, p);
     return 1;
 }
 
