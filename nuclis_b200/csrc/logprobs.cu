@@ -62,6 +62,7 @@ struct Shared {
     uint32_t maxima[THREADS];
     Stats stats[WARPS];
     uint32_t count, bound, last;
+    uint32_t bar;  // what the k-th value of some warp lies above: the others look no lower
 };
 
 __device__ __forceinline__ unsigned long long warp_max(unsigned long long v) {
@@ -197,7 +198,8 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) token_logprobs_kernel(const
     const uint32_t begin = r_begin == 0 ? 0 : min(j.count, ahead + r_begin * ROUND), end = r_end == p.rounds ? j.count : min(j.count, ahead + r_end * ROUND);
     const uint32_t shift = r_begin == 0 ? (4 - ahead) % 4 : 0;  // values of the first vector that lie before the row
     if (lane == 0) sh.counts[warp] = 0;
-    __syncwarp();
+    if (tid == 0) sh.bar = 0;
+    __syncthreads();
 
     Stats s{-INFINITY, 0.0f, 0.0f, 0u};
     uint32_t floor = 0;      // order of the k-th value this warp has kept: later equals have higher indexes and lose
@@ -236,10 +238,10 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) token_logprobs_kernel(const
             s.w = fmaf(fmaxf(d, -1000.0f), e, s.w);  // the bound only meets terms whose e is zero
         }
         if (k == 0) return;
-        const uint32_t mine = order(top);
-        const uint32_t hopeful = __ballot_sync(0xffffffffu, mine > floor);
+        const uint32_t mine = order(top), least = max(floor, *(volatile uint32_t *)&sh.bar);
+        const uint32_t hopeful = __ballot_sync(0xffffffffu, mine > least);
         if (hopeful == 0) return;
-        uint32_t bound = floor;
+        uint32_t bound = __reduce_max_sync(0xffffffffu, least);
         if (__popc(hopeful) >= (int)k) {  // only what reaches the k-th largest of the lanes' maxima can be among the k largest
             uint32_t above = 0;  // lanes ahead of this one, equals by number
 #pragma unroll
@@ -247,7 +249,7 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) token_logprobs_kernel(const
                 const uint32_t o = __shfl_sync(0xffffffffu, mine, i);
                 above += o > mine || (o == mine && i < (int)lane);
             }
-            bound = max(floor, __reduce_max_sync(0xffffffffu, above == k - 1 ? mine - 1 : 0u));  // (an order is never zero)
+            bound = max(bound, __reduce_max_sync(0xffffffffu, above == k - 1 ? mine - 1 : 0u));  // (an order is never zero)
         }
         // which of the lane's values pass: compared as floats, unless minus infinities count too (the row has had fewer than k others)
         uint32_t passed = 0;
@@ -275,8 +277,11 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) token_logprobs_kernel(const
         const uint32_t c = sh.counts[warp];
         if (c >= k && (floor == 0 || c > k + CUT)) {
             cut_back(own, c, k);
-            if (lane == 0) sh.counts[warp] = k;
             floor = (uint32_t)(own[k - 1] >> 32);
+            if (lane == 0) {
+                sh.counts[warp] = k;
+                atomicMax(&sh.bar, floor - 1);  // equals elsewhere may have lower indexes
+            }
         }
         __syncwarp();
     };
