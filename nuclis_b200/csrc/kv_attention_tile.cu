@@ -3,7 +3,7 @@
 // One block a multiprocessor walks its share of all (sequence, row tile, head) units, as the kernel for few rows does
 // (kv_attention.cu), in steps of 128 keys (64 at width 256). A unit's row tile is 256 query rows, two M = 128 tiles that share every key
 // step (one tile at width 256, whose accumulator alone takes half the tensor memory).
-//   * warps 8..15 decode: a step's keys and values become f16 in shared memory, in the 128-byte-swizzled K-major layout of
+//   * two of the last warps bring the step's scales near f16's upper end, warps 8..15 decode: a step's keys and values become f16 in shared memory, in the 128-byte-swizzled K-major layout of
 //     the tensor core: keys as rows of dimensions, values transposed as rows of positions. The dimensions of a key's eight
 //     stand in the order 0,4,1,5,2,6,3,7 that unpacking gives, and the queries are laid out alike.
 //   * warp 16 issues S = Q K^T and O += P V, in an order that keeps one tile's softmax under the other's products.
@@ -40,11 +40,9 @@ struct Tile {
     // Registers a thread, of the 96 x 640 that the block starts with
     static constexpr int SOFT_REGS = 136, PROD_REGS = 80, MMA_REGS = 48;
     static_assert(SOFT * SOFT_REGS + PROD * PROD_REGS + 4 * MMA_REGS <= (SOFT + PROD + 4) * 96, "more registers than the block has");
-    static constexpr int PARTS = 128 / KT;         // of the 128 threads that rate the scales, a key's
-    static constexpr int NBT = NB / PARTS;         // a key's blocks of a thread
     // shared memory
     static constexpr int Q_TILE = 128 * W * 2, Q = 0, K_BYTES = KT * W * 2, K = Q + QT * Q_TILE, V = K + 2 * K_BYTES, TABLE = V + 2 * K_BYTES;
-    static constexpr int NANS = TABLE + 6 * NB * KT * 2, EXCHANGE = NANS + 4 * 2 * 128, SMALL = EXCHANGE + 3 * 256 * 4, BARS = SMALL + 128, BYTES = BARS + 32 * 8 + 1024;
+    static constexpr int NANS = TABLE + 6 * NB * KT * 2, EXCHANGE = NANS + 4 * 128, SMALL = EXCHANGE + 3 * 256 * 4, BARS = SMALL + 128, BYTES = BARS + 32 * 8 + 1024;
     // tensor memory columns
     static constexpr int S_COLS = KT, O_COL = 2 * KT;
     static constexpr int PARTIAL = ROWS * (W + 2);
@@ -157,12 +155,6 @@ __device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::l
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 template <int ID, int N>
 __device__ __forceinline__ void named_barrier() { asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N) : "memory"); }
-// A barrier of the decoding warps that returns whether any of their threads says yes.
-__device__ __forceinline__ bool barrier_or(bool mine) {
-    uint32_t any;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 2, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(any) : "r"((uint32_t)mine) : "memory");
-    return any != 0;
-}
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 // The 16-byte chunk that eight dimensions 32 b + 8 t .. of a row are kept in: an order in which the lanes (g, t) of a tile of keys, eight at
 // a time, meet no bank twice.
@@ -193,17 +185,18 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
     __half *value_scales = (__half *)(smem + T::TABLE);             // [2][NB][KT] of a step
     __half *value_offsets = value_scales + 2 * NB * KT;             // [2][NB][KT]: what their codes' offset takes off
     __half *key_scales = value_offsets + 2 * NB * KT;               // [2][KT][NB]
-    uint8_t *nans = smem + T::NANS;                                 // [4][2][128]: blocks of a key's values with a NaN scale
+    uint8_t *nans = smem + T::NANS;                                 // [4][128]: blocks of a key's values with a NaN scale
     float *exchange = (float *)(smem + T::EXCHANGE);                // [2][256] row maxima and sums between the two halves of a row (width 256), [256] row scales
     float *row_scale = exchange + 512;
     int *exponents = (int *)(smem + T::SMALL);                      // [4][2] of a step's keys and values
-    uint32_t *largest = (uint32_t *)(smem + T::SMALL) + 8;          // [4][2] their largest scale's bits
+    uint32_t *largest = (uint32_t *)(smem + T::SMALL) + 8;          // [2][rating warp][keys, values] a step's largest scales, as bits
     uint32_t *any_nan = largest + 8;                                // [4]
     uint32_t *tmem_slot = any_nan + 4, *last = tmem_slot + 1;
     volatile uint32_t *abort_flag = last + 1;
+    uint32_t *rated_nan = last + 2;                                 // [2][rating warp]
     const uint32_t bars = smem_u32(smem + T::BARS);
     auto bar = [&](int i) { return bars + i * 8; };
-    constexpr int K_FULL = 0, K_EMPTY = 2, V_FULL = 4, V_EMPTY = 6, S_FULL = 8, P_FULL = 10, PV_DONE = 12, Q_FULL = 14;
+    constexpr int K_FULL = 0, K_EMPTY = 2, V_FULL = 4, V_EMPTY = 6, S_FULL = 8, P_FULL = 10, PV_DONE = 12, Q_FULL = 14, SCALES_FULL = 16, SCALES_EMPTY = 18;
     const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
 
     if (tid == 0) {
@@ -215,9 +208,10 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
             mbar_init(bar(S_FULL + i), 1);
             mbar_init(bar(P_FULL + i), T::SOFT / QT);
             mbar_init(bar(PV_DONE + i), 1);
+            mbar_init(bar(SCALES_FULL + i), 2);
+            mbar_init(bar(SCALES_EMPTY + i), T::PROD);
         }
         mbar_init(bar(Q_FULL), T::SOFT);
-        for (int i = 0; i < 8; ++i) largest[i] = 0;
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -447,7 +441,7 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                         const uint32_t k0 = (QT == 1 ? group * COLS : 0) + k * 32;
 #pragma unroll
                         for (int c = 0; c < 32; ++c)
-                            if (q16[c / 2] >> (c % 2 * 16) & 0xffffu) nan_blocks |= nans[ring * 256 + k0 + c] | nans[ring * 256 + 128 + k0 + c];
+                            if (q16[c / 2] >> (c % 2 * 16) & 0xffffu) nan_blocks |= nans[ring * 128 + k0 + c];
                     }
                 }
                 l += sum * power_of_two(-shift);
@@ -591,46 +585,32 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
         fence_before();
     } else if (warp < T::SOFT + T::PROD) {
         fewer_registers<T::PROD_REGS>();
-        // ---- decoding: a warp has one granule of a step of 128 keys, half a granule of one of 64. Keys: lane (g, t) its own vectors of a tile of
-        // eight; values: lane (half, words w, g) the four lanes' words of two neighbouring words, which are eight positions each of a dimension
-        // and (Q4_0) the one eight on. The first four warps' threads (key, part) rate the scales ----
-        const uint32_t t = tid - T::SOFT * 32, key = t % KT, part = t / KT, pw = warp - T::SOFT, g8 = lane / 4, t4 = lane % 4;
-        const bool rater = t < 128;
-        constexpr int TILES = KT / 64;                                          // of eight keys, of a warp
+        // ---- decoding: a warp has TILES tiles of eight keys of a step, and the values of as many positions. Keys: lane (g, t) its own
+        // vectors of a tile; values: lane (half, words w, g) the four lanes' words of two neighbouring words, which are eight positions each of a
+        // dimension and (Q4_0) the one eight on ----
+        const uint32_t pw = warp - T::SOFT, g8 = lane / 4, t4 = lane % 4;
+        constexpr int TILES = KT / 8 / T::PROD;
         constexpr int KVEC = L.k_vec, KWORDS = KVEC / 4;                        // words of a vector
         constexpr int KVECS = (K8 ? 2 : 1) * NB / KWORDS, KITEMS = TILES * KVECS;  // vectors of a tile; of a warp in a step
         constexpr int VVECS = W / (V8 ? 8 : 16) / 4;                            // vectors of a granule
-        constexpr int VTURN = 4 / TILES, VITEMS = VVECS < VTURN ? 1 : VVECS / VTURN;  // a half warp has every VTURN-th of them
+        constexpr int VTURN = 4 / TILES, VITEMS = VVECS < VTURN ? 1 : VVECS / VTURN;  // a half warp has every VTURN-th of a granule's
         const uint32_t half = lane / 16, vpair = lane / 8 % 2, vg = lane % 8;
-        const uint32_t wgran = TILES == 2 ? pw : pw / 2, v0 = TILES == 2 ? half : pw % 2 * 2 + half;
+        const uint32_t kgran = pw * TILES / 2, vgran = TILES == 4 ? pw * 2 + half : pw * TILES / 2, v0 = TILES == 4 ? 0 : TILES == 2 ? half : pw % 2 * 2 + half;
         const bool valued = VVECS >= VTURN || v0 < (uint32_t)VVECS;             // (one vector a granule: half a warp)
         uint32_t step = 0;
         while (walk.next(p, pl, sg)) {
             const uint32_t live_rows = sg.span.count * p.group;
-            const uint32_t first_row = sg.tile * ROWS, last_row = min(live_rows, first_row + ROWS) - 1;
-            const uint32_t first_pos = sg.span.first + first_row / p.group, high = sg.span.first + last_row / p.group;
-            const uint32_t low = p.window && first_pos >= p.window ? first_pos - p.window + 1 : 0;   // some row sees [low, high]
+            const uint32_t high = sg.span.first + (min(live_rows, sg.tile * ROWS + ROWS) - 1) / p.group;
             const uint8_t *base = kv_head(p.c, sg.span.slot, sg.head);
             const uint32_t last_granule = high / KV_GRANULE;  // what is behind it may lie past the slot's end: it is not read
-            uint32_t kw[KITEMS][KWORDS], vw[VITEMS][4][2], ks[T::NBT / 2], vs[T::NBT / 2];
-            auto load_scales = [&](uint32_t key0) {
-                if (!rater) return;
-                const uint32_t at = key0 + key;
-                const uint8_t *g = base + (size_t)(at / KV_GRANULE) * L.bytes + (at % KV_GRANULE * NB + part * T::NBT) * 2;
-                const bool in = at / KV_GRANULE <= last_granule;
-#pragma unroll
-                for (int i = 0; i < T::NBT / 2; ++i) {
-                    ks[i] = in ? *(const uint32_t *)(g + L.k_scales + i * 4) : 0u;
-                    vs[i] = in ? *(const uint32_t *)(g + L.v_scales + i * 4) : 0u;
-                }
-            };
+            uint32_t kw[KITEMS][KWORDS], vw[VITEMS][4][2];
             auto load_keys = [&](uint32_t key0) {
-                const uint32_t gran = key0 / KV_GRANULE + wgran;
-                const bool in = gran <= last_granule;
-                const uint8_t *g = base + (size_t)gran * L.bytes + (TILES == 2 ? 0 : pw % 2 * (L.k_scales / 2)) + lane * KVEC;
+                const uint32_t gran = key0 / KV_GRANULE + kgran;
+                const uint8_t *g = base + (size_t)gran * L.bytes + (TILES == 1 ? pw % 2 * (L.k_scales / 2) : 0) + lane * KVEC;
 #pragma unroll
                 for (int i = 0; i < KITEMS; ++i) {
-                    const uint8_t *src = g + i / KVECS * (L.k_scales / 2) + i % KVECS * 32 * KVEC;
+                    const uint8_t *src = g + i / KVECS / 2 * L.bytes + i / KVECS % 2 * (L.k_scales / 2) + i % KVECS * 32 * KVEC;
+                    const bool in = gran + i / KVECS / 2 <= last_granule;
                     if (KVEC == 16) {
                         const uint4 x = in ? __ldg((const uint4 *)src) : make_uint4(0u, 0u, 0u, 0u);
                         kw[i][0] = x.x; kw[i][1] = x.y; kw[i][KWORDS - 2] = x.z; kw[i][KWORDS - 1] = x.w;
@@ -641,7 +621,7 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                 }
             };
             auto load_values = [&](uint32_t key0) {
-                const uint32_t gran = key0 / KV_GRANULE + wgran;
+                const uint32_t gran = key0 / KV_GRANULE + vgran;
                 const bool in = gran <= last_granule && valued;
                 const uint8_t *g = base + (size_t)gran * L.bytes + L.v_codes + v0 * 512 + vg * 64 + vpair * 8;
 #pragma unroll
@@ -653,72 +633,18 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                     }
             };
             const uint32_t begin = (sg.first + sg.skip) * KT;
-            float dk[T::NBT], dv[T::NBT];
-            uint32_t nan_mask = 0;
-            // the scales of the step at key0 (global step `of`): what no row of the tile sees counts as zero; the largest of all sets the step's power of two
-            auto rate = [&](uint32_t key0, uint32_t of) {
-                if (!rater) return;
-                const bool seen = key0 + key >= low && key0 + key <= high;
-                float kmax = 0.0f, vmax = 0.0f;
-                nan_mask = 0;
-#pragma unroll
-                for (int b = 0; b < T::NBT; ++b) {
-                    dk[b] = seen ? __half2float(__ushort_as_half((unsigned short)(ks[b / 2] >> (b % 2 * 16)))) : 0.0f;
-                    dv[b] = seen ? __half2float(__ushort_as_half((unsigned short)(vs[b / 2] >> (b % 2 * 16)))) : 0.0f;
-                    if (dv[b] != dv[b]) {
-                        nan_mask |= 1u << (part * T::NBT + b);
-                        dv[b] = 0.0f;
-                    }
-                    kmax = fmaxf(kmax, fabsf(dk[b]));
-                    vmax = fmaxf(vmax, fabsf(dv[b]));
-                }
-                const uint32_t kbits = __reduce_max_sync(0xffffffffu, __float_as_uint(kmax)), vbits = __reduce_max_sync(0xffffffffu, __float_as_uint(vmax));
-                if (lane == 0) {
-                    atomicMax(largest + (of & 3u) * 2, kbits);
-                    atomicMax(largest + (of & 3u) * 2 + 1, vbits);
-                }
-                nans[(of & 3u) * 256 + part * 128 + key] = (uint8_t)nan_mask;
-                if (KT == 128) nans[(of & 3u) * 256 + 128 + key] = 0;
-            };
-            // behind the barrier that follows: the powers of two, and the scales times them
-            auto publish = [&](uint32_t of, bool nan) {
-                if (!rater) return;
-                const uint32_t ring = of & 3u;
-                const int xk = (int)max(largest[ring * 2] >> 23, 64u) - 127, xv = (int)max(largest[ring * 2 + 1] >> 23, 64u) - 127;
-                const float fk = power_of_two(14 - xk), fv = power_of_two(14 - xv);  // the largest scale to [2^14, 2^15)
-#pragma unroll
-                for (int b = 0; b < T::NBT; b += 2)
-                    *(__half2 *)(key_scales + ((of & 1u) * KT + key) * NB + part * T::NBT + b) = __floats2half2_rn(dk[b] * fk, dk[b + 1] * fk);
-#pragma unroll
-                for (int b = 0; b < T::NBT; ++b) {
-                    const float d = dv[b] * fv;
-                    value_scales[((of & 1u) * NB + part * T::NBT + b) * KT + key] = __float2half_rn(d);
-                    value_offsets[((of & 1u) * NB + part * T::NBT + b) * KT + key] = __float2half_rn(d * (V8 ? -128.0f / 16777216.0f : -8.0f / 16777216.0f));
-                }
-                if (t == 0) {
-                    exponents[ring * 2] = xk + 10;
-                    exponents[ring * 2 + 1] = xv + 10;
-                    any_nan[ring] = nan;
-                    largest[((of + 2) & 3u) * 2] = 0;  // next used two barriers on
-                    largest[((of + 2) & 3u) * 2 + 1] = 0;
-                }
-            };
-            load_scales(begin);
             load_keys(begin);
             load_values(begin);
-            rate(begin, step);
-            publish(step, barrier_or(nan_mask != 0));
-            named_barrier<2, 256>();
             for (uint32_t i = 0; i < sg.n; ++i, ++step) {
                 const uint32_t key0 = begin + i * KT, stage = step & 1u, parity = (step >> 1) & 1u;
                 const bool more = i + 1 < sg.n;
-                if (more) load_scales(key0 + KT);
                 // keys
+                wait_or_give_up(bar(SCALES_FULL + stage), parity, abort_flag);
                 if (step >= 2) wait_or_give_up(bar(K_EMPTY + stage), parity ^ 1u, abort_flag);
                 uint8_t *kt = smem + T::K + stage * T::K_BYTES;
 #pragma unroll
                 for (int j = 0; j < KITEMS; ++j) {
-                    const uint32_t row = pw * (KT / 8) + j / KVECS * 8 + g8, v = j % KVECS;
+                    const uint32_t row = (pw * TILES + j / KVECS) * 8 + g8, v = j % KVECS;
                     constexpr int BLOCKS = KWORDS / (K8 ? 2 : 1);
                     const uint32_t b0 = v * BLOCKS;
                     uint32_t pairs[BLOCKS / 2];
@@ -748,11 +674,7 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(K_FULL + stage));
-                if (more) {
-                    load_keys(key0 + KT);
-                    rate(key0 + KT, step + 1);
-                }
-                const bool nan = barrier_or(nan_mask != 0);  // the next step's scales are rated
+                if (more) load_keys(key0 + KT);
 
                 // values
                 if (step >= 2) wait_or_give_up(bar(V_EMPTY + stage), parity ^ 1u, abort_flag);
@@ -760,7 +682,7 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
 #pragma unroll
                 for (int j = 0; j < VITEMS; ++j) {
                     if (!valued) break;
-                    const uint32_t v = j * VTURN + v0, gran = wgran, word = v * 4 + vpair * 2, block = word / (V8 ? 4 : 2);
+                    const uint32_t v = j * VTURN + v0, gran = vgran, word = v * 4 + vpair * 2, block = word / (V8 ? 4 : 2);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {  // eight positions of the granule: 2t, 2t + 1 of every t
                         const uint4 d4 = *(const uint4 *)(value_scales + (stage * NB + block) * KT + gran * 16 + h * 8);
@@ -787,12 +709,11 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bar(V_FULL + stage));
-                if (more) {
-                    load_values(key0 + KT);
-                    publish(step + 1, nan);
-                    named_barrier<2, 256>();  // the next step's scales are there
+                if (lane == 0) {
+                    mbar_arrive(bar(V_FULL + stage));
+                    mbar_arrive(bar(SCALES_EMPTY + stage));
                 }
+                if (more) load_values(key0 + KT);
             }
         }
     } else {
@@ -842,6 +763,91 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                 if (QT == 2 && more) commit(bar(K_EMPTY + (next & 1u)));
             }
             ++segment;
+        }
+        // ---- the scales, by the next two warps, a step or two ahead of the decoding: a thread has KT / 64 keys. What no row of the tile
+        // sees counts as zero; the largest of all sets the step's power of two ----
+        if (warp == T::SOFT + T::PROD + 1 || warp == T::SOFT + T::PROD + 2) {
+            constexpr int KEYS = KT / 64;
+            const uint32_t rw = warp - (T::SOFT + T::PROD + 1), t = rw * 32 + lane;
+            while (walk.next(p, pl, sg)) {
+                const uint32_t live_rows = sg.span.count * p.group, first_row = sg.tile * ROWS;
+                const uint32_t first_pos = sg.span.first + first_row / p.group, high = sg.span.first + (min(live_rows, first_row + ROWS) - 1) / p.group;
+                const uint32_t low = p.window && first_pos >= p.window ? first_pos - p.window + 1 : 0;   // some row sees [low, high]
+                const uint8_t *head = kv_head(p.c, sg.span.slot, sg.head);
+                uint32_t ks[KEYS][NB / 2], vs[KEYS][NB / 2];
+                auto load = [&](uint32_t key0) {
+#pragma unroll
+                    for (int j = 0; j < KEYS; ++j) {
+                        const uint32_t at = key0 + t + j * 64;
+                        const bool seen = at >= low && at <= high;
+                        const uint8_t *g = head + (size_t)(at / KV_GRANULE) * L.bytes + at % KV_GRANULE * NB * 2;
+#pragma unroll
+                        for (int i = 0; i < NB / 2; ++i) {
+                            ks[j][i] = seen ? *(const uint32_t *)(g + L.k_scales + i * 4) : 0u;
+                            vs[j][i] = seen ? *(const uint32_t *)(g + L.v_scales + i * 4) : 0u;
+                        }
+                    }
+                };
+                const uint32_t begin = (sg.first + sg.skip) * KT;
+                load(begin);
+                for (uint32_t i = 0; i < sg.n; ++i, ++step) {
+                    const uint32_t stage = step & 1u, ring = step & 3u;
+                    __half2 kmax = __float2half2_rn(0.0f), vmax = kmax;  // (a NaN loses)
+                    uint32_t masks[KEYS], any = 0;
+#pragma unroll
+                    for (int j = 0; j < KEYS; ++j) {
+                        masks[j] = 0;
+#pragma unroll
+                        for (int k = 0; k < NB / 2; ++k) {
+                            const uint32_t x = vs[j][k];
+                            if ((x & 0x7fffu) > 0x7c00u) { masks[j] |= 1u << (2 * k); vs[j][k] &= 0xffff0000u; }
+                            if ((x >> 16 & 0x7fffu) > 0x7c00u) { masks[j] |= 2u << (2 * k); vs[j][k] &= 0x0000ffffu; }
+                            kmax = __hmax2(kmax, __habs2(as_h2(ks[j][k])));
+                            vmax = __hmax2(vmax, __habs2(as_h2(vs[j][k])));
+                        }
+                        any |= masks[j];
+                    }
+                    const float2 k2 = __half22float2(kmax), v2 = __half22float2(vmax);
+                    uint32_t kbits = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(k2.x, k2.y))), vbits = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(v2.x, v2.y)));
+                    any = __reduce_or_sync(0xffffffffu, any);
+                    if (lane == 0) {
+                        largest[stage * 4 + rw * 2] = kbits;
+                        largest[stage * 4 + rw * 2 + 1] = vbits;
+                        rated_nan[stage * 2 + rw] = any;
+                    }
+                    named_barrier<3, 64>();
+                    kbits = max(largest[stage * 4], largest[stage * 4 + 2]);
+                    vbits = max(largest[stage * 4 + 1], largest[stage * 4 + 3]);
+                    any = rated_nan[stage * 2] | rated_nan[stage * 2 + 1];
+                    const int xk = (int)max(kbits >> 23, 64u) - 127, xv = (int)max(vbits >> 23, 64u) - 127;
+                    const float fk = power_of_two(14 - xk), fv = power_of_two(14 - xv);  // the largest scale to [2^14, 2^15)
+                    // the tables of two steps ago have been read, and with them (the values' stage was free) that softmax's four steps ago
+                    if (step >= 2) wait_or_give_up(bar(SCALES_EMPTY + stage), ((step >> 1) & 1u) ^ 1u, abort_flag);
+#pragma unroll
+                    for (int j = 0; j < KEYS; ++j) {
+                        const uint32_t key = t + j * 64;
+                        nans[ring * 128 + key] = (uint8_t)masks[j];
+#pragma unroll
+                        for (int k = 0; k < NB / 2; ++k) {
+                            const float2 dk = __half22float2(as_h2(ks[j][k])), dv = __half22float2(as_h2(vs[j][k]));
+                            *(__half2 *)(key_scales + (stage * KT + key) * NB + 2 * k) = __floats2half2_rn(dk.x * fk, dk.y * fk);
+                            constexpr float OFFSET = (V8 ? -128.0f : -8.0f) / 16777216.0f;
+                            value_scales[(stage * NB + 2 * k) * KT + key] = __float2half_rn(dv.x * fv);
+                            value_scales[(stage * NB + 2 * k + 1) * KT + key] = __float2half_rn(dv.y * fv);
+                            value_offsets[(stage * NB + 2 * k) * KT + key] = __float2half_rn(dv.x * fv * OFFSET);
+                            value_offsets[(stage * NB + 2 * k + 1) * KT + key] = __float2half_rn(dv.y * fv * OFFSET);
+                        }
+                    }
+                    if (t == 0) {
+                        exponents[ring * 2] = xk + 10;
+                        exponents[ring * 2 + 1] = xv + 10;
+                        any_nan[ring] = any;
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(SCALES_FULL + stage));
+                    if (i + 1 < sg.n) load(begin + (i + 1) * KT);
+                }
+            }
         }
     }
     __syncwarp();
