@@ -856,9 +856,9 @@ int Backend::kvJob(const char *who, const Buffer &buffer, const nu_kv_cache &c, 
 }
 
 namespace {
-// Bytes from the first to the last of `rows` rows; 0 when the stride is too small or beyond all bounds.
+// Bytes from the first to the last of `rows` rows (2^32 at most); 0 when the stride is too small or beyond all bounds.
 size_t rowsBytes(size_t rows, size_t width, size_t stride, size_t element) {
-    if (stride < width || stride > (1ull << 40)) return 0;
+    if (stride < width || stride > (1ull << 40) || rows > (1ull << 60) / stride) return 0;
     return ((rows - 1) * stride + width) * element;
 }
 }  // namespace

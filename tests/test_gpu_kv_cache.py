@@ -7,6 +7,8 @@ score of width/32 blocks has that many F32 roundings on terms of its own size (8
 normal rows of 256: 5e-6 of a probability at worst, and of random sign), and a sum over n positions on the tensor cores truncates
 once per 16 positions and warp (n / 128 x 2^-23: below 1e-6 for the lengths here). To BF16 the rounding comes on top: half a step, 2^-8 of
 the value."""
+import threading
+
 import numpy as np
 import pytest
 
@@ -410,6 +412,103 @@ def test_the_values_of_one_sequence_may_grow(backend):
         assert rel_l2(attend(b, held, cache, shape, [(0, 999, 1)], 1, q, 4), want) <= 1e-5
 
 
+@pytest.mark.parametrize("width", [64, 128, 256])
+def test_a_unit_of_many_blocks(backend, width):
+    """One head over a long cache: its steps go to most of the device's blocks, and one joins more than 32 parts."""
+    b = backend
+    length, rows = 20001, 130
+    shape = KvCache(1, 20016, 1, width, enc.Q4_0, enc.Q8_0)
+    with Held(b) as held:
+        cache, k, v, rng = case(b, held, shape, [length], 31)
+        q = rng.standard_normal((rows, 1, width)).astype(np.float32)
+        spans = [(0, length - rows, rows)]
+        want = kv_oracle.attention(q, k[0], v[0], length - rows, 1)
+        assert rel_l2(attend(b, held, cache, shape, spans, rows, q, 1), want) <= 1e-5
+        assert rel_l2(attend(b, held, cache, shape, spans, rows, q, 1, dtype=enc.BF16), want) <= 2.0 ** -8
+        one = attend(b, held, cache, shape, [(0, length - 1, 1)], 1, q[-1:], 1)
+        assert rel_l2(one, want[-1:]) <= 1e-5
+
+
+@pytest.mark.parametrize("window", [0, 200])
+@pytest.mark.parametrize("width", [64, 128, 256])
+def test_more_units_than_blocks(backend, width, window):
+    """A prompt whose units outnumber the device's blocks for either kernel, so that blocks take several whole ones."""
+    b = backend
+    heads, group, rows = 8, 4, 1300
+    shape = KvCache(1, 1312, heads, width, enc.Q8_0, enc.Q4_0)
+    with Held(b) as held:
+        cache, k, v, rng = case(b, held, shape, [rows], 32)
+        q = rng.standard_normal((rows, heads * group, width)).astype(np.float32)
+        want = kv_oracle.attention(q, k[0], v[0], 0, group, window=window)
+        spans = [(0, 0, rows)]
+        assert rel_l2(attend(b, held, cache, shape, spans, rows, q, heads * group, window=window), want) <= 1e-5
+        assert rel_l2(attend(b, held, cache, shape, spans, rows, q, heads * group, window=window, dtype=enc.BF16), want) <= 2.0 ** -8
+
+
+def test_graphs_that_join_in_one_scratch(backend):
+    """Two recordings whose calls all leave partial results in the handle's scratch, launched in turn: each result is the first one's, bit for bit."""
+    b = backend
+    shape = KvCache(2, 4096, 2, 128, enc.Q8_0, enc.Q8_0)
+    with Held(b) as held:
+        cache, k, v, rng = case(b, held, shape, [4000, 2500], 33)
+        graphs = []
+        for rows, dtype, n in ((1, 0, 4000), (70, enc.BF16, 2500)):
+            q = held.up(rng.standard_normal(rows * 4 * 128).astype(np.float32))
+            out = held.new(rows * 4 * 128 * (4 if dtype == 0 else 2))
+            sp = held.up(kv_spans([(0, n - rows, rows), (1, 2500 - rows, rows)][: 2 if rows == 70 else 1]))
+            count = 2 if rows == 70 else 1
+            if count == 2:
+                q, out = held.up(np.tile(q.floats(), 2)), held.new(2 * out.len)
+            logits, tokens, logp = held.up(rng.standard_normal((3, 200001)).astype(np.float32)), held.up(np.array([5, 200000, 77], np.uint32)), held.new(12)
+            entropies = held.new(12)
+            b.begin()
+            b.attention(cache, shape, sp, count, rows, q, 512, 4, out, 512, out_dtype=dtype)
+            b.token_logprobs(logits, 3, 200001, 200001, tokens, logp, entropies)
+            graphs.append((b.commit_retain(), out, logp))
+        first = []
+        for g, out, logp in graphs:
+            b.graph_launch(g)
+            first.append((out.read(np.uint16).copy(), logp.read(np.uint32).copy()))
+        for _ in range(5):
+            for g, out, logp in graphs:
+                b.graph_launch(g, 3)
+            for (g, out, logp), (a, l) in zip(graphs, first):
+                np.testing.assert_array_equal(out.read(np.uint16), a)
+                np.testing.assert_array_equal(logp.read(np.uint32), l)
+        for g in graphs:
+            b.graph_release(g[0])
+
+
+def test_two_handles_at_once(backend):
+    """A handle a thread, each with its own stream and scratch: the results are those of one alone."""
+    shape = KvCache(1, 4096, 2, 128, enc.Q8_0, enc.Q8_0)
+
+    def work(b, seed, turns, results):
+        with Held(b) as held:
+            cache, k, v, rng = case(b, held, shape, [3000], seed)
+            q = rng.standard_normal((40, 4, 128)).astype(np.float32)
+            for _ in range(turns):
+                results.append(attend(b, held, cache, shape, [(0, 2960, 40)], 40, q, 4, dtype=enc.BF16))
+                results.append(attend(b, held, cache, shape, [(0, 2999, 1)], 1, q[-1:], 4))
+            want = kv_oracle.attention(q, k[0], v[0], 2960, 2)
+            assert rel_l2(results[0], want) <= 2.0 ** -8 and rel_l2(results[1], want[-1:]) <= 1e-5
+
+    other = Backend(0)
+    try:
+        results = [[], []]
+        threads = [threading.Thread(target=work, args=(b, 40 + i, 20, results[i])) for i, b in enumerate((backend, other))]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        for r in results:
+            assert len(r) == 40
+            for i in range(2, 40):
+                np.testing.assert_array_equal(r[i], r[i % 2])
+    finally:
+        other.deinit()
+
+
 @pytest.mark.parametrize("width", [64, 128, 256, 96])
 def test_a_recorded_step_follows_its_spans(backend, width):
     """One recording of write + attention, replayed token by token with the spans buffer moved on; a second graph in between."""
@@ -484,6 +583,22 @@ def test_a_cache_beyond_32_bits(backend):
         out = attend(b, held, cache, shape, [(1, (1 << 20) - 1, 1)], 1, q, 40, window=290)
         want = kv_oracle.attention(q, kv_oracle.stored(k, enc.Q8_0)[10:], kv_oracle.stored(v, enc.Q8_0)[10:], 289, 5)
         assert rel_l2(out, want) <= 1e-5
+
+
+def test_rows_whose_bytes_pass_64_bits_are_refused(backend):
+    """97 x 172,961 rows are 2^24 + 1: at a stride of 2^40 the last one's offset is 2^64 elements."""
+    b = backend
+    with Held(b) as held:
+        shape = KvCache(1, 32, 1, 64)
+        cache, sp, rows = held.new(shape.bytes), held.up(kv_spans([(0, 0, 1)] * 97)), held.new(4096)
+        for call in (lambda: b.kv_write(cache, shape, sp, 97, 172961, rows, 1 << 40, rows, 1 << 40),
+                     lambda: b.kv_read(cache, shape, sp, 97, 172961, rows.slice(0, 1024), 1 << 40, rows.slice(2048, 1024), 1 << 40),
+                     lambda: b.attention(cache, shape, sp, 97, 172961, rows.slice(0, 1024), 1 << 40, 1, rows.slice(2048, 1024), 1 << 40)):
+            b.begin()
+            with pytest.raises(NuclisError) as e:
+                call()
+            assert e.value.name == "InvalidShape"
+            b.discard()
 
 
 def test_refusals(backend):
