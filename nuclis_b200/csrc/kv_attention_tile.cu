@@ -3,9 +3,11 @@
 // One block a multiprocessor walks its share of all (sequence, row tile, head) units, as the kernel for few rows does
 // (kv_attention.cu), in steps of 128 keys (64 at width 256). A unit's row tile is 256 query rows, two M = 128 tiles that share every key
 // step (one tile at width 256, whose accumulator alone takes half the tensor memory).
-//   * two of the last warps bring the step's scales near f16's upper end, warps 8..15 decode: a step's keys and values become f16 in shared memory, in the 128-byte-swizzled K-major layout of
+//   * warps 8..15 decode: a step's keys and values become f16 in shared memory, in the 128-byte-swizzled K-major layout of
 //     the tensor core: keys as rows of dimensions, values transposed as rows of positions. The dimensions of a key's eight
-//     stand in the order 0,4,1,5,2,6,3,7 that unpacking gives, and the queries are laid out alike.
+//     stand in the order 0,4,1,5,2,6,3,7 that unpacking gives, and the queries are laid out alike. Two more warps bring the
+//     scales of the next step near f16's upper end meanwhile (done by the decoding warps themselves, with a barrier before and after,
+//     387 rows at position 24,100 took 338 us instead of 267).
 //   * warp 16 issues S = Q K^T and O += P V, in an order that keeps one tile's softmax under the other's products.
 //   * warps 0..7 are the softmax: a thread has a row; it reads S from tensor memory, writes P = 2^(S scale - m) as f16 over it, and
 //     the tensor core takes P from there. The maximum m is only moved when a score passes it by 8 (log2), so O is rarely rescaled.
@@ -17,6 +19,12 @@
 //
 // A value's scale that is NaN would reach rows that do not see its position (0 * NaN), so it is decoded as zeros and marked, and
 // the rows that do see it write NaN in its block's dimensions.
+//
+// Bound by the work on both sides of the tensor core, not by memory: at width 256 a step of 64 keys costs the decoding warps more than its
+// products take; at width 128 a softmax warp spends 3,300 cycles on 128 keys, of which the exponentials are a third and reading S from
+// tensor memory twice most of the rest (its 128 columns do not fit in registers beside eight decoding warps). Measured: 387 rows
+// of 20 heads on 4 (width 256) at position 24,100 267 us, 709 TFLOP/s; a prompt of 2,048 rows, 40 heads on 8 of width 128, 117 us, 366 TFLOP/s over
+// the causal half.
 //
 // Every wait is bounded: a thread whose wait runs out raises the block's flag, all waits then fall through, and the block
 // ends as ever with the status word raised.
@@ -225,7 +233,7 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
     const uint32_t tmem = *tmem_slot;
     wait_for_previous_operator();
 
-    const Plan pl = plan<ROWS, KT, T::SEGMENT, 2>(p);
+    const Plan pl = plan<ROWS, KT, T::SEGMENT, 2, 1>(p);
     Walk<ROWS, KT, T::SEGMENT> walk(pl);
     Segment sg;
 
@@ -883,9 +891,13 @@ bool attention_tile_configure() {
     return ok;
 }
 
+// From 128 query rows a key/value head. Below, the kernel for few rows is the faster one unless the context is very long, and its time grows with the
+// rows; here it hardly does. Measured (it / this one, us; Q8_0 keys, Q4_0 values, 8 heads of width 128): at position 700 64 rows
+// 17 / 42, 128 rows 19 / 43, 256 rows 21 / 45; at 8,000 41 / 73, 66 / 74, 107 / 76; at 60,000 180 / 171, 342 / 172, 666 / 175. Width 256, 4
+// heads: 8,000 40 / 83, 67 / 86, 104 / 86; 60,000 173 / 180, 321 / 182, 612 / 164. (The positions are only known on the device.)
 bool attention_tile_supported(const AttentionJob &j) {
     const uint32_t w = j.cache.width;
-    return j.bf16 && (w == 64 || w == 128 || w == 256) && (uint64_t)j.tokens * (j.heads / j.cache.heads) >= 64;
+    return j.bf16 && (w == 64 || w == 128 || w == 256) && (uint64_t)j.tokens * (j.heads / j.cache.heads) >= 128;
 }
 
 int launch_attention_tile(cudaStream_t s, const AttentionJob &j, AttentionParams p) {

@@ -6,6 +6,10 @@
 // The stored scale is d rounded to f16. A block whose scale rounds to zero stores zeros; one whose scale passes the f16
 // range stores the largest scale and saturated codes; one that holds a NaN or an infinity stores a NaN scale, so that it
 // reads back as NaN and cannot pass for data.
+//
+// Measured (8 heads of width 128, against a copy's 6.46 TB/s): 65,536 rows of Q4_0 read to BF16 66 us, 5.2 TB/s; 4,096 rows written as
+// Q8_0 / Q4_0 and read back to F32 23 us, 3.4 TB/s, of which the write waits for its own instructions more than for memory; one row
+// written and read back 6.3 us, which is two launches and two chains of dependent loads.
 #include <cuda_bf16.h>
 
 #include "kernels.hpp"
@@ -109,7 +113,7 @@ __device__ __forceinline__ void transpose_bytes(uint32_t a, uint32_t b, uint32_t
 constexpr int KV_WARPS = KV_THREADS / 32;
 
 // FULL: the piece has 128 dimensions and the codes lie in vectors of 16 bytes (widths of whole 128s), so that every place is a
-// matter of shifts.
+// matter of shifts (65,536 rows of width 128 read: 94 us without, 66 with it; 4,096 written and read 38 and 24).
 // The second half of writing values: the rows' codes in `words` ([position][lane], four a word) become the cache's words.
 template <bool Q8, bool FULL>
 __device__ __forceinline__ void transpose_item(const KvLayout &l, const Item &it, uint8_t *g, uint32_t (&words)[512]) {
