@@ -345,6 +345,31 @@ def test_a_batch_of_unlike_sequences(backend, width):
                 assert np.all(got[s, count:].view(np.uint32) == UNTOUCHED.view(np.uint32)), s  # padding rows are left as they were
 
 
+@pytest.mark.parametrize("count,rows,dtype", [(300, 2, 0), (45, 64, enc.BF16), (150, 9, 0)])
+@pytest.mark.parametrize("width", [64, 128, 256])
+def test_many_sequences(backend, width, count, rows, dtype):
+    """More sequences than a warp has lanes, a third of them absent, their lengths from one position to hundreds, on slots in no order."""
+    b = backend
+    group = 2
+    rng = np.random.default_rng(count + width)
+    lengths = rng.integers(1, 40000 // count, count)
+    shape = KvCache(count, (40000 // count + 15) // 16 * 16, 2, width, enc.Q4_0, enc.Q8_0)
+    with Held(b) as held:
+        cache, k, v, rng = case(b, held, shape, [int(n) for n in lengths], 50)
+        q = rng.standard_normal((count * rows, 2 * group, width)).astype(np.float32)
+        spans = []
+        for slot in rng.permutation(count):
+            n = int(min(rng.integers(1, rows + 1), lengths[slot]))
+            spans.append((int(slot), int(lengths[slot]) - n, 0 if slot % 3 == 0 else n))
+        got = attend(b, held, cache, shape, spans, rows, q, 2 * group, dtype=dtype).reshape(count, rows, 2 * group, width)
+        untouched = UNTOUCHED.view(np.uint32) if dtype == 0 else 0xc1c10000
+        for s, (slot, first, n) in enumerate(spans):
+            if n:
+                want = kv_oracle.attention(q[s * rows: s * rows + n], k[slot], v[slot], first, group)
+                assert rel_l2(got[s, :n], want) <= (1e-5 if dtype == 0 else 2.0 ** -8), s
+            assert np.all(got[s, n:].view(np.uint32) == untouched), s
+
+
 @pytest.mark.parametrize("kenc,venc", PAIRS[:2])
 @pytest.mark.parametrize("width", [64, 128, 256, 160])
 def test_what_a_row_does_not_see_may_hold_anything(backend, width, kenc, venc):
