@@ -345,6 +345,34 @@ def test_a_batch_of_unlike_sequences(backend, width):
                 assert np.all(got[s, count:].view(np.uint32) == UNTOUCHED.view(np.uint32)), s  # padding rows are left as they were
 
 
+@pytest.mark.parametrize("pad,at", [(1, 0), (24, 1), (8, 8)])
+@pytest.mark.parametrize("dtype,length,rows", [(0, 500, 3), (0, 9000, 1), (enc.BF16, 500, 3), (enc.BF16, 300, 90), (enc.BF16, 9000, 70)])
+@pytest.mark.parametrize("width", [64, 128, 256, 96])
+def test_output_rows_apart(backend, width, dtype, length, rows, pad, at):
+    """A stride beyond the row, and rows that start anywhere: the same values, and nothing between or around them is written."""
+    b = backend
+    heads, size = 4, 4 if dtype == 0 else 2
+    n = heads * width
+    shape = KvCache(1, 9008, 2, width, enc.Q8_0, enc.Q8_0)
+    with Held(b) as held:
+        cache, k, v, rng = case(b, held, shape, [length], 60)
+        q = rng.standard_normal((rows, heads, width)).astype(np.float32)
+        spans = [(0, length - rows, rows)]
+        plain = attend(b, held, cache, shape, spans, rows, q, heads, dtype=dtype)
+        word = np.uint32 if dtype == 0 else np.uint16
+        out = held.up(np.full((rows + 1) * (n + pad) + at, 0xc1c1, word))
+        qb, sp = held.up(q), held.up(kv_spans(spans))
+        b.begin()
+        b.attention(cache, shape, sp, 1, rows, qb, n, heads, out.slice(at * size, out.len - at * size), n + pad, out_dtype=dtype)
+        b.commit()
+        got = out.read(word)
+        assert np.all(got[:at] == 0xc1c1) and np.all(got[at + rows * (n + pad):] == 0xc1c1)
+        got = got[at: at + rows * (n + pad)].reshape(rows, n + pad)
+        assert np.all(got[:, n:] == 0xc1c1)
+        bits = plain.view(np.uint32) if dtype == 0 else (plain.view(np.uint32) >> 16).astype(np.uint16)
+        np.testing.assert_array_equal(got[:, :n], bits.reshape(rows, n))
+
+
 @pytest.mark.parametrize("count,rows,dtype", [(300, 2, 0), (45, 64, enc.BF16), (150, 9, 0)])
 @pytest.mark.parametrize("width", [64, 128, 256])
 def test_many_sequences(backend, width, count, rows, dtype):
