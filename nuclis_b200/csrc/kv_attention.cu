@@ -29,7 +29,7 @@
 // Bound by fixed latencies more than by memory: a granule takes about 500 instructions, and a thread's accumulators leave room for four warps
 // a scheduler, which keep its issue slots 55 % busy. Measured (Q4_0, 40 query heads on 8 of width 128, one row): position 131,072 68 us,
 // 2.2 TB/s; position 700 14.5 us, launch, plan, one stage and join. Six rows (30 a head: four tiles of eight, each unpacks the cache
-// again) over 20,000 positions of Q8_0 at width 256 48 us. 24 sequences at width 64 under a window 32 us, 2.0 TB/s.
+// again) over 20,000 positions of Q8_0 at width 256 49 us. 24 sequences at width 64 under a window 33 us, 2.0 TB/s.
 //
 // generic_kernel: one warp per query row and head, any width up to 512; also what generic_only selects.
 #include <type_traits>

@@ -147,15 +147,13 @@ __device__ __forceinline__ Plan plan(const AttentionParams &p) {
     if (p.sequences == 1 && units > blocks) {
         const uint32_t n = (uint32_t)units, rounds = (n + blocks - 1) / blocks;
         uint32_t longest = 0;
-        if (rounds <= 8)
-            for (uint32_t b = lane; b < blocks; b += 32) {
-                uint32_t load = 0;
-                for (uint32_t j = 0; j < rounds; ++j) {
-                    const uint32_t u = j * blocks + (j & 1u ? blocks - 1 - b : b);
-                    if (u < n) load += steps((n - 1 - u) / heads) + SEGMENT;
-                }
-                longest = max(longest, load);
+        if (rounds <= 8) {  // 32 blocks stand for all: their neighbours' units are as long to a step, but for the last round's end (all: 4 us more)
+            const uint32_t rest = n - (rounds - 1) * blocks - 1, b = lane == 0 ? ((rounds - 1) & 1u ? blocks - 1 - rest : rest) : lane * blocks / 32;
+            for (uint32_t j = 0; j < rounds; ++j) {
+                const uint32_t u = j * blocks + (j & 1u ? blocks - 1 - b : b);
+                if (u < n) longest += steps((n - 1 - u) / heads) + SEGMENT;
             }
+        }
         r.whole = __reduce_max_sync(0xffffffffu, longest) <= r.share + SEGMENT;
         if (r.whole) {
             r.in = n;
