@@ -13,8 +13,8 @@
 //     the tensor core takes P from there. The maximum m is only moved when a score passes it by 8 (log2), so O is rarely rescaled.
 //
 // Range: a step's keys and values are brought into f16's range by a power of two each (their largest scale's), a row's query
-// by one of its own; the score's factor takes the first and last back, P that of the values relative to the largest so far. So f16's
-// 11 bits hold for every magnitude a cache can store; products are exact and sums F32. Against 64 bits the result is off by
+// by one of its own; the score's factor takes the first and last back, O carries the values'. Where that moves by more than P has room for, O is
+// multiplied by the power of two between them, up or down, so P's bits do not depend on what the values of other steps are. Products are exact and sums F32. Against 64 bits the result is off by
 // its own BF16 rounding and little else (1.7e-3 relative).
 //
 // A value's scale that is NaN would reach rows that do not see its position (0 * NaN), so it is decoded as zeros and marked, and
@@ -54,6 +54,11 @@ struct Tile {
     // tensor memory columns
     static constexpr int S_COLS = KT, O_COL = 2 * KT;
     static constexpr int PARTIAL = ROWS * (W + 2);
+    // P is kept 2^P_UP above the probabilities (at most 2^8 before a maximum moves), so that it ends below 2^15. O carries the exponent of a
+    // step's values; a step whose values' lies up to SPREAD below takes P down by that (a probability of one keeps 11 bits down to 2^-14, so a SPREAD of
+    // 12 leaves those of 2^-9 all of theirs), any other moves O's exponent to its own, up or down. O is at most 2^31 positions of 2^15 times a value in
+    // f16, and the exponents are 40 apart at most, so F32 holds it.
+    static constexpr int P_UP = 7, SPREAD = 12, NO_VALUES = -1000;  // NO_VALUES: a step of zeros
     static constexpr uint32_t SEGMENT = 6;         // steps that a block decodes in the time that a second segment costs it
 };
 
@@ -363,13 +368,14 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                     top = fmaxf(top, exchange[(step & 1u) * 256 + (tid ^ 128u)]);
                 }
                 bool waited = i == 0;
+                const int own = ev == T::NO_VALUES ? big : ev;  // a step of zeros goes with any exponent
                 if (i == 0) {
                     m = top;
-                    big = ev;
-                } else if (__any_sync(0xffffffffu, top > m + 8.0f) || ev > big) {
+                    big = own;
+                } else if (__any_sync(0xffffffffu, top > m + 8.0f) || own > big || own < big - T::SPREAD) {
                     const float next = fmaxf(m, top), fl = m == -INFINITY ? 0.0f : exp2_approx(m - next);
-                    const int next_big = max(big, ev);
-                    const float f = fl * power_of_two(max(big - next_big, -126));
+                    const int next_big = own;
+                    const float f = fl * power_of_two(big - next_big);
                     m = next;
                     l *= fl;
                     big = next_big;
@@ -387,7 +393,7 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                     }
                     tmem_store_wait();
                 }
-                const int shift = max(ev - big, -100);
+                const int shift = (ev == T::NO_VALUES ? 0 : ev - big) + T::P_UP;
                 const float offset = (float)shift - (m == -INFINITY ? 0.0f : m);
                 const uint64_t factor2 = two(factor, factor), offset2 = two(offset, offset);
                 uint64_t sums[4] = {0, 0, 0, 0};
@@ -472,7 +478,7 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                 named_barrier<1, 256>();
             }
             const bool whole = sg.n == sg.count;
-            const float up = power_of_two(max(min(big, 127), -126)) * (whole ? 1.0f / l : 1.0f);
+            const float up = power_of_two(big - T::P_UP) * (whole ? 1.0f / l : 1.0f);
             float *partial = p.partials + ((size_t)blockIdx.x * 2 + (sg.skip == 0)) * T::PARTIAL;  // a unit that starts here goes into the second place
             const uint32_t dim0 = QT == 2 ? 0 : group * OCOLS;
 #pragma unroll 1
@@ -848,7 +854,7 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                     }
                     if (t == 0) {
                         exponents[ring * 2] = xk + 10;
-                        exponents[ring * 2 + 1] = xv + 10;
+                        exponents[ring * 2 + 1] = vbits ? xv + 10 : T::NO_VALUES;
                         any_nan[ring] = any;
                     }
                     __syncwarp();

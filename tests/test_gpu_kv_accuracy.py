@@ -1,0 +1,80 @@
+"""Attention over the quantized cache on data that is not unit normal: positions whose values dwarf the others', one key that holds
+nearly all the weight, queries and keys with a mean, channels that set their block's scale, long sums of one sign.
+
+Bounds. To BF16 a result is rounded by at most half a step, 2^-8 of the value; the 16-bit operands of a call of many rows are rounded
+to 11 bits each (2^-12 of random sign on average: together below 1e-3 of the result), so relative L2 stays within 2^-8, whose root mean square over a binade is
+1.7e-3. To F32 the library's bound for F32 accumulation holds, relative L2 1e-5."""
+import numpy as np
+import pytest
+
+import kv_oracle
+from nuclis_b200 import KvCache, encoding as enc
+from parity import rel_l2
+from test_gpu_kv_cache import Held, attend, backend, write  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def one_key_and_one_value(width, length, rows, dominant, large, ratio, seed):
+    """q, k, v of one head: the key at `dominant` holds some 95 % of every row's weight, that at `large` next to none, whose values are
+    `ratio` times the others'."""
+    rng = np.random.default_rng(seed)
+    u = rng.standard_normal(width)
+    u /= np.linalg.norm(u)
+    gain = np.sqrt((np.log(length) + 3.5) * np.sqrt(width))  # q . k / sqrt(width) of the two along u
+    k, v, q = (rng.standard_normal((n, 1, width)) for n in (length, length, rows))
+    k -= (k @ u)[..., None] * u
+    q -= (q @ u)[..., None] * u
+    q += gain * u
+    k[dominant] += gain * u
+    k[large] -= gain * u
+    v *= 2.0 ** -6
+    v[large] *= ratio
+    return (x.astype(np.float32) for x in (q, k, v))
+
+
+@pytest.mark.parametrize("ratio", [2 ** 7, 2 ** 10, 2 ** 12, 2 ** 20])
+@pytest.mark.parametrize("venc", [enc.Q8_0, enc.Q4_0])
+@pytest.mark.parametrize("width", [64, 128, 256])
+def test_large_values_ahead_of_those_that_count(backend, width, venc, ratio):
+    """The probabilities of later steps keep their bits, whatever the values of an earlier one were."""
+    b = backend
+    length, rows = 4096, 140
+    shape = KvCache(1, length, 1, width, enc.Q8_0, venc)
+    q, k, v = one_key_and_one_value(width, length, rows, 3000, 100, ratio, 5)
+    with Held(b) as held:
+        cache = held.new(shape.bytes)
+        write(b, held, cache, shape, [(0, 0, length)], length, k, v)
+        want = kv_oracle.attention(q, kv_oracle.stored(k, enc.Q8_0), kv_oracle.stored(v, venc), length - rows, 1)
+        spans = [(0, length - rows, rows)]
+        assert rel_l2(attend(b, held, cache, shape, spans, rows, q, 1, dtype=enc.BF16), want) <= 2.0 ** -8
+        assert rel_l2(attend(b, held, cache, shape, spans, rows, q, 1), want) <= 1e-5
+
+
+@pytest.mark.parametrize("venc", [enc.Q8_0, enc.Q4_0])
+@pytest.mark.parametrize("width", [64, 128, 256])
+def test_steps_of_zeros_and_of_alternating_sizes(backend, width, venc):
+    """Values that are zero for a while (a cache written in part), then tiny, then large, step by step: their exponent moves both ways.
+    Row by row within half a step of BF16, and f16's end: a probability times 2^7 and the power of two of its step's values over the largest so far is
+    rounded by at most 2^-25 where it is next to zero, so a position adds at most 2^-32 max|v|, of random sign, and the norm of a row's result
+    is off by sqrt(length) x 2^-32 max|v| sqrt(width). It shows in the rows that look at a position of zeros: all they hold is the share of the others,
+    whose probabilities are near e^-20."""
+    b = backend
+    length, rows = 2000, 140
+    shape = KvCache(1, length, 1, width, enc.Q8_0, venc)
+    rng = np.random.default_rng(9)
+    k, v = (rng.standard_normal((length, 1, width)).astype(np.float32) for _ in range(2))
+    v[:300] = 0
+    step = np.arange(length) // 128
+    v[300:] *= np.where(step % 3 == 0, 2.0 ** -8, np.where(step % 3 == 1, 1.0, 2.0 ** 6))[300:, None, None].astype(np.float32)
+    v[900:1300] = 0
+    q = rng.standard_normal((rows, 1, width)).astype(np.float32)
+    q[::2] = 4 * k[rng.integers(300, 1800, rows // 2)]  # every other row looks at one position
+    with Held(b) as held:
+        cache = held.new(shape.bytes)
+        write(b, held, cache, shape, [(0, 0, length)], length, k, v)
+        want = kv_oracle.attention(q, kv_oracle.stored(k, enc.Q8_0), kv_oracle.stored(v, venc), length - rows, 1)
+        got = attend(b, held, cache, shape, [(0, length - rows, rows)], rows, q, 1, dtype=enc.BF16)
+        assert np.all(np.isfinite(got))
+        lost = np.sqrt(length) * 2.0 ** -32 * np.abs(v).max() * np.sqrt(width)
+        assert np.all(np.linalg.norm(got - want, axis=-1) <= 2.0 ** -8 * np.linalg.norm(want, axis=-1) + lost)
