@@ -50,15 +50,18 @@ struct Tile {
     static_assert(SOFT * SOFT_REGS + PROD * PROD_REGS + 4 * MMA_REGS <= (SOFT + PROD + 4) * 96, "more registers than the block has");
     // shared memory
     static constexpr int Q_TILE = 128 * W * 2, Q = 0, K_BYTES = KT * W * 2, K = Q + QT * Q_TILE, V = K + 2 * K_BYTES, TABLE = V + 2 * K_BYTES;
-    static constexpr int NANS = TABLE + 6 * NB * KT * 2, EXCHANGE = NANS + 4 * 128, SMALL = EXCHANGE + 3 * 256 * 4, BARS = SMALL + 128, BYTES = BARS + 32 * 8 + 1024;
+    static constexpr int NANS = TABLE + 4 * NB * KT * 2, EXCHANGE = NANS + 4 * 128, SMALL = EXCHANGE + 3 * 256 * 4, BARS = SMALL + 128, BYTES = BARS + 32 * 8 + 1024;
     // tensor memory columns
     static constexpr int S_COLS = KT, O_COL = 2 * KT;
     static constexpr int PARTIAL = ROWS * (W + 2);
     // P is kept 2^P_UP above the probabilities (at most 2^8 before a maximum moves), so that it ends below 2^15. O carries the exponent of a
     // step's values; a step whose values' lies up to SPREAD below takes P down by that (a probability of one keeps 11 bits down to 2^-14, so a SPREAD of
-    // 12 leaves those of 2^-9 all of theirs), any other moves O's exponent to its own, up or down. O is at most 2^31 positions of 2^15 times a value in
-    // f16, and the exponents are 40 apart at most, so F32 holds it.
+    // 12 leaves those of 2^-9 all of theirs), any other moves O's exponent to its own, up or down. O is at most 2^31 positions of 2^15 times a value
+    // below 2^16, and the exponents are 40 apart at most, so F32 holds it.
     static constexpr int P_UP = 7, SPREAD = 12, NO_VALUES = -1000;  // NO_VALUES: a step of zeros
+    // The largest scale of a step goes to [2^TOP, 2^(TOP+1)), so that times the largest code it just ends in f16 (65,504). A value keeps f16's 11 bits down to 2^-29 of the
+    // largest value of its step, and all to 2^-40 of it.
+    static constexpr int K_TOP = K8 ? 8 : 12, V_TOP = V8 ? 8 : 12;
     static constexpr uint32_t SEGMENT = 6;         // steps that a block decodes in the time that a second segment costs it
 };
 
@@ -176,17 +179,8 @@ __host__ __device__ constexpr uint32_t chunk_of(uint32_t b, uint32_t t) { return
 __device__ __forceinline__ uint32_t swizzled(uint32_t rows, uint32_t row, uint32_t chunk) {
     return chunk / 8 * rows * 128 + row / 8 * 1024 + row % 8 * 128 + ((chunk % 8) ^ (row % 8)) * 16;
 }
-// A code without sign, left where it lies in its word, is the f16 code * 2^-24 (16 times that from a high nibble): times 2^24 of
-// the scale, less the offset's share, is the value in one operation. All of it is kept 2^24 / (the largest scale's power of two) up.
-__device__ __forceinline__ uint32_t value2(uint32_t codes, uint32_t d, uint32_t c) { return h2(__hfma2(as_h2(codes), as_h2(d), as_h2(c))); }
-template <bool Q8>
-struct Scale {  // of a block, twice
-    uint32_t low, high, offset;
-    __device__ __forceinline__ explicit Scale(uint32_t d) : low(d) {
-        high = Q8 ? d : h2(__hmul2(as_h2(d), __float2half2_rn(0.0625f)));
-        offset = h2(__hmul2(as_h2(d), __float2half2_rn(Q8 ? -128.0f / 16777216.0f : -8.0f / 16777216.0f)));
-    }
-};
+// Two codes with their sign, exact in f16, times their scales: a value is rounded once.
+__device__ __forceinline__ uint32_t value2(uint32_t codes, uint32_t d) { return h2(__hmul2(as_h2(codes), as_h2(d))); }
 
 template <int W, bool K8, bool V8>
 __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const __grid_constant__ AttentionParams p) {
@@ -196,8 +190,7 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + ((0u - smem_u32(smem_raw)) & 1023u);  // (an offset, so that the pointer stays one to shared memory)
     __half *value_scales = (__half *)(smem + T::TABLE);             // [2][NB][KT] of a step
-    __half *value_offsets = value_scales + 2 * NB * KT;             // [2][NB][KT]: what their codes' offset takes off
-    __half *key_scales = value_offsets + 2 * NB * KT;               // [2][KT][NB]
+    __half *key_scales = value_scales + 2 * NB * KT;                // [2][KT][NB]
     uint8_t *nans = smem + T::NANS;                                 // [4][128]: blocks of a key's values with a NaN scale
     float *exchange = (float *)(smem + T::EXCHANGE);                // [2][256] row maxima and sums between the two halves of a row (width 256), [256] row scales
     float *row_scale = exchange + 512;
@@ -252,7 +245,7 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
         const uint32_t ocol = tmem + lanes + T::O_COL + (QT == 2 ? q * W : group * OCOLS);
         uint32_t step = 0;  // over all segments
         while (walk.next(p, pl, sg)) {
-            // the queries: a row's largest value is brought to [1, 2) by a power of two
+            // the queries: a row's largest value is brought to [2^14, 2^15) by a power of two (or 2^126 times its own)
             const uint32_t live_rows = sg.span.count * p.group, tile_row0 = sg.tile * ROWS;
             const size_t rows0 = (size_t)sg.sequence * p.tokens;
             {
@@ -296,7 +289,7 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                         for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(x[i][k]) & 0x7fffffffu);
 #pragma unroll
                         for (uint32_t o = 1; o < LPR; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-                        const int e = top == 0 ? 0 : min((int)max(top >> 23, 1u) - 127, 126);
+                        const int e = top == 0 ? 0 : min(max((int)(top >> 23) - 127 - 14, -126), 126);
                         const bool bad = top >= 0x7f800000u;
                         const float down = power_of_two(-e);
                         if (chunk == 0) row_scale[r] = bad ? NAN : p.scale * power_of_two(e);
@@ -611,6 +604,8 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
         const uint32_t half = lane / 16, vpair = lane / 8 % 2, vg = lane % 8;
         const uint32_t kgran = pw * TILES / 2, vgran = TILES == 4 ? pw * 2 + half : pw * TILES / 2, v0 = TILES == 4 ? 0 : TILES == 2 ? half : pw % 2 * 2 + half;
         const bool valued = VVECS >= VTURN || v0 < (uint32_t)VVECS;             // (one vector a granule: half a warp)
+        uint32_t k1024 = 0x64006400u;
+        asm volatile("" : "+r"(k1024));
         uint32_t step = 0;
         while (walk.next(p, pl, sg)) {
             const uint32_t live_rows = sg.span.count * p.group;
@@ -671,16 +666,15 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                     }
 #pragma unroll
                     for (int b = 0; b < BLOCKS; ++b) {
-                        const Scale<K8> d(__byte_perm(pairs[b / 2], 0u, b % 2 ? 0x3232 : 0x1010));
+                        const uint32_t d = __byte_perm(pairs[b / 2], 0u, b % 2 ? 0x3232 : 0x1010);
                         uint4 x;
                         if (K8) {
                             const uint32_t w0 = kw[j][2 * b % KWORDS], w1 = kw[j][(2 * b + 1) % KWORDS];
-                            x = make_uint4(value2(__byte_perm(w0, 0u, 0x4140), d.low, d.offset), value2(__byte_perm(w0, 0u, 0x4342), d.low, d.offset),
-                                           value2(__byte_perm(w1, 0u, 0x4140), d.low, d.offset), value2(__byte_perm(w1, 0u, 0x4342), d.low, d.offset));
+                            x = make_uint4(value2(byte_codes(w0, 0x4140), d), value2(byte_codes(w0, 0x4342), d), value2(byte_codes(w1, 0x4140), d),
+                                           value2(byte_codes(w1, 0x4342), d));
                         } else {
                             const uint32_t w = kw[j][b], w8 = w >> 8;
-                            x = make_uint4(value2(w & 0x000f000fu, d.low, d.offset), value2(w & 0x00f000f0u, d.high, d.offset), value2(w8 & 0x000f000fu, d.low, d.offset),
-                                           value2(w8 & 0x00f000f0u, d.high, d.offset));
+                            x = make_uint4(value2(low_codes(w, k1024), d), value2(high_codes(w, k1024), d), value2(low_codes(w8, k1024), d), value2(high_codes(w8, k1024), d));
                         }
                         *(uint4 *)(kt + swizzled(KT, row, chunk_of(b0 + b, t4))) = x;
                     }
@@ -700,8 +694,7 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {  // eight positions of the granule: 2t, 2t + 1 of every t
                         const uint4 d4 = *(const uint4 *)(value_scales + (stage * NB + block) * KT + gran * 16 + h * 8);
-                        const uint4 c4 = *(const uint4 *)(value_offsets + (stage * NB + block) * KT + gran * 16 + h * 8);
-                        const uint32_t d[4] = {d4.x, d4.y, d4.z, d4.w}, c[4] = {c4.x, c4.y, c4.z, c4.w};
+                        const uint32_t d[4] = {d4.x, d4.y, d4.z, d4.w};
 #pragma unroll
                         for (int w = 0; w < 2; ++w) {
                             uint32_t x[4], y[4];  // a dimension's eight positions; Q4_0: the dimension eight on
@@ -709,10 +702,11 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                             for (int tt = 0; tt < 4; ++tt) {
                                 const uint32_t z = vw[j][tt][w];
                                 if (V8) {
-                                    x[tt] = value2(__byte_perm(z, 0u, h ? 0x4342 : 0x4140), d[tt], c[tt]);
+                                    x[tt] = value2(byte_codes(z, h ? 0x4342 : 0x4140), d[tt]);
                                 } else {
-                                    x[tt] = value2((h ? z >> 8 : z) & 0x000f000fu, d[tt], c[tt]);
-                                    y[tt] = value2((h ? z >> 12 : z >> 4) & 0x000f000fu, d[tt], c[tt]);
+                                    const uint32_t z8 = h ? z >> 8 : z;
+                                    x[tt] = value2(low_codes(z8, k1024), d[tt]);
+                                    y[tt] = value2(high_codes(z8, k1024), d[tt]);
                                 }
                             }
                             const uint32_t dim = (word + w) * (V8 ? 8 : 16) + vg;
@@ -834,7 +828,7 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                     vbits = max(largest[stage * 4 + 1], largest[stage * 4 + 3]);
                     any = rated_nan[stage * 2] | rated_nan[stage * 2 + 1];
                     const int xk = (int)max(kbits >> 23, 64u) - 127, xv = (int)max(vbits >> 23, 64u) - 127;
-                    const float fk = power_of_two(14 - xk), fv = power_of_two(14 - xv);  // the largest scale to [2^14, 2^15)
+                    const float fk = power_of_two(T::K_TOP - xk), fv = power_of_two(T::V_TOP - xv);
                     // the tables of two steps ago have been read, and with them (the values' stage was free) that softmax's four steps ago
                     if (step >= 2) wait_or_give_up(bar(SCALES_EMPTY + stage), ((step >> 1) & 1u) ^ 1u, abort_flag);
 #pragma unroll
@@ -845,16 +839,13 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                         for (int k = 0; k < NB / 2; ++k) {
                             const float2 dk = __half22float2(as_h2(ks[j][k])), dv = __half22float2(as_h2(vs[j][k]));
                             *(__half2 *)(key_scales + (stage * KT + key) * NB + 2 * k) = __floats2half2_rn(dk.x * fk, dk.y * fk);
-                            constexpr float OFFSET = (V8 ? -128.0f : -8.0f) / 16777216.0f;
                             value_scales[(stage * NB + 2 * k) * KT + key] = __float2half_rn(dv.x * fv);
                             value_scales[(stage * NB + 2 * k + 1) * KT + key] = __float2half_rn(dv.y * fv);
-                            value_offsets[(stage * NB + 2 * k) * KT + key] = __float2half_rn(dv.x * fv * OFFSET);
-                            value_offsets[(stage * NB + 2 * k + 1) * KT + key] = __float2half_rn(dv.y * fv * OFFSET);
                         }
                     }
                     if (t == 0) {
-                        exponents[ring * 2] = xk + 10;
-                        exponents[ring * 2 + 1] = vbits ? xv + 10 : T::NO_VALUES;
+                        exponents[ring * 2] = xk - T::K_TOP;
+                        exponents[ring * 2 + 1] = vbits ? xv - T::V_TOP : T::NO_VALUES;
                         any_nan[ring] = any;
                     }
                     __syncwarp();

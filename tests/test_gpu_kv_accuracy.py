@@ -10,7 +10,7 @@ import pytest
 import kv_oracle
 from nuclis_b200 import KvCache, encoding as enc
 from parity import rel_l2
-from test_gpu_kv_cache import Held, attend, backend, write  # noqa: F401
+from test_gpu_kv_cache import Held, PAIRS, attend, backend, write  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -49,6 +49,27 @@ def test_large_values_ahead_of_those_that_count(backend, width, venc, ratio):
         spans = [(0, length - rows, rows)]
         assert rel_l2(attend(b, held, cache, shape, spans, rows, q, 1, dtype=enc.BF16), want) <= 2.0 ** -8
         assert rel_l2(attend(b, held, cache, shape, spans, rows, q, 1), want) <= 1e-5
+
+
+@pytest.mark.parametrize("ratio", [2 ** 7, 2 ** 12, 2 ** 16, 2 ** 20])
+@pytest.mark.parametrize("kenc,venc", PAIRS)
+@pytest.mark.parametrize("width", [64, 128, 256])
+def test_large_values_beside_those_that_count(backend, width, kenc, venc, ratio):
+    """The same with both positions in one step of either kernel: the values keep their bits beside larger ones. To F32 a position's product of
+    probability and scale has its halves' end, 2^-36 of the largest value beside it, of random sign over the positions."""
+    b = backend
+    length, rows = 700, 140
+    shape = KvCache(1, 704, 1, width, kenc, venc)
+    q, k, v = one_key_and_one_value(width, length, rows, 129, 130, ratio, 6)
+    with Held(b) as held:
+        cache = held.new(shape.bytes)
+        write(b, held, cache, shape, [(0, 0, length)], length, k, v)
+        want = kv_oracle.attention(q, kv_oracle.stored(k, kenc), kv_oracle.stored(v, venc), length - rows, 1)
+        spans = [(0, length - rows, rows)]
+        assert rel_l2(attend(b, held, cache, shape, spans, rows, q, 1, dtype=enc.BF16), want) <= 2.0 ** -8
+        got = attend(b, held, cache, shape, spans, rows, q, 1)
+        lost = np.sqrt(length) * 2.0 ** -36 * np.abs(v).max() * np.sqrt(want.size)
+        assert np.linalg.norm(got - want) <= 1e-5 * np.linalg.norm(want) + lost
 
 
 @pytest.mark.parametrize("venc", [enc.Q8_0, enc.Q4_0])
