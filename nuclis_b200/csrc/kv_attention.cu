@@ -9,13 +9,11 @@
 //     to the codes. What is not exact in f16, the query and the probabilities, is split: x = hi + lo with both in
 //     f16 (22 bits). The 16 rows of the A operand are the hi parts of eight query rows and their lo parts, so the split
 //     costs no second instruction, and the two sums of a row come out in the same thread.
-//   * q . k = sum_b d_b (q_b . c_b): one accumulator pair of instructions per block of 32, then F32 FMAs with d_b. Four-bit codes
-//     get their sign on the way (two operations a pair). Eight-bit key codes are left without sign where they lie in their word: as
-//     f16 that is code * 2^-24, a subnormal number, so a pair costs one permute; the offset of 128 comes off the
-//     sum instead, sum_b d_b * sum(q_b): one more product with the scales as they lie. It is as large as the sums themselves, so
-//     nothing is lost. (Four-bit codes left like that lose the product's low bits: it is aligned by the subnormal's exponent,
-//     under which they have six leading zeros more; the result was off by 1.9e-6 instead of 3e-7. And the values' sums
-//     run over the positions, where the offset's share would grow with their number.)
+//   * q . k = sum_b d_b (q_b . c_b): one accumulator pair of instructions per block of 32, then F32 FMAs with d_b. Codes
+//     get their sign on the way (two operations a pair), so that the sums are no larger than the scores. (Eight-bit key codes can stay as they lie, with the
+//     share of their offset of 128, sum_b d_b * sum(q_b), taken off afterwards: an operation a pair less and no faster, six rows at 20,000 positions
+//     49 us either way. Where a block's queries do not cancel and one channel sets the scale, the offset's share is many times the score:
+//     the result was off by up to 9e-5.)
 //   * p v = sum_j (p_j d_jb) c_j: the scale goes into the probability, once per block, before it is split. The products
 //     p d are kept near 2^11 by a power of two per warp (`bias`), lowered when a larger scale comes by: f16's range is no limit,
 //     and what is lost of a position is below 2^-36 of the largest value seen.
@@ -190,7 +188,7 @@ struct Split {
     static constexpr int JOIN = WARPS * ROWS * W * 4;  // the warps' accumulators; takes the ring's place
     static constexpr int BUFFER = WARPS * STAGES * STAGE > JOIN ? WARPS * STAGES * STAGE : JOIN;
     static constexpr int FRAGMENTS = KT * 512;
-    static constexpr int SMEM = BUFFER + FRAGMENTS + 256 + WARPS * STAGES * 8 + (WARPS * 2 + 1) * ROWS * 4 + 64;
+    static constexpr int SMEM = BUFFER + FRAGMENTS + WARPS * STAGES * 8 + (WARPS * 2 + 1) * ROWS * 4 + 64;
     static constexpr int PARTIAL = ROWS * (W + 2);
     // A second segment costs a block about 6 us of prologue and join; the bytes that its warps read in that time.
     static constexpr uint32_t SEGMENT = 96 * 1024 / L.bytes;
@@ -207,8 +205,7 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
     uint8_t *ring = smem;
     float *join = (float *)smem;
     uint4 *fragments = (uint4 *)(smem + S::BUFFER);                     // [KT][32]
-    __half *block_sums = (__half *)(smem + S::BUFFER + S::FRAGMENTS);   // [hi, lo][ROWS][8]: sums of a row's blocks, for the offset
-    uint64_t *bars = (uint64_t *)(smem + S::BUFFER + S::FRAGMENTS + 256);  // [WARPS][STAGES]
+    uint64_t *bars = (uint64_t *)(smem + S::BUFFER + S::FRAGMENTS);     // [WARPS][STAGES]
     float *join_m = (float *)(bars + WARPS * STAGES);                   // [WARPS][ROWS]
     float *join_l = join_m + WARPS * ROWS;                              // [WARPS][ROWS]
     float *row_scale = join_l + WARPS * ROWS;                           // [ROWS]
@@ -270,21 +267,9 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
             // 2^e: from the exponent's bits; rows of zeros and of subnormal values count as 2^-126
             const int e = (int)max(top >> 23, 1u) - 127;
             const float down = top >= 0x7f800000u ? NAN : scalbnf(1.0f, -e);
-            if (lane == 0) row_scale[r] = scalbnf(p.scale, e - 13 + (K8 ? 24 : 0));  // the query's power of two, and the codes'
-            float sum = 0.0f;
+            if (lane == 0) row_scale[r] = scalbnf(p.scale, e - 13);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[i] = x[i] * down * 8192.0f;
-                sum += x[i];
-            }
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            if (lane % 4 == 0) {  // at most 32 * 2^14 * 2^-5
-                const float y = sum * 0.03125f;
-                const __half hi = __float2half_rn(y);
-                block_sums[r * 8 + lane / 4] = hi;
-                block_sums[(ROWS + r) * 8 + lane / 4] = __float2half_rn(y - __half2float(hi));
-            }
+            for (int i = 0; i < 8; ++i) x[i] = x[i] * down * 8192.0f;
             if (lane < (uint32_t)W / 8) {
                 const uint32_t b = lane / 4, tt = lane % 4;
                 uint32_t hi[4], lo[4];
@@ -306,7 +291,6 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
         const uint32_t tile_low = p.window && first_pos >= p.window ? first_pos - p.window + 1 : 0;   // some row sees [tile_low, tile_high]
         const uint32_t all_low = p.window && tile_high >= p.window ? tile_high - p.window + 1 : 0;    // every live row sees [all_low, first_pos]
         const float my_scale = row_scale[g];
-        const uint4 sums = make_uint4(((const uint32_t *)block_sums)[lane], ((const uint32_t *)block_sums)[ROWS * 4 + lane], 0u, 0u);
         uint32_t k1024 = 0x64006400u;
         asm volatile("" : "+r"(k1024));
 
@@ -343,14 +327,6 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
                     load_words<K8 ? 2 * NB : NB, L.k_vec>(gran + j % 2 * (L.k_scales / 2), lane, codes[j]);
                     load_scales<NB>(gran + L.k_scales, j % 2 * 8 + 2 * t, scales[j]);
                     s[j][0] = s[j][1] = 0.0f;
-                    if (K8) {  // what the codes' offset takes off: sum_b d_b * 128 * sum(q_b), in units of 2^-24; the sums carry 2^-5
-                        float c[4];
-                        const uint32_t pair = 2 * t < NB ? *(const uint32_t *)(gran + L.k_scales + ((j % 2 * 8 + g) * NB + 2 * t) * 2) : 0u;
-                        mma_zero(c, sums, pair, 0u);
-                        constexpr float OFFSET = -128.0f * 32.0f / 16777216.0f;
-                        s[j][0] = (c[0] + c[2]) * OFFSET;
-                        s[j][1] = (c[1] + c[3]) * OFFSET;
-                    }
                 }
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
@@ -359,8 +335,8 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
                     for (int j = 0; j < SG * 2; ++j) {
                         float c[4];
                         if (K8) {
-                            mma_zero(c, q0, __byte_perm(codes[j][2 * b], 0u, 0x4140), __byte_perm(codes[j][2 * b], 0u, 0x4342));
-                            mma(c, q1, __byte_perm(codes[j][2 * b + 1], 0u, 0x4140), __byte_perm(codes[j][2 * b + 1], 0u, 0x4342));
+                            mma_zero(c, q0, byte_codes(codes[j][2 * b], 0x4140), byte_codes(codes[j][2 * b], 0x4342));
+                            mma(c, q1, byte_codes(codes[j][2 * b + 1], 0x4140), byte_codes(codes[j][2 * b + 1], 0x4342));
                         } else {
                             const uint32_t w = codes[j][b], w8 = w >> 8;
                             mma_zero(c, q0, low_codes(w, k1024), high_codes(w, k1024));

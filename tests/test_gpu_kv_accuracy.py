@@ -99,3 +99,24 @@ def test_steps_of_zeros_and_of_alternating_sizes(backend, width, venc):
         assert np.all(np.isfinite(got))
         lost = np.sqrt(length) * 2.0 ** -32 * np.abs(v).max() * np.sqrt(width)
         assert np.all(np.linalg.norm(got - want, axis=-1) <= 2.0 ** -8 * np.linalg.norm(want, axis=-1) + lost)
+
+
+@pytest.mark.parametrize("width", [64, 128, 256])
+def test_queries_with_a_mean_and_keys_with_large_channels(backend, width):
+    """What projections write: a channel in each block of the keys sets its scale, the other codes lie near zero, and a block's queries
+    do not cancel. The scores are far smaller than what an offset of the codes would contribute."""
+    b = backend
+    length, rows, group = 4000, 3, 2
+    shape = KvCache(1, length, 1, width, enc.Q8_0, enc.Q8_0)
+    rng = np.random.default_rng(width)
+    k, v = (rng.standard_normal((length, 1, width)) for _ in range(2))
+    k *= 0.3
+    k[..., 5::32] += 60
+    q = rng.standard_normal((rows, group, width)) + 2
+    q[..., 5::32] *= 0.02
+    q, k, v = (x.astype(np.float32) for x in (q, k, v))
+    with Held(b) as held:
+        cache = held.new(shape.bytes)
+        write(b, held, cache, shape, [(0, 0, length)], length, k, v)
+        want = kv_oracle.attention(q, kv_oracle.stored(k, enc.Q8_0), kv_oracle.stored(v, enc.Q8_0), length - rows, group)
+        assert rel_l2(attend(b, held, cache, shape, [(0, length - rows, rows)], rows, q, group), want) <= 1e-5
