@@ -17,6 +17,9 @@
 //   * p v = sum_j (p_j d_jb) c_j: the scale goes into the probability, once per block, before it is split. The products
 //     p d are kept near 2^11 by a power of two per warp (`bias`), lowered when a larger scale comes by: f16's range is no limit,
 //     and what is lost of a position is below 2^-36 of the largest value seen.
+//   * A tensor core's sum is cut off, not rounded, at each step (about 2^-24 of it, always towards zero: a unit of 100,000 positions in one block was
+//     up to 9e-5 off), so a warp adds its accumulators up elsewhere, rounded, every 64 products: 592 rows at 100,000 positions, width 256, 4,604 us
+//     without and 4,667 with it (5,079 every 32, with the place of the sums kept in registers).
 //   * The running maximum of a row is only raised when a score passes it by 3 (in log2): the accumulators are rarely rescaled.
 //
 // Work split: the granules of all (sequence, row tile, head) units are laid end to end and every block takes the same
@@ -190,6 +193,8 @@ struct Split {
     static constexpr int FRAGMENTS = KT * 512;
     static constexpr int SMEM = BUFFER + FRAGMENTS + WARPS * STAGES * 8 + (WARPS * 2 + 1) * ROWS * 4 + 64;
     static constexpr int PARTIAL = ROWS * (W + 2);
+    static constexpr int FOLD = 64 / SG;               // stages that a warp's accumulators sum at most: 64 products each
+    static constexpr int FOLDED = WARPS * (NT + 1) * 64;  // floats of a block's sums behind all blocks' partial results: a thread's own, and their m and bias
     // A second segment costs a block about 6 us of prologue and join; the bytes that its warps read in that time.
     static constexpr uint32_t SEGMENT = 96 * 1024 / L.bytes;
     static_assert(STAGES >= 2, "a ring needs two stages");
@@ -298,7 +303,17 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
 #pragma unroll
         for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
 
-        for (uint32_t i = 0; i < mystages && alive; ++i) {
+        // the sums of earlier stages, of a maximum and a bias of then
+        auto sums_so_far = [&]() {
+            uint32_t thread = threadIdx.x;
+            asm volatile("" : "+r"(thread));  // (found anew each time: the loop has no registers to keep it in)
+            return (float2 *)(p.partials + (size_t)gridDim.x * 2 * S::PARTIAL + (size_t)blockIdx.x * S::FOLDED) + thread / 32 * (NT + 1) * 32 + thread % 32;
+        };
+        auto weight_of = [&](float2 then) {
+            return then.x == -INFINITY ? 0.0f : exp2_approx(then.x - m) * (bias / then.y);
+        };
+        for (uint32_t i = 0, upto = S::FOLD;; upto += S::FOLD) {
+        for (const uint32_t end = min(upto, mystages); i < end && alive; ++i) {
             const uint32_t slot = turn;
             alive = mbar_wait(smem_u32(bars + warp * STAGES + slot), phase);
             if (!__all_sync(0xffffffffu, alive)) {  // a copy never came: report, let the others in flight land, give up the block's results
@@ -443,6 +458,30 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
             else take(std::false_type{});
             __syncwarp();
             if (lane == 0 && left) request();
+        }
+            if (i == mystages || !alive) break;
+            // (only its own thread reads what it writes)
+            float2 *folded = sums_so_far();
+            const float f = upto == S::FOLD ? 0.0f : weight_of(folded[NT * 32]);
+#pragma unroll
+            for (int k = 0; k < NT; ++k) {
+                float2 x = upto == S::FOLD ? make_float2(0.0f, 0.0f) : folded[k * 32];
+                x.x = fmaf(x.x, f, o[k][0] + o[k][2]);
+                x.y = fmaf(x.y, f, o[k][1] + o[k][3]);
+                folded[k * 32] = x;
+                o[k][0] = o[k][1] = o[k][2] = o[k][3] = 0.0f;
+            }
+            folded[NT * 32] = make_float2(m, bias);
+        }
+        if (mystages > (uint32_t)S::FOLD) {
+            const float2 *folded = sums_so_far();
+            const float f = weight_of(folded[NT * 32]);
+#pragma unroll
+            for (int k = 0; k < NT; ++k) {
+                const float2 x = folded[k * 32];
+                o[k][0] = fmaf(x.x, f, o[k][0]);
+                o[k][1] = fmaf(x.y, f, o[k][1]);
+            }
         }
 
         // ---- join the warps ----

@@ -120,3 +120,23 @@ def test_queries_with_a_mean_and_keys_with_large_channels(backend, width):
         write(b, held, cache, shape, [(0, 0, length)], length, k, v)
         want = kv_oracle.attention(q, kv_oracle.stored(k, enc.Q8_0), kv_oracle.stored(v, enc.Q8_0), length - rows, group)
         assert rel_l2(attend(b, held, cache, shape, [(0, length - rows, rows)], rows, q, group), want) <= 1e-5
+
+
+@pytest.mark.parametrize("length", [24100, 100000])
+@pytest.mark.parametrize("width,heads,group", [(256, 1, 8), (128, 2, 4), (64, 1, 8)])
+def test_long_sums_of_whole_units(backend, width, heads, group, length):
+    """More units than blocks over a long cache, to F32: a block sums all positions of a unit, and values of one sign make the sums grow."""
+    b = backend
+    rows = 592
+    shape = KvCache(1, (length + 15) // 16 * 16, heads, width, enc.Q8_0, enc.Q4_0)
+    rng = np.random.default_rng(length)
+    k, v = (rng.standard_normal((length, heads, width), dtype=np.float32) for _ in range(2))
+    v += 3
+    q = rng.standard_normal((rows, heads * group, width), dtype=np.float32) * np.float32(0.3)
+    with Held(b) as held:
+        cache = held.new(shape.bytes)
+        write(b, held, cache, shape, [(0, 0, length)], length, k, v)
+        got = attend(b, held, cache, shape, [(0, length - rows, rows)], rows, q, heads * group)
+        k, v = kv_oracle.stored(k, enc.Q8_0), kv_oracle.stored(v, enc.Q4_0)
+        for i in (0, 301, 591):
+            assert rel_l2(got[i:i + 1], kv_oracle.attention(q[i:i + 1], k, v, length - rows + i, group)) <= 1e-5, i
