@@ -15,8 +15,8 @@
 //     49 us either way. Where a block's queries do not cancel and one channel sets the scale, the offset's share is many times the score:
 //     the result was off by up to 9e-5.)
 //   * p v = sum_j (p_j d_jb) c_j: the scale goes into the probability, once per block, before it is split. The products
-//     p d are kept near 2^11 by a power of two per warp (`bias`), lowered when a larger scale comes by: f16's range is no limit,
-//     and what is lost of a position is below 2^-36 of the largest value seen.
+//     p d are kept near 2^11 by a power of two per warp (`bias`), moved when a scale above 2^12 comes by or all that a warp takes at once (16 positions, 32
+//     at width 64) lie below 2^6: f16's range is no limit, and what is lost of a position is below 2^-31 of the largest value beside it.
 //   * A tensor core's sum is cut off, not rounded, at each step (about 2^-24 of it, always towards zero: a unit of 100,000 positions in one block was
 //     up to 9e-5 off), so a warp adds its accumulators up elsewhere, rounded, every 64 products: 592 rows at 100,000 positions, width 256, 4,604 us
 //     without and 4,667 with it (5,079 every 32, with the place of the sums kept in registers).
@@ -401,11 +401,11 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
             for (int j = 0; j < SG * 2; ++j) top = fmaxf(top, fmaxf(s[j][0], s[j][1]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            if (__any_sync(0xffffffffu, top > m + 3.0f || dmax * bias > 4096.0f)) {
+            if (__any_sync(0xffffffffu, top > m + 3.0f || dmax * bias > 4096.0f) || __all_sync(0xffffffffu, dmax * bias < 64.0f)) {
                 float d = fmaxf(dmax, __shfl_xor_sync(0xffffffffu, dmax, 1));
                 d = fmaxf(d, __shfl_xor_sync(0xffffffffu, d, 2));
                 const float next = fmaxf(m, top);
-                const float bias_next = d * bias > 4096.0f ? scalbnf(1.0f, 127 + 11 - (int)(__float_as_uint(fminf(d, 65504.0f)) >> 23)) : bias;
+                const float bias_next = d * bias > 4096.0f || (d * bias < 64.0f && d > 0.0f) ? scalbnf(1.0f, 127 + 11 - (int)(__float_as_uint(fminf(d, 65504.0f)) >> 23)) : bias;
                 const float fl = m == -INFINITY ? 0.0f : exp2_approx(m - next), f = fl * (bias_next / bias);
                 bias = bias_next;
                 m = next;

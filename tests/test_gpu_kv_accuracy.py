@@ -51,6 +51,24 @@ def test_large_values_ahead_of_those_that_count(backend, width, venc, ratio):
         assert rel_l2(attend(b, held, cache, shape, spans, rows, q, 1), want) <= 1e-5
 
 
+@pytest.mark.parametrize("venc", [enc.Q8_0, enc.Q4_0])
+@pytest.mark.parametrize("width", [64, 128, 256])
+def test_large_values_ahead_in_one_block_to_f32(backend, width, venc):
+    """More units than blocks, so that one block (and of it the warp that has both positions) walks past the large values to those that count."""
+    b = backend
+    length, rows = 4096, 592
+    shape = KvCache(1, length, 1, width, enc.Q8_0, venc)
+    q, k, v = one_key_and_one_value(width, length, rows * 8, 2661, 101, 2 ** 20, 7)  # granules 166 and 6, 160 apart
+    q = q.reshape(rows, 8, width)
+    with Held(b) as held:
+        cache = held.new(shape.bytes)
+        write(b, held, cache, shape, [(0, 0, length)], length, k, v)
+        got = attend(b, held, cache, shape, [(0, length - rows, rows)], rows, q, 8)
+        k, v = kv_oracle.stored(k, enc.Q8_0), kv_oracle.stored(v, venc)
+        for i in (0, 300, 591):
+            assert rel_l2(got[i:i + 1], kv_oracle.attention(q[i:i + 1], k, v, length - rows + i, 8)) <= 1e-5, i
+
+
 @pytest.mark.parametrize("ratio", [2 ** 7, 2 ** 12, 2 ** 16, 2 ** 20])
 @pytest.mark.parametrize("kenc,venc", PAIRS)
 @pytest.mark.parametrize("width", [64, 128, 256])
