@@ -70,11 +70,11 @@ Backend *Backend::create(int device, std::string &error) {
     ok = ok && cudaStreamCreateWithFlags(&b->stream_, cudaStreamNonBlocking) == cudaSuccess;
     ok = ok && cudaEventCreate(&b->ev_start_) == cudaSuccess && cudaEventCreate(&b->ev_stop_) == cudaSuccess;
     ok = ok && cudaMalloc(&b->partials_, kPartialsFloats * sizeof(float)) == cudaSuccess;
-    ok = ok && cudaMalloc(&b->counters_, (kCounters + 3) * sizeof(uint32_t)) == cudaSuccess;
-    ok = ok && cudaMemset(b->counters_, 0, (kCounters + 3) * sizeof(uint32_t)) == cudaSuccess;
-    ok = ok && cudaHostAlloc(&b->status_host_, sizeof(uint32_t), cudaHostAllocMapped) == cudaSuccess;
+    ok = ok && cudaMalloc(&b->counters_, (kCounters + 2) * sizeof(uint32_t)) == cudaSuccess;
+    ok = ok && cudaMemset(b->counters_, 0, (kCounters + 2) * sizeof(uint32_t)) == cudaSuccess;
+    ok = ok && cudaHostAlloc(&b->status_host_, STATUS_WORDS * sizeof(uint32_t), cudaHostAllocMapped) == cudaSuccess;
     ok = ok && cudaHostGetDevicePointer(&b->status_device_, b->status_host_, 0) == cudaSuccess;
-    if (ok) *b->status_host_ = 0;
+    if (ok) memset(b->status_host_, 0, STATUS_WORDS * sizeof(uint32_t));
     ok = ok && cudaMalloc(&b->argmax_records_, (128 * 4 + 4) * sizeof(float)) == cudaSuccess;
     ok = ok && cudaMemset(b->argmax_records_, 0, (128 * 4 + 4) * sizeof(float)) == cudaSuccess;
     if (!ok) {
@@ -277,7 +277,7 @@ int Backend::flushChain() {
     if (!chain_ || chain_->jobs.empty()) return NU_OK;
     std::vector<FastJob> &jobs = chain_->jobs;
     int launched = 0;
-    if (jobs.size() >= 2) launched = launch_chain(stream_, jobs.data(), (uint32_t)jobs.size(), counters_ + counters_len_ + 1, sm_count_);
+    if (jobs.size() >= 2) launched = launch_chain(stream_, jobs.data(), (uint32_t)jobs.size(), counters_ + counters_len_, sm_count_);
     if (launched) {
         launches_ += launched;
     } else {
@@ -326,19 +326,24 @@ int Backend::finishCapture(cudaGraphExec_t *exec) {
     return cuda(e, "commit: instantiate");
 }
 
-// Waits for everything enqueued so far and reads the kernels' status word. It lies in host memory that the kernels that have something to
+// Waits for everything enqueued so far and reads the kernels' status words. They lie in host memory that the kernels that have something to
 // report write to themselves, so a replay copies nothing back for it (a copy and a second wait cost 10 us of a replay's 37).
 int Backend::checkKernelStatus() {
     if (int rc = cuda(cudaStreamSynchronize(stream_), "launch: wait")) return rc;
-    const uint32_t status = *(volatile uint32_t *)status_host_;
-    if (status != 0) {
-        *(volatile uint32_t *)status_host_ = 0;
-        cudaMemsetAsync(counters_, 0, (counters_len_ + 3) * sizeof(uint32_t), stream_);  // counters, status word, the chain kernel's two arrival counts
-        cudaStreamSynchronize(stream_);
-        if (status == 3) return fail(NU_ERR_EXECUTION, "a span of rows lies outside the key/value cache: its sequence was left out");
-        return fail(NU_ERR_EXECUTION, status == 2 ? "allreduce over peer memory: a rank never arrived (bounded wait ran out); the path stays closed" : "a kernel gave up a bounded wait (copy never completed)");
+    static const char *const text[STATUS_WORDS] = {"a kernel gave up a bounded wait (copy never completed)",
+                                                   "allreduce over peer memory: a rank never arrived (bounded wait ran out); the path stays closed",
+                                                   "a span of rows lies outside the key/value cache: its sequence was left out"};
+    std::string met;
+    for (int i = 0; i < STATUS_WORDS; ++i) {
+        volatile uint32_t *word = status_host_ + i;
+        if (*word == 0) continue;
+        *word = 0;
+        met += (met.empty() ? "" : "; ") + std::string(text[i]);
     }
-    return NU_OK;
+    if (met.empty()) return NU_OK;
+    cudaMemsetAsync(counters_, 0, (counters_len_ + 2) * sizeof(uint32_t), stream_);  // with the chain kernel's two
+    cudaStreamSynchronize(stream_);
+    return fail(NU_ERR_EXECUTION, met.c_str());
 }
 
 int Backend::runGraph(cudaGraphExec_t exec, uint32_t count, float *elapsed_ms) {
@@ -1263,7 +1268,7 @@ int Backend::allreduceSumF32(const Buffer &buffer, size_t count, const Buffer *a
         pp.buf = p; pp.count = (uint32_t)count; pp.ranks = (uint32_t)peer_ranks_; pp.rank = (uint32_t)peer_rank_; pp.capacity = (uint32_t)kPushCapacity;
         for (int r = 0; r < peer_ranks_; ++r) pp.inbox[r] = (uint2 *)peer_base_[r];
         pp.seq = (uint32_t *)(inbox_ + kPushWordBytes);
-        pp.status = status_device_;
+        pp.status = status_device_ + STATUS_PEER;
         pp.wait_ns = peer_wait_ns_;
         pp.add_to = res;
         if (fuse) {

@@ -152,13 +152,13 @@ private:
     double gpu_seconds_ = 0;
     uint64_t launches_ = 0;
     std::string error_;
-    // scratch of the split-K kernels: partial sums, arrival counters and a status word
+    // scratch of the split-K kernels: partial sums and arrival counters (behind them the chain kernel's two)
     float *partials_ = nullptr;
     size_t partials_floats_ = 0;
     uint32_t *counters_ = nullptr;
     float *argmax_records_ = nullptr;  // 128 x (value, index, non-finite) of the argmax blocks, then their arrival counter
     size_t counters_len_ = 0;
-    uint32_t *status_host_ = nullptr, *status_device_ = nullptr;  // the status word, in host memory, and where the kernels see it
+    uint32_t *status_host_ = nullptr, *status_device_ = nullptr;  // the status words (StatusWord), in host memory, and where the kernels see them
     // per-operator profile
     bool profiling_ = false;
     uint32_t profile_max_ = 0;

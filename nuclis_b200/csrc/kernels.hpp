@@ -194,11 +194,15 @@ uint32_t prepared_layout(uint32_t enc, uint32_t rows, uint32_t columns);
 int launch_prepare(cudaStream_t s, uint32_t enc, const uint8_t *src, uint8_t *dst, uint32_t rows, uint32_t columns);
 
 // ---- the quantized key/value cache and the attention that reads it (kv_layout.cuh) ---------
+// The handle's status words, in host memory, one a condition, so that none hides another: a kernel with something to report makes its own nonzero. Where a
+// job's status is a single word it is that of STATUS_WAIT (or of the operator's own scratch).
+enum StatusWord { STATUS_WAIT = 0, STATUS_PEER = 1, STATUS_SPAN = 2, STATUS_WORDS = 3 };
+
 struct KvCacheJob {
     uint8_t *base;
     bool k8, v8;  // Q8_0 instead of Q4_0
     uint32_t slots, capacity, heads, width;
-    uint32_t *status;  // raised when a span lies outside the cache
+    uint32_t *status;  // the status words
 };
 // keys and values: [sequences * tokens] rows at their strides (in elements); spans: one nu_kv_span a sequence, on the device.
 int launch_kv_write(cudaStream_t s, const KvCacheJob &cache, const void *spans, uint32_t sequences, uint32_t tokens, const float *keys, size_t key_stride,

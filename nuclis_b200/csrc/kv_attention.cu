@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
             const uint32_t slot = turn;
             alive = mbar_wait(smem_u32(bars + warp * STAGES + slot), phase);
             if (!__all_sync(0xffffffffu, alive)) {  // a copy never came: report, let the others in flight land, give up the block's results
-                *(volatile uint32_t *)p.c.status = 1u;
+                *(volatile uint32_t *)(p.c.status + STATUS_WAIT) = 1u;
                 for (uint32_t k = i + 1; k < min(i + STAGES, mystages); ++k) {
                     if (++turn == STAGES) { turn = 0; phase ^= 1u; }
                     mbar_wait(smem_u32(bars + warp * STAGES + turn), phase);

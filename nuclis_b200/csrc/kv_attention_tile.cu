@@ -861,7 +861,7 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
-    if (tid == 0 && *abort_flag) *(volatile uint32_t *)p.c.status = 1u;
+    if (tid == 0 && *abort_flag) *(volatile uint32_t *)(p.c.status + STATUS_WAIT) = 1u;
 }
 
 template <int W, bool K8, bool V8>

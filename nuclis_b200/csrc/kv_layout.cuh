@@ -24,6 +24,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "kernels.hpp"
+
 namespace nu {
 
 constexpr uint32_t KV_GRANULE = 16;  // positions
@@ -63,7 +65,7 @@ struct KvView {
     uint8_t *base;
     KvLayout l;
     uint32_t slots, heads, granules;  // granules of a (slot, head)
-    uint32_t *status;
+    uint32_t *status;  // the status words
 };
 
 __device__ __forceinline__ uint8_t *kv_head(const KvView &c, uint32_t slot, uint32_t head) {
@@ -71,12 +73,12 @@ __device__ __forceinline__ uint8_t *kv_head(const KvView &c, uint32_t slot, uint
 }
 
 // A span that names a slot or a position outside the cache, or more rows than the call has, counts as empty and raises
-// the status word, which the next commit or graph launch reports.
+// its status word, which the next commit or graph launch reports.
 __device__ __forceinline__ KvSpan kv_span(const KvView &c, const KvSpan *spans, uint32_t sequence, uint32_t tokens) {
     const uint4 w = *(const uint4 *)(spans + sequence);
     KvSpan s{w.x, w.y, w.z, 0};
     if (s.count && (s.slot >= c.slots || s.count > tokens || (uint64_t)s.first + s.count > (uint64_t)c.granules * KV_GRANULE)) {
-        *(volatile uint32_t *)c.status = 3u;
+        *(volatile uint32_t *)(c.status + STATUS_SPAN) = 1u;
         s.count = 0;
     }
     return s;

@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(256) push_allreduce_kernel(PushParams p) {
     }
     __syncthreads();
     if (head[0] != 0) {  // uniform over the block
-        if (tid == 0) *(volatile uint32_t *)p.status = 2u;
+        if (tid == 0) *(volatile uint32_t *)p.status = 1u;
         return;
     }
     const uint32_t seq = head[1];
@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(256) push_allreduce_kernel(PushParams p) {
     }
     if (__syncthreads_or(failed)) {
         if (tid == 0) {
-            *(volatile uint32_t *)p.status = 2u;
+            *(volatile uint32_t *)p.status = 1u;
             atomicExch(p.seq + 2, 1u);
         }
         return;
