@@ -22,9 +22,6 @@ struct FastChain { std::vector<FastJob> jobs; };
 namespace {
 
 constexpr size_t kPad = 256;                       // slack after every allocation: bulk copies may read up to 15 bytes past a row
-constexpr size_t kPartialsFloats = 64u << 20;      // 256 MiB of scratch: split-K partial sums, the bf16 staging of F32 prefill activations,
-                                                   // the gathered rows of the grouped (expert) prefill
-constexpr size_t kCounters = 1u << 16;             // row-block arrival counters
 constexpr size_t kPushCapacity = 8 * 8192;         // floats per inbox slot: 8 token rows of up to 8192 values
 constexpr size_t kPushWordBytes = 2 * PUSH_MAX_RANKS * kPushCapacity * 8;   // (value, tag) words
 constexpr size_t kPushBytes = kPushWordBytes + 64;                          // then sequence number, finished blocks, sticky failure
@@ -66,12 +63,17 @@ Backend *Backend::create(int device, std::string &error) {
         delete b;
         return nullptr;
     }
+    if (ok && prop.multiProcessorCount > (int)SCRATCH_SMS) {
+        error = "the scratch of a handle is for at most " + std::to_string(SCRATCH_SMS) + " multiprocessors; found " + std::to_string(prop.multiProcessorCount);
+        delete b;
+        return nullptr;
+    }
     b->sm_count_ = prop.multiProcessorCount;
     ok = ok && cudaStreamCreateWithFlags(&b->stream_, cudaStreamNonBlocking) == cudaSuccess;
     ok = ok && cudaEventCreate(&b->ev_start_) == cudaSuccess && cudaEventCreate(&b->ev_stop_) == cudaSuccess;
-    ok = ok && cudaMalloc(&b->partials_, kPartialsFloats * sizeof(float)) == cudaSuccess;
-    ok = ok && cudaMalloc(&b->counters_, (kCounters + 2) * sizeof(uint32_t)) == cudaSuccess;
-    ok = ok && cudaMemset(b->counters_, 0, (kCounters + 2) * sizeof(uint32_t)) == cudaSuccess;
+    ok = ok && cudaMalloc(&b->partials_, SCRATCH_FLOATS * sizeof(float)) == cudaSuccess;
+    ok = ok && cudaMalloc(&b->counters_, (SCRATCH_COUNTERS + 2) * sizeof(uint32_t)) == cudaSuccess;
+    ok = ok && cudaMemset(b->counters_, 0, (SCRATCH_COUNTERS + 2) * sizeof(uint32_t)) == cudaSuccess;
     ok = ok && cudaHostAlloc(&b->status_host_, STATUS_WORDS * sizeof(uint32_t), cudaHostAllocMapped) == cudaSuccess;
     ok = ok && cudaHostGetDevicePointer(&b->status_device_, b->status_host_, 0) == cudaSuccess;
     if (ok) memset(b->status_host_, 0, STATUS_WORDS * sizeof(uint32_t));
@@ -87,8 +89,8 @@ Backend *Backend::create(int device, std::string &error) {
         delete b;
         return nullptr;
     }
-    b->partials_floats_ = kPartialsFloats;
-    b->counters_len_ = kCounters;
+    b->partials_floats_ = SCRATCH_FLOATS;
+    b->counters_len_ = SCRATCH_COUNTERS;
     b->buffers_.push_back({});  // id 0 is never handed out
     return b;
 }
@@ -824,7 +826,7 @@ int Backend::tokenLogprobs(const Buffer &logits, size_t rows, size_t count, size
             if (part[a].b && part[b].b && overlaps(*part[a].b, part[a].len, *part[b].b, part[b].len)) return fail(NU_ERR_INVALID_SHAPE, "token_logprobs: an output overlaps another buffer");
     if (int rc = needRecording()) return rc;
     j.rows = (uint32_t)rows; j.count = (uint32_t)count; j.stride = in_stride; j.k = (uint32_t)k;
-    j.partials = partials_; j.partials_floats = partials_floats_; j.counters = counters_; j.counters_len = counters_len_; j.sm_count = sm_count_;
+    j.partials = partials_; j.counters = counters_; j.sm_count = sm_count_;
     launches_ += launch_token_logprobs(stream_, j);
     wrote(logprobs); wrote(entropies);
     if (k) { wrote(*top); wrote(*top_logprobs); }

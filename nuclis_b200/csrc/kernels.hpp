@@ -8,6 +8,13 @@
 
 namespace nu {
 
+// A handle's scratch: floats for partial sums, the bf16 staging of F32 prefill activations, the gathered rows of the grouped (expert) prefill and the
+// parts of attention units and logit rows; and arrival counters, zero between launches. Kernels whose need goes by the device's multiprocessors
+// alone assert here, for SCRATCH_SMS of them (a device with more is refused), that it suffices; those whose need goes by the shapes compare it.
+constexpr size_t SCRATCH_FLOATS = 64u << 20;    // 256 MiB
+constexpr size_t SCRATCH_COUNTERS = 1u << 16;
+constexpr size_t SCRATCH_SMS = 256;
+
 // ---- plain decode-and-FMA kernels (any encoding, any alignment) -----------
 
 // Decodes `columns` values of one row to F32 or BF16.
@@ -222,8 +229,8 @@ struct AttentionJob {
     float scale;
     uint32_t window;  // 0: none
     bool generic;
-    float *partials;     // of the handle
-    uint32_t *counters;  // of the handle, zero between launches
+    float *partials;     // of the handle: SCRATCH_FLOATS
+    uint32_t *counters;  // of the handle: SCRATCH_COUNTERS, zero between launches
     int sm_count;
 };
 bool attention_configure();
@@ -240,10 +247,8 @@ struct LogprobJob {
     uint32_t k;
     uint32_t *top;
     float *top_logprobs;
-    float *partials;     // of the handle
-    size_t partials_floats;
-    uint32_t *counters;  // of the handle, zero between launches
-    size_t counters_len;
+    float *partials;     // of the handle: SCRATCH_FLOATS
+    uint32_t *counters;  // of the handle: SCRATCH_COUNTERS, zero between launches
     int sm_count;
 };
 int launch_token_logprobs(cudaStream_t s, const LogprobJob &job);

@@ -197,6 +197,7 @@ struct Split {
     static constexpr int FOLDED = WARPS * (NT + 1) * 64;  // floats of a block's sums behind all blocks' partial results: a thread's own, and their m and bias
     // A second segment costs a block about 6 us of prologue and join; the bytes that its warps read in that time.
     static constexpr uint32_t SEGMENT = 96 * 1024 / L.bytes;
+    static_assert(SCRATCH_SMS * RESIDENT * (2 * PARTIAL + FOLDED) <= SCRATCH_FLOATS && SCRATCH_SMS * RESIDENT <= SCRATCH_COUNTERS, "the handle's scratch");
     static_assert(STAGES >= 2, "a ring needs two stages");
     static_assert(SMEM <= 113 * 1024, "two blocks share a multiprocessor");
 };

@@ -54,6 +54,7 @@ struct Tile {
     // tensor memory columns
     static constexpr int S_COLS = KT, O_COL = 2 * KT;
     static constexpr int PARTIAL = ROWS * (W + 2);
+    static_assert(SCRATCH_SMS * 2 * PARTIAL <= SCRATCH_FLOATS && SCRATCH_SMS <= SCRATCH_COUNTERS, "the handle's scratch");
     // P is kept 2^P_UP above the probabilities (at most 2^8 before a maximum moves), so that it ends below 2^15. O carries the exponent of a
     // step's values; a step whose values' lies up to SPREAD below takes P down by that (a probability of one keeps 11 bits down to 2^-14, so a SPREAD of
     // 12 leaves those of 2^-9 all of theirs), any other moves O's exponent to its own, up or down. O is at most 2^31 positions of 2^15 times a value

@@ -31,6 +31,8 @@ static_assert(PARTS_MAX * MAX_K <= (uint32_t)CANDIDATES && PARTS_MAX <= (uint32_
 constexpr int FEW = 256;                    // candidates that are ranked by counting
 constexpr int RECORD = 4 + 2 * MAX_K;       // floats a block leaves: m, Z, sum, bad, then the keys
 
+static_assert(SCRATCH_SMS * RESIDENT * 2 * RECORD <= SCRATCH_FLOATS && SCRATCH_SMS * RESIDENT <= SCRATCH_COUNTERS, "the handle's scratch");
+
 struct Params {
     LogprobJob j;
     uint32_t rounds, share;  // rounds a row, rounds a block
