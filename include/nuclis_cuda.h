@@ -353,8 +353,9 @@ typedef struct nu_kv_span {
 } nu_kv_span;
 
 /* Quantizes rows of keys and values (F32, [heads][width] contiguous within a row, strides in floats) into the cache. The
- * rule is GGUF's, in F32: Q8_0 d = amax * (1 / 127), code = round(x * (1 / d)); Q4_0 d = m / -8 with m the first value of the largest
- * magnitude, code = min(15, trunc(x * (1 / d) + 8.5)); d is stored as f16. A scale beyond f16 saturates, a block with a NaN or
+ * rule, in F32: Q8_0 d = amax * (1 / 127), code = round(x * (1 / d)); Q4_0 d = m / -8 with m the first value of the largest
+ * magnitude, code = min(15, trunc(x * (1 / d) + 8.5)); d is stored as f16. Q4_0's is GGUF's. GGUF's Q8_0 divides by 127 where this
+ * multiplies by the reciprocal: a scale may be a step of f16 apart, and a code one, where the quotient lies next to a border. A scale beyond f16 saturates, a block with a NaN or
  * an infinity reads back as NaN. Where two spans of one call cover the same position, the later span's row is kept. */
 int nu_cuda_kv_write(nu_cuda *h, const nu_buffer *buffer, const nu_kv_cache *cache, const nu_buffer *spans, size_t sequences, size_t tokens,
                      const nu_buffer *keys, size_t key_stride, const nu_buffer *values, size_t value_stride);

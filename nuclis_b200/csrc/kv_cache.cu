@@ -1,7 +1,8 @@
 // Writing rows of keys and values into the quantized cache, and reading them back. Both are one pass over the rows:
 // bound by memory for a prompt, by the launch for a single row.
 //
-// The rule of a block of 32 (GGUF's, in F32 arithmetic): Q8_0 d = amax * (1 / 127), code = round(x * (1 / d)) with halves away
+// The rule of a block of 32 (in F32; GGUF's but for Q8_0's division by 127, here a product with the reciprocal: no slow division in a warp's chain
+// of dependent steps, and d within 2^-23 of the quotient): Q8_0 d = amax * (1 / 127), code = round(x * (1 / d)) with halves away
 // from zero; Q4_0 d = m / -8 with m the first value of the largest magnitude, code = min(15, trunc(x * (1 / d) + 8.5)).
 // The stored scale is d rounded to f16. A block whose scale rounds to zero stores zeros; one whose scale passes the f16
 // range stores the largest scale and saturated codes; one that holds a NaN or an infinity stores a NaN scale, so that it
