@@ -368,7 +368,8 @@ int nu_cuda_kv_read(nu_cuda *h, const nu_buffer *buffer, const nu_kv_cache *cach
  * (window 0: all from 0), which must have been written. `heads` query heads, a multiple of the cache's: query head h
  * reads key/value head h / (heads / cache heads).
  *   output[row][h] = sum_j softmax_j(scale * query[row][h] . key_j) value_j
- * Queries are F32, [heads][width] contiguous within a row, strides in elements; scale 0 stands for 1 / sqrt(width).
+ * Queries are F32, [heads][width] contiguous within a row, strides in elements; scale 0 stands for 1 / sqrt(width), any other is positive and at
+ * most 2e38.
  * `out_dtype` NU_F32 gives the result in F32 accuracy for any number of rows; NU_BF16 rounds it to BF16 (what `matmul` takes as
  * its input), and may use 16-bit operands in the products where a call has many rows. */
 typedef struct nu_attention {

@@ -380,7 +380,9 @@ class Backend:
     def attention(self, cache: Buffer, shape: KvCache, spans: Buffer, sequences: int, tokens: int, queries: Buffer, q_stride: int, heads: int, output: Buffer,
                   out_stride: int, scale: float | None = None, window: int = 0, out_dtype: int = 0) -> None:
         """Causal grouped-query attention of ``heads`` query heads over the cache: the row at position p sees the last ``window``
-        positions up to p (0: all). ``scale`` defaults to 1 / sqrt(width); ``out_dtype`` F32 or BF16 (see nu_cuda_attention)."""
+        positions up to p (0: all). ``scale`` defaults to 1 / sqrt(width) and is positive else; ``out_dtype`` F32 or BF16 (see nu_cuda_attention)."""
+        if scale is not None and np.float32(scale) == 0:  # which the C call takes for the default
+            raise NuclisError(4, "attention: a scale of zero")
         spec = _lib.CAttention(heads, q_stride, out_stride, out_dtype, window, 0.0 if scale is None else scale)
         self._check(self._lib.nu_cuda_attention(self._h, cache._c(), shape._c(), spans._c(), sequences, tokens, queries._c(), output._c(), ctypes.byref(spec)))
 

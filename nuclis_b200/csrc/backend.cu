@@ -924,7 +924,7 @@ int Backend::attention(const Buffer &buffer, const nu_kv_cache &c, const Buffer 
     if (int rc = kvJob("attention", buffer, c, spans, sequences, tokens, &job, &span)) return rc;
     if (a.heads == 0 || a.heads % c.heads || a.heads > 16384) return fail(NU_ERR_INVALID_SHAPE, "attention: query heads are a multiple of the cache's");
     if (a.out_dtype != NU_F32 && a.out_dtype != NU_BF16) return fail(NU_ERR_INVALID_SHAPE, "attention: output type");
-    if (!(a.scale >= 0.0f) || a.scale > 3.0e38f || a.window > (1u << 31)) return fail(NU_ERR_INVALID_SHAPE, "attention: scale or window");
+    if (!(a.scale >= 0.0f) || a.scale > 2.0e38f /* the kernels take it times log2(e) */ || a.window > (1u << 31)) return fail(NU_ERR_INVALID_SHAPE, "attention: scale or window");
     const size_t element = a.out_dtype == NU_F32 ? 4 : 2, width = a.heads * c.width, rows = sequences * tokens;
     const size_t qlen = rowsBytes(rows, width, a.q_stride, 4), olen = rowsBytes(rows, width, a.out_stride, element);
     if (!qlen || !olen) return fail(NU_ERR_INVALID_SHAPE, "attention: stride");
