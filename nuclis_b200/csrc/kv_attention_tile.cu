@@ -889,10 +889,16 @@ bool attention_tile_configure() {
     return ok;
 }
 
-// From 128 query rows a key/value head. Below, the kernel for few rows is the faster one unless the context is very long, and its time grows with the
-// rows; here it hardly does. Measured (it / this one, us; Q8_0 keys, Q4_0 values, 8 heads of width 128): at position 700 64 rows
-// 17 / 42, 128 rows 19 / 43, 256 rows 21 / 45; at 8,000 41 / 73, 66 / 74, 107 / 76; at 60,000 180 / 171, 342 / 172, 666 / 175. Width 256, 4
-// heads: 8,000 40 / 83, 67 / 86, 104 / 86; 60,000 173 / 180, 321 / 182, 612 / 164. (The positions are only known on the device.)
+// From 128 query rows a key/value head, whatever the position. The kernel for few rows has a smaller fixed cost and takes time with rows x positions x heads; this
+// one hardly does. Measured (few rows / this one, us; Q8_0 keys, Q4_0 values, rows a head at a position):
+//   8 heads of width 128: 128 rows at 300 17 / 37, at 2,000 29 / 51, at 8,000 66 / 75; 256 rows 16 / 41, 38 / 53, 109 / 78; 512 rows 23 / 41, 70 / 55, 201 / 79;
+//     1,024 rows 35 / 43, 123 / 55, 383 / 102
+//   4 heads of width 256: 128 rows 23 / 39, 33 / 57, 68 / 86; 256 rows 23 / 40, 43 / 58, 107 / 87; 1,024 rows 29 / 40, 114 / 53, 358 / 84
+//   8 heads of width 64: 128 rows 14 / 33, 21 / 45, 39 / 66; 512 rows 18 / 35, 39 / 49, 111 / 68; 1,024 rows 28 / 37, 75 / 47, 205 / 88
+//   32 heads of width 128: 128 rows 23 / 41, 70 / 54, 201 / 99; 512 rows 86 / 49, 201 / 70, 738 / 164
+// So they meet near rows x positions x heads x width = 2^29, and this rule is 20 to 28 us slower than the better kernel for a short prompt at the start of a
+// session (up to 2.6 times), for up to ten times that gained on a long one. What it would take to do better, the positions, is in the spans on the device; all
+// that the host has is the capacity, which in a session's cache is far above them.
 bool attention_tile_supported(const AttentionJob &j) {
     const uint32_t w = j.cache.width;
     return j.bf16 && (w == 64 || w == 128 || w == 256) && (uint64_t)j.tokens * (j.heads / j.cache.heads) >= 128;
