@@ -439,18 +439,10 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                 tmem_store8(pfirst + (PIECES - 1) * 8, pk);
                 sums[0] = add2(add2(sums[0], sums[1]), add2(sums[2], sums[3]));
                 const float sum = low_of(sums[0]) + high_of(sums[0]);
-                if (any_nan[ring]) {  // the blocks that are NaN at a position this row has weight on: P once more
-                    tmem_store_wait();
+                if (any_nan[ring]) {  // the blocks that are NaN at a position this row sees, whatever weight it has there
+                    const uint8_t *mine = nans + ring * 128 + (QT == 1 ? group * COLS : 0);
 #pragma unroll 1
-                    for (int k = 0; k < COLS / 32; ++k) {
-                        uint32_t q16[16];
-                        tmem_load16(pfirst + k * 16, q16);
-                        tmem_load_wait();
-                        const uint32_t k0 = (QT == 1 ? group * COLS : 0) + k * 32;
-#pragma unroll
-                        for (int c = 0; c < 32; ++c)
-                            if (q16[c / 2] >> (c % 2 * 16) & 0xffffu) nan_blocks |= nans[ring * 128 + k0 + c];
-                    }
+                    for (int c = from; c <= min(to, COLS - 1); ++c) nan_blocks |= mine[c];
                 }
                 l += sum * power_of_two(-shift);
                 tmem_store_wait();
