@@ -432,11 +432,13 @@ __global__ void __launch_bounds__(Split<W, K8, V8>::THREADS, 2) split_kernel(con
                 for (int b = 0; b < NB; ++b) {
                     float x0 = p0 * scale_of<NB>(vs[2 * k], 0, b), x1 = p1 * scale_of<NB>(vs[2 * k], 1, b);
                     float x2 = p2 * scale_of<NB>(vs[2 * k + 1], 0, b), x3 = p3 * scale_of<NB>(vs[2 * k + 1], 1, b);
-                    if (edge) {  // a position that this row does not see, another does, and whose scale is a NaN
-                        if (p0 == 0.0f) x0 = 0.0f;
-                        if (p1 == 0.0f) x1 = 0.0f;
-                        if (p2 == 0.0f) x2 = 0.0f;
-                        if (p3 == 0.0f) x3 = 0.0f;
+                    if (edge) {  // a position that this row does not see, another does, and whose scale is a NaN (one that it sees reaches it at any weight)
+                        const uint32_t key = key0 + k * KV_GRANULE + 2 * t;
+                        auto unseen = [&](uint32_t at) { return at < row_low || at > row_high; };
+                        if (unseen(key)) x0 = 0.0f;
+                        if (unseen(key + 1)) x1 = 0.0f;
+                        if (unseen(key + 8)) x2 = 0.0f;
+                        if (unseen(key + 9)) x3 = 0.0f;
                     }
                     uint4 a;
                     a.x = pack_hi_lo(x0, x1, a.y);
