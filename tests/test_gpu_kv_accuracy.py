@@ -158,3 +158,22 @@ def test_long_sums_of_whole_units(backend, width, heads, group, length):
         k, v = kv_oracle.stored(k, enc.Q8_0), kv_oracle.stored(v, enc.Q4_0)
         for i in (0, 301, 591):
             assert rel_l2(got[i:i + 1], kv_oracle.attention(q[i:i + 1], k, v, length - rows + i, group)) <= 1e-5, i
+
+
+@pytest.mark.parametrize("width,length", [(32, 2000000), (96, 400001), (512, 60001)])
+def test_long_sums_of_other_widths(backend, width, length):
+    """A warp sums all positions of a row, whose values have one sign."""
+    b = backend
+    shape = KvCache(1, (length + 15) // 16 * 16, 1, width, enc.Q8_0, enc.Q4_0)
+    rng = np.random.default_rng(width)
+    k, v = (rng.standard_normal((length, 1, width), dtype=np.float32) for _ in range(2))
+    v += 3
+    q = rng.standard_normal((2, 2, width), dtype=np.float32) * np.float32(0.3)
+    with Held(b) as held:
+        cache = held.new(shape.bytes)
+        for at in range(0, length, 1 << 20):  # (what a call takes)
+            n = min(1 << 20, length - at)
+            write(b, held, cache, shape, [(0, at, n)], n, k[at:at + n], v[at:at + n])
+        got = attend(b, held, cache, shape, [(0, length - 2, 2)], 2, q, 2)
+        want = kv_oracle.attention(q, kv_oracle.stored(k, enc.Q8_0), kv_oracle.stored(v, enc.Q4_0), length - 2, 2)
+        assert rel_l2(got, want) <= 1e-5
