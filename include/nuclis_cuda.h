@@ -371,7 +371,8 @@ int nu_cuda_kv_read(nu_cuda *h, const nu_buffer *buffer, const nu_kv_cache *cach
  * Queries are F32, [heads][width] contiguous within a row, strides in elements; scale 0 stands for 1 / sqrt(width), any other is positive and at
  * most 2e38.
  * `out_dtype` NU_F32 gives the result in F32 accuracy for any number of rows; NU_BF16 rounds it to BF16 (what `matmul` takes as
- * its input), and may use 16-bit operands in the products where a call has many rows. */
+ * its input), and may use 16-bit operands in the products where a call has many rows. Widths 64, 128 and 256 have kernels of their own; the others take
+ * some hundred times as long. */
 typedef struct nu_attention {
     uint64_t heads, q_stride, out_stride;
     uint32_t out_dtype, window;

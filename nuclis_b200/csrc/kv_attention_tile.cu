@@ -23,7 +23,7 @@
 // Bound by the work on both sides of the tensor core, not by memory: at width 256 a step of 64 keys costs the decoding warps more than its
 // products take; at width 128 a softmax warp spends 3,300 cycles on 128 keys, of which the exponentials are a third and reading S from
 // tensor memory twice most of the rest (its 128 columns do not fit in registers beside eight decoding warps). Measured: 387 rows
-// of 20 heads on 4 (width 256) at position 24,100 267 us, 709 TFLOP/s; a prompt of 2,048 rows, 40 heads on 8 of width 128, 113 us, 379 TFLOP/s over
+// of 20 heads on 4 (width 256) at position 24,100 271 us, 700 TFLOP/s; a prompt of 2,048 rows, 40 heads on 8 of width 128, 111 us, 388 TFLOP/s over
 // the causal half.
 //
 // Every wait is bounded: a thread whose wait runs out raises the block's flag, all waits then fall through, and the block

@@ -14,7 +14,7 @@
 // The rounds of 4096 values of all rows are laid end to end and every block takes the same number of them, so that all end
 // together; a row that several blocks share is joined by the one that arrives last, in block order.
 //
-// Bound by memory where there are many rows: 509 rows of 248,320 106 us, 4.8 TB/s, 74 % of a copy (127 us before
+// Bound by memory where there are many rows: 509 rows of 248,320 107 us, 4.7 TB/s, 73 % of a copy (127 us before
 // the equal shares and with a longer round, 111 with a bar of each warp's own instead of a shared one). One row of 248,320 is 61 blocks of one round, the ranking and the join: 16.6 us.
 #include "kernels.hpp"
 #include "launch.cuh"
