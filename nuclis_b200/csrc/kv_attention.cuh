@@ -24,7 +24,7 @@ struct AttentionParams {
     bool bf16;
     float scale;     // times log2(e)
     uint32_t window; // 0: none
-    float *partials;      // [block][2][rows * (width + 2)], and behind them the few-row kernel's sums (Split::FOLDED a block)
+    float *partials;      // [block][2][rows * (width + 2)], and behind them the sums of long units ([block][FOLDED] of the kernel)
     uint32_t *counters;   // one a block, zero between launches
 };
 

@@ -15,7 +15,8 @@
 // Range: a step's keys and values are brought into f16's range by a power of two each (their largest scale's), a row's query
 // by one of its own; the score's factor takes the first and last back, O carries the values'. Where that moves by more than P has room for, O is
 // multiplied by the power of two between them, up or down, so P's bits do not depend on what the values of other steps are. Products are exact and sums F32. Against 64 bits the result is off by
-// its own BF16 rounding and little else (1.7e-3 relative).
+// its own BF16 rounding and little else (1.7e-3 relative). The tensor cores cut a sum off at each product (about 2^-24 of it, always towards zero: 1,500,000 positions in one
+// block were 1.1e-2 off), so over a long cache (`launch`) the softmax warps add O up elsewhere, rounded, every 32,768 positions, and it starts again at zero.
 //
 // A value's scale that is NaN would reach rows that do not see its position (0 * NaN), so it is decoded as zeros and marked, and
 // the rows that do see it write NaN in its block's dimensions.
@@ -28,6 +29,8 @@
 //
 // Every wait is bounded: a thread whose wait runs out raises the block's flag, all waits then fall through, and the block
 // ends as ever with the status word raised.
+#include <algorithm>
+
 #include "kv_attention.cuh"
 #include "launch.cuh"
 
@@ -54,7 +57,9 @@ struct Tile {
     // tensor memory columns
     static constexpr int S_COLS = KT, O_COL = 2 * KT;
     static constexpr int PARTIAL = ROWS * (W + 2);
-    static_assert(SCRATCH_SMS * 2 * PARTIAL <= SCRATCH_FLOATS && SCRATCH_SMS <= SCRATCH_COUNTERS, "the handle's scratch");
+    static constexpr int FOLD = 32768 / KT;                        // steps that O sums at most
+    static constexpr int FOLDED = 256 * (W / (QT == 2 ? 1 : 2) + 2);  // floats of a block's sums behind all blocks' partial results: a thread's columns of its row, m and exponent
+    static_assert(SCRATCH_SMS * (2 * PARTIAL + FOLDED) <= SCRATCH_FLOATS && SCRATCH_SMS <= SCRATCH_COUNTERS, "the handle's scratch");
     // P is kept 2^P_UP above the probabilities (at most 2^8 before a maximum moves), so that it ends below 2^15. O carries the exponent of a
     // step's values; a step whose values' lies up to SPREAD below takes P down by that (a probability of one keeps 11 bits down to 2^-14, so a SPREAD of
     // 12 leaves those of 2^-9 all of theirs), any other moves O's exponent to its own, up or down. O is at most 2^31 positions of 2^15 times a value
@@ -183,7 +188,8 @@ __device__ __forceinline__ uint32_t swizzled(uint32_t rows, uint32_t row, uint32
 // Two codes with their sign, exact in f16, times their scales: a value is rounded once.
 __device__ __forceinline__ uint32_t value2(uint32_t codes, uint32_t d) { return h2(__hmul2(as_h2(codes), as_h2(d))); }
 
-template <int W, bool K8, bool V8>
+// LONG: O is added up elsewhere every FOLD steps.
+template <int W, bool K8, bool V8, bool LONG>
 __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const __grid_constant__ AttentionParams p) {
     using T = Tile<W, K8, V8>;
     constexpr int QT = T::QT, ROWS = T::ROWS, KT = T::KT, NB = T::NB;
@@ -319,7 +325,19 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
             int big = 0;            // exponent that O carries
             uint32_t nan_blocks = 0;
 
-            for (uint32_t i = 0; i < sg.n; ++i, ++step) {
+            // the sums of O of earlier steps ([column][thread]), of a maximum and an exponent of then
+            auto sums_so_far = [&]() {
+                uint32_t thread = threadIdx.x;
+                asm volatile("" : "+r"(thread));  // (found anew each time: the loop has no registers to keep it in)
+                return p.partials + (size_t)gridDim.x * 2 * T::PARTIAL + (size_t)blockIdx.x * T::FOLDED + thread;
+            };
+            auto weight_of_sums = [&]() {
+                const float then = sums_so_far()[OCOLS * 256];
+                return then == -INFINITY ? 0.0f : exp2_approx(then - m) * power_of_two(__float_as_int(sums_so_far()[OCOLS * 256 + 256]) - big);
+            };
+
+            for (uint32_t i = 0, upto = T::FOLD;; upto += T::FOLD) {
+            for (const uint32_t end = LONG ? min(upto, sg.n) : sg.n; i < end; ++i, ++step) {
                 const uint32_t buffer = QT == 2 ? q : step & 1u, ring = step & 3u;
                 const uint32_t key0 = (sg.first + sg.skip + i) * KT + (QT == 1 ? group * COLS : 0);
                 const bool edge = key0 < all_low || key0 + COLS - 1 > first_pos;
@@ -451,6 +469,27 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(P_FULL + q));
             }
+                if (!LONG || i == sg.n) break;
+                // (only its own thread reads what it writes)
+                wait_or_give_up(bar(PV_DONE + q), (step - 1) & 1u, abort_flag);
+                fence_after();
+                const float g = upto == T::FOLD ? 0.0f : weight_of_sums();
+#pragma unroll 1
+                for (int c0 = 0; c0 < OCOLS; c0 += 32) {
+                    uint32_t o[32];
+                    float *to = sums_so_far() + c0 * 256;
+                    tmem_load32(ocol + c0, o);
+                    tmem_load_wait();
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(fmaf(upto == T::FOLD ? 0.0f : to[c * 256], g, __uint_as_float(o[c])));
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) { to[c * 256] = __uint_as_float(o[c]); o[c] = 0u; }
+                    tmem_store32(ocol + c0, o);
+                }
+                sums_so_far()[OCOLS * 256] = m;
+                sums_so_far()[OCOLS * 256 + 256] = __int_as_float(big);
+                tmem_store_wait();  // (the next step's arrival is for these too)
+            }
 
             // ---- the result, or this block's part of it ----
             wait_or_give_up(bar(PV_DONE + q), (step - 1) & 1u, abort_flag);
@@ -467,11 +506,18 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
             const float up = power_of_two(big - T::P_UP) * (whole ? 1.0f / l : 1.0f);
             float *partial = p.partials + ((size_t)blockIdx.x * 2 + (sg.skip == 0)) * T::PARTIAL;  // a unit that starts here goes into the second place
             const uint32_t dim0 = QT == 2 ? 0 : group * OCOLS;
+            const bool folded = LONG && sg.n > (uint32_t)T::FOLD;
+            const float g = folded ? weight_of_sums() : 0.0f;
 #pragma unroll 1
             for (int c0 = 0; c0 < OCOLS; c0 += 32) {
                 uint32_t o[32];
                 tmem_load32(ocol + c0, o);
                 tmem_load_wait();
+                if (folded) {
+                    const float *before = sums_so_far() + c0 * 256;
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(fmaf(before[c * 256], g, __uint_as_float(o[c])));
+                }
                 const bool nan = nan_blocks >> ((dim0 + c0) / 32) & 1u;
 #pragma unroll
                 for (int c = 0; c < 32; ++c) o[c] = nan ? 0x7fffffffu : __float_as_uint(__uint_as_float(o[c]) * up);
@@ -859,13 +905,19 @@ __global__ void __launch_bounds__(Tile<W, K8, V8>::THREADS, 1) tile_kernel(const
 
 template <int W, bool K8, bool V8>
 bool configure() {
-    return cudaFuncSetAttribute(tile_kernel<W, K8, V8>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<W, K8, V8>::BYTES) == cudaSuccess;
+    return cudaFuncSetAttribute(tile_kernel<W, K8, V8, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<W, K8, V8>::BYTES) == cudaSuccess &&
+           cudaFuncSetAttribute(tile_kernel<W, K8, V8, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<W, K8, V8>::BYTES) == cudaSuccess;
 }
 template <int W, bool K8, bool V8>
 int launch(cudaStream_t s, AttentionParams p, int sm_count) {
     using T = Tile<W, K8, V8>;
     p.tiles = (uint32_t)(((uint64_t)p.tokens * p.group + T::ROWS - 1) / T::ROWS);
-    launch_after_previous_smem(tile_kernel<W, K8, V8>, dim3(sm_count), dim3(T::THREADS), T::BYTES, s, p);
+    // What a row sees is at most the cache's capacity, and the window. Sums of values of one sign were up to 4e-4 too small over 100,000 positions (400,000 1.6e-3,
+    // 1,500,000 1.1e-2; with the sums elsewhere 4e-4 over any number), a tenth of BF16's half step, and the loop without them is the faster one (2,048 rows of 40 heads on 8, width 128, at
+    // 100,000 6,275 against 6,345 us, 20 on 4 of width 256 5,510 / 5,555; 1,024 rows at 400,000, width 64, 10,390 / 11,090).
+    const uint64_t capacity = (uint64_t)p.c.granules * KV_GRANULE, seen = p.window ? std::min(capacity, (uint64_t)p.window + T::ROWS) : capacity;
+    if (seen > 1u << 17) launch_after_previous_smem(tile_kernel<W, K8, V8, true>, dim3(sm_count), dim3(T::THREADS), T::BYTES, s, p);
+    else launch_after_previous_smem(tile_kernel<W, K8, V8, false>, dim3(sm_count), dim3(T::THREADS), T::BYTES, s, p);
     return 1;
 }
 #define NU_EVERY(F, W, ...) (k8 ? (v8 ? F<W, true, true>(__VA_ARGS__) : F<W, true, false>(__VA_ARGS__)) : (v8 ? F<W, false, true>(__VA_ARGS__) : F<W, false, false>(__VA_ARGS__)))

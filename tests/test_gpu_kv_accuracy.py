@@ -177,3 +177,48 @@ def test_long_sums_of_other_widths(backend, width, length):
         got = attend(b, held, cache, shape, [(0, length - 2, 2)], 2, q, 2)
         want = kv_oracle.attention(q, kv_oracle.stored(k, enc.Q8_0), kv_oracle.stored(v, enc.Q4_0), length - 2, 2)
         assert rel_l2(got, want) <= 1e-5
+
+
+@pytest.mark.parametrize("venc", [enc.Q8_0, enc.Q4_0])
+@pytest.mark.parametrize("width", [64, 128, 256])
+def test_long_sums_of_many_rows(backend, width, venc):
+    """More units of the many-row kernel than blocks over 24 times the same 65,536 positions, values of one sign: a row counts a position as often as it sees it."""
+    b = backend
+    piece, times, rows = 65536, 24, 20000 if width == 256 else 40000
+    length = piece * times
+    shape = KvCache(1, length, 1, width, enc.Q8_0, venc)
+    rng = np.random.default_rng(width)
+    k, v = (rng.standard_normal((piece, 1, width), dtype=np.float32) for _ in range(2))
+    v += 3
+    q = rng.standard_normal((rows, 1, width), dtype=np.float32) * np.float32(0.3)
+    with Held(b) as held:
+        cache = held.new(shape.bytes)
+        for at in range(times):
+            write(b, held, cache, shape, [(0, at * piece, piece)], piece, k, v)
+        got = attend(b, held, cache, shape, [(0, length - rows, rows)], rows, q, 1, dtype=enc.BF16)
+    k, v = kv_oracle.stored(k, enc.Q8_0)[:, 0], kv_oracle.stored(v, venc)[:, 0]
+    for i in (0, rows // 2 + 1, rows - 1):
+        weight = np.exp(k @ q[i, 0].astype(np.float64) / np.sqrt(width)) * ((length - rows + i - np.arange(piece)) // piece + 1)
+        assert rel_l2(got[i, 0], weight @ v / weight.sum()) <= 2.0 ** -8, i
+
+
+@pytest.mark.parametrize("rows,group,window", [(140, 1, 0), (20000, 2, 270000), (20000, 2, 0)])
+@pytest.mark.parametrize("width", [64, 128, 256])
+def test_many_rows_over_a_long_cache(backend, width, rows, group, window):
+    """Unit normal values, whose sums do not grow, so that a wrong share of any of them shows: units cut into parts, and whole ones under a window."""
+    b = backend
+    length = 400000
+    shape = KvCache(1, length, 1, width, enc.Q8_0, enc.Q8_0)
+    rng = np.random.default_rng(width)
+    k, v = (rng.standard_normal((length, 1, width), dtype=np.float32) for _ in range(2))
+    v[:200000] *= 2  # exponents and, with the keys' growth, maxima that move on the way
+    k *= np.linspace(0.2, 1.5, length, dtype=np.float32)[:, None, None]
+    q = rng.standard_normal((rows, group, width), dtype=np.float32)
+    with Held(b) as held:
+        cache = held.new(shape.bytes)
+        write(b, held, cache, shape, [(0, 0, length)], length, k, v)
+        got = attend(b, held, cache, shape, [(0, length - rows, rows)], rows, q, group, dtype=enc.BF16, window=window)
+    k, v = kv_oracle.stored(k, enc.Q8_0), kv_oracle.stored(v, enc.Q8_0)
+    for i in (0, rows // 2 + 1, rows - 1):
+        want = kv_oracle.attention(q[i:i + 1], k, v, length - rows + i, group, window=window)
+        assert rel_l2(got[i:i + 1], want) <= 2.0 ** -8, i
